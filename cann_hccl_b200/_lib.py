@@ -177,6 +177,11 @@ def lib():
         "HcclB200GemmLaunchCounts": [P(u64), P(u64)],
         "HcclB200AllGatherMatmul": [vp, P(vp), P(vp), P(vp), i32, i32, i32, vp],
         "HcclB200MatmulReduceScatter": [vp, P(vp), P(vp), P(vp), i32, i32, i32, vp],
+        "HcclB200Embedding": [vp, C.c_int, C.c_int64, vp, C.c_int64, C.c_int64, C.c_int64, i32, C.c_int, C.c_float, vp, vp],
+        "HcclB200EmbeddingGrad": [vp, C.c_int, C.c_int64, vp, C.c_int64, C.c_int64, C.c_int64, i32, C.c_int, C.c_float, vp, C.c_int, i32, vp, vp],
+        "HcclB200MoeGate": [vp, C.c_int, C.c_int64, i32, C.c_int64, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp],
+        "HcclB200MoeBalance": [vp, vp, vp, i32, i32, vp, vp],
+        "HcclB200MoeGateGrad": [vp, C.c_int, C.c_int64, i32, C.c_int64, i32, i32, vp, vp, vp, vp, vp, C.c_float, vp, vp],
         "HcclB200GetKernelTrace": [vp, u32, P(u64), C.c_size_t, P(i32)],
         "HcclB200WaitProbe": [vp, u32, C.c_double, vp],
         "HcclB200DescribeStatus": [vp, u32, C.c_char_p, C.c_size_t],
@@ -224,6 +229,9 @@ def lib():
         fn.restype = C.c_int
     L.HcclB200MoeScratchBytes.argtypes = [i32, C.c_int64, i32, i32]
     L.HcclB200MoeScratchBytes.restype = C.c_int64
+    L.HcclB200EmbeddingGradScratchBytes.argtypes = [C.c_int64, C.c_int64, i32]
+    L.HcclB200MoeGateScratchBytes.argtypes = [C.c_int64, i32]
+    L.HcclB200EmbeddingGradScratchBytes.restype = L.HcclB200MoeGateScratchBytes.restype = C.c_int64
     L.HcclGetErrorString.argtypes = [C.c_int]
     L.HcclGetErrorString.restype = C.c_char_p
     L.HcclB200GetLastError.argtypes = []

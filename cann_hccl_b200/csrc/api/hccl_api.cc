@@ -22,6 +22,8 @@
 #include "health/fault_inject.h"
 #include "kernels/fused/gemm_local.h"
 #include "kernels/moe_a2a.h"
+#include "kernels/moe_gate.h"
+#include "kernels/vocab_embed.h"
 
 using namespace hcclb;
 
@@ -755,6 +757,107 @@ HcclResult HcclB200MoeCombineLocal(HcclComm comm, const HcclB200MoeLayer *layer,
     CHK_RET(moe_layer(c, layer, "HcclB200MoeCombineLocal", {rows, out}, {topkIdx, gates}, &l));
     CHK_RET(c->begin_launches(1));
     return moe_local_combine(l, rows, (const int32_t *const *)topkIdx, (const float *const *)gates, out, stream);
+}
+// Operands of the embedding and the router: a float type, addresses and strides on element boundaries.
+static HcclResult check_float(HcclDataType t, const char *api)
+{
+    CHK_RET_LOG(t != HCCL_DATA_TYPE_FP32 && t != HCCL_DATA_TYPE_FP16 && t != HCCL_DATA_TYPE_BFP16, HCCL_E_NOT_SUPPORT, "%s: data type %d is not FP32, FP16 or BFP16", api, (int)t);
+    return HCCL_SUCCESS;
+}
+static HcclResult check_aligned(std::initializer_list<const void *> ptrs, int bytes, const char *api)
+{
+    uintptr_t bits = 0;
+    for (const void *p : ptrs) bits |= (uintptr_t)p;
+    CHK_RET_LOG(bits & (uintptr_t)(bytes - 1), HCCL_E_PARA, "%s: an address is not a multiple of %d bytes", api, bytes);
+    return HCCL_SUCCESS;
+}
+static HcclResult check_embed(const void *ids, HcclDataType idType, int64_t tokens, const void *rows, int64_t stride, int64_t vocab, int64_t first,
+                              int32_t hidden, HcclDataType type, const void *out, const char *api, EmbedTable *t, EmbedIds *i)
+{
+    CHK_RET_LOG(idType != HCCL_DATA_TYPE_INT32 && idType != HCCL_DATA_TYPE_INT64, HCCL_E_NOT_SUPPORT, "%s: ids of type %d are not INT32 or INT64", api, (int)idType);
+    CHK_RET(check_float(type, api));
+    CHK_RET_LOG(tokens < 0 || tokens > INT32_MAX || vocab < 1 || vocab >= INT32_MAX || hidden < 1 || first < 0 || stride < hidden, HCCL_E_PARA,
+                "%s: %lld tokens, vocabulary of %lld from %lld, rows of %d, stride %lld", api, (long long)tokens, (long long)vocab, (long long)first,
+                hidden, (long long)stride);
+    CHK_RET_LOG(!out || (tokens > 0 && (!ids || !rows)), HCCL_E_PTR, "[EI0003] %s: null pointer", api);
+    CHK_RET(check_aligned({ids}, dtype_size(idType), api));
+    CHK_RET(check_aligned({rows, out}, dtype_size(type), api));
+    *t = EmbedTable{vocab, first, hidden, type};
+    *i = EmbedIds{ids, idType == HCCL_DATA_TYPE_INT64, tokens};
+    return HCCL_SUCCESS;
+}
+HcclResult HcclB200Embedding(const void *ids, HcclDataType idType, int64_t tokens, const void *weights, int64_t weightStride, int64_t vocab, int64_t firstId,
+                             int32_t hidden, HcclDataType dataType, float scale, void *out, aclrtStream stream)
+{
+    EmbedTable t;
+    EmbedIds i;
+    if (!tokens) return HCCL_SUCCESS;
+    CHK_RET(check_embed(ids, idType, tokens, weights, weightStride, vocab, firstId, hidden, dataType, out, "HcclB200Embedding", &t, &i));
+    return embed_lookup(t, i, weights, weightStride, scale, out, stream);
+}
+int64_t HcclB200EmbeddingGradScratchBytes(int64_t tokens, int64_t vocab, int32_t hidden)
+{
+    return tokens < 0 || tokens > INT32_MAX || vocab < 1 || vocab >= INT32_MAX || hidden < 1 ? -1 : embed_grad_scratch_bytes(tokens, vocab, hidden);
+}
+HcclResult HcclB200EmbeddingGrad(const void *ids, HcclDataType idType, int64_t tokens, const void *grad, int64_t gradStride, int64_t vocab, int64_t firstId,
+                                 int32_t hidden, HcclDataType dataType, float scale, void *out, HcclDataType outType, int32_t accumulate, void *scratch,
+                                 aclrtStream stream)
+{
+    EmbedTable t;
+    EmbedIds i;
+    CHK_RET(check_embed(ids, idType, tokens, grad, gradStride, vocab, firstId, hidden, dataType, out, "HcclB200EmbeddingGrad", &t, &i));
+    CHK_RET_LOG(outType != (accumulate ? HCCL_DATA_TYPE_FP32 : dataType), HCCL_E_NOT_SUPPORT, "HcclB200EmbeddingGrad: out has the type of grad, or FP32 where it is added to");
+    CHK_RET_LOG(!scratch, HCCL_E_PTR, "[EI0003] HcclB200EmbeddingGrad: null pointer");
+    CHK_RET(check_aligned({scratch}, 16, "HcclB200EmbeddingGrad"));
+    CHK_RET(check_aligned({out}, dtype_size(outType), "HcclB200EmbeddingGrad"));
+    return embed_grad(t, i, grad, gradStride, scale, out, accumulate != 0, scratch, stream);
+}
+static HcclResult check_gate(const void *logits, HcclDataType type, int64_t tokens, int32_t nExperts, int64_t stride, int32_t topk, int32_t normalize,
+                             std::initializer_list<const void *> words, std::initializer_list<const void *> per_token, const char *api, GateShape *s)
+{
+    CHK_RET(check_float(type, api));
+    CHK_RET_LOG(nExperts > kGateMaxExperts || topk > kGateMaxTopk, HCCL_E_NOT_SUPPORT, "%s: at most %d experts and top %d (got %d, %d)", api, kGateMaxExperts,
+                kGateMaxTopk, nExperts, topk);
+    CHK_RET_LOG(tokens < 0 || tokens > INT32_MAX || nExperts < 1 || topk < 1 || topk > nExperts || stride < nExperts, HCCL_E_PARA,
+                "%s: %lld tokens, %d experts, top %d, stride %lld", api, (long long)tokens, nExperts, topk, (long long)stride);
+    bool null = tokens > 0 && !logits;
+    for (const void *p : words) null = null || !p;
+    for (const void *p : per_token) null = null || (tokens > 0 && !p);
+    CHK_RET_LOG(null, HCCL_E_PTR, "[EI0003] %s: null pointer", api);
+    CHK_RET(check_aligned({logits}, dtype_size(type), api));
+    CHK_RET(check_aligned(words, 4, api));
+    CHK_RET(check_aligned(per_token, dtype_size(type), api));
+    *s = GateShape{tokens, nExperts, topk, type, stride, normalize != 0};
+    return HCCL_SUCCESS;
+}
+int64_t HcclB200MoeGateScratchBytes(int64_t tokens, int32_t nExperts)
+{
+    return tokens < 0 || nExperts < 1 || nExperts > kGateMaxExperts ? -1 : moe_gate_scratch_bytes(tokens, nExperts);
+}
+HcclResult HcclB200MoeGate(const void *logits, HcclDataType dataType, int64_t tokens, int32_t nExperts, int64_t stride, int32_t topk, int32_t normalize,
+                           const uint8_t *mask, int32_t *idx, float *gates, int32_t *counts, float *probSum, int32_t *routed, float *balance, void *scratch,
+                           aclrtStream stream)
+{
+    GateShape s;
+    CHK_RET(check_gate(logits, dataType, tokens, nExperts, stride, topk, normalize, {counts, probSum, routed, balance, scratch}, {idx, gates}, "HcclB200MoeGate", &s));
+    CHK_RET(check_aligned({idx, gates}, 4, "HcclB200MoeGate"));
+    return moe_gate(s, logits, mask, idx, gates, counts, probSum, routed, balance, scratch, stream);
+}
+HcclResult HcclB200MoeBalance(const int32_t *counts, const float *probSum, const int32_t *routed, int32_t nExperts, int32_t topk, float *balance,
+                              aclrtStream stream)
+{
+    GateShape s;
+    CHK_RET(check_gate(nullptr, HCCL_DATA_TYPE_FP32, 0, nExperts, nExperts, topk, 0, {counts, probSum, routed, balance}, {}, "HcclB200MoeBalance", &s));
+    return moe_balance(counts, probSum, routed, nExperts, topk, balance, stream);
+}
+HcclResult HcclB200MoeGateGrad(const void *logits, HcclDataType dataType, int64_t tokens, int32_t nExperts, int64_t stride, int32_t topk, int32_t normalize,
+                               const uint8_t *mask, const int32_t *idx, const float *dGates, const int32_t *counts, const int32_t *routed, float dBalance,
+                               void *dLogits, aclrtStream stream)
+{
+    GateShape s;
+    CHK_RET(check_gate(logits, dataType, tokens, nExperts, stride, topk, normalize, {counts, routed}, {idx, dLogits}, "HcclB200MoeGateGrad", &s));
+    CHK_RET(check_aligned({idx, dGates}, 4, "HcclB200MoeGateGrad"));
+    return moe_gate_grad(s, logits, idx, dGates, counts, routed, mask, dBalance, dLogits, stream);
 }
 static HcclResult check_act(int32_t act, const char *api)
 {

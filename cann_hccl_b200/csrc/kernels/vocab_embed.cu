@@ -1,0 +1,636 @@
+// Token embedding:  out[t] = scale * W[id_t - first], zeros for ids outside the table, and its gradient
+// dW[v] = scale * sum over the tokens with id_t = first + v of dY[t].
+//
+// Lookup: a warp takes one stretch of one row (128 bytes per lane in flight), so that a decode batch spreads over the GPU and a
+// prefill batch keeps every SM's loads in flight.  Bound: HBM.
+//
+// Gradient: the tokens are sorted by id (stable, so that the sums have one order whatever ran before), then a CTA walks a tile of
+// the sorted list, keeps the running row in fp32 registers and writes it when the id changes: every row of dY is read once and
+// every row of the table written once, without atomics.  A run of one id that crosses tiles leaves fp32 pieces, which a second
+// launch adds in order, so that a token that makes up a large part of a text is summed by many CTAs.  Rows of the table without a
+// token are zeroed by the same launch as the sums.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <algorithm>
+#include <cstring>
+#include "common/base.h"
+#include "common/log.h"
+#include "kernels/pdl.cuh"
+#include "kernels/vocab_embed.h"
+
+namespace hcclb {
+
+namespace {
+
+// ---------------------------------------------------------------------------------------------------- vectors of B bytes
+template <int B> struct Bytes;
+template <> struct Bytes<32> { uint32_t w[8]; };
+template <> struct Bytes<16> { uint32_t w[4]; };
+template <> struct Bytes<4> { uint32_t w[1]; };
+template <> struct Bytes<2> { uint16_t h; };
+
+__device__ __forceinline__ void ld(Bytes<32> &v, const void *p)
+{
+    asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]), "=r"(v.w[4]), "=r"(v.w[5]), "=r"(v.w[6]), "=r"(v.w[7]) : "l"(p) : "memory");
+}
+__device__ __forceinline__ void ld(Bytes<16> &v, const void *p)
+{
+    const uint4 u = *(const uint4 *)p;
+    v.w[0] = u.x; v.w[1] = u.y; v.w[2] = u.z; v.w[3] = u.w;
+}
+__device__ __forceinline__ void ld(Bytes<4> &v, const void *p) { v.w[0] = *(const uint32_t *)p; }
+__device__ __forceinline__ void ld(Bytes<2> &v, const void *p) { v.h = *(const uint16_t *)p; }
+__device__ __forceinline__ void st(void *p, const Bytes<32> &v)
+{
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 ::"l"(p), "r"(v.w[0]), "r"(v.w[1]), "r"(v.w[2]), "r"(v.w[3]), "r"(v.w[4]), "r"(v.w[5]), "r"(v.w[6]), "r"(v.w[7]) : "memory");
+}
+__device__ __forceinline__ void st(void *p, const Bytes<16> &v) { *(uint4 *)p = make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]); }
+__device__ __forceinline__ void st(void *p, const Bytes<4> &v) { *(uint32_t *)p = v.w[0]; }
+__device__ __forceinline__ void st(void *p, const Bytes<2> &v) { *(uint16_t *)p = v.h; }
+
+__device__ __forceinline__ float to_f(float x) { return x; }
+__device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <class T> __device__ __forceinline__ T from_f(float x);
+template <> __device__ __forceinline__ float from_f<float>(float x) { return x; }
+template <> __device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+template <class T, int B> __device__ __forceinline__ void unpack(const Bytes<B> &v, float (&f)[B / sizeof(T)])
+{
+    T e[B / sizeof(T)];
+    memcpy(e, &v, B);
+#pragma unroll
+    for (int i = 0; i < (int)(B / sizeof(T)); ++i) f[i] = to_f(e[i]);
+}
+template <class T, int B> __device__ __forceinline__ Bytes<B> pack(const float (&f)[B / sizeof(T)], float scale)
+{
+    T e[B / sizeof(T)];
+#pragma unroll
+    for (int i = 0; i < (int)(B / sizeof(T)); ++i) e[i] = from_f<T>(f[i] * scale);
+    Bytes<B> v;
+    memcpy(&v, e, B);
+    return v;
+}
+
+__device__ __forceinline__ int64_t id_at(const void *ids, int wide, int64_t t) { return wide ? ((const int64_t *)ids)[t] : (int64_t)((const int32_t *)ids)[t]; }
+// Row of the table that id stands for, -1 outside it (no overflow for any id: the difference is taken unsigned).
+__device__ __forceinline__ int64_t row_of(int64_t id, int64_t first, int64_t vocab)
+{
+    const uint64_t r = (uint64_t)id - (uint64_t)first;
+    return r < (uint64_t)vocab ? (int64_t)r : -1;
+}
+
+// ---------------------------------------------------------------------------------------------------- lookup
+struct LookupArgs {
+    const void *ids;
+    const uint8_t *w;
+    uint8_t *out;
+    int64_t tokens, units, vocab, first, stride;  // units: stretches of all rows; stride: bytes between rows of w
+    int wide, nvec, nseg;
+    float scale;
+};
+constexpr int kLookupThreads = 128;
+template <int B> constexpr int kLookupVecs = B >= 16 ? 128 / B : 8;  // vectors of a lane
+
+template <class T, int B, bool kScale>
+__global__ void __launch_bounds__(kLookupThreads) embed_lookup_kernel(const __grid_constant__ LookupArgs a)
+{
+    constexpr int U = kLookupVecs<B>;
+    pdl_trigger();
+    const int lane = threadIdx.x & 31;
+    const int64_t unit = (int64_t)blockIdx.x * (kLookupThreads / 32) + threadIdx.x / 32;
+    if (unit >= a.units) return;
+    const int64_t t = a.nseg == 1 ? unit : unit / a.nseg;
+    const int v0 = (int)(unit - t * a.nseg) * (32 * U) + lane;
+    pdl_wait();
+    const int64_t row = row_of(id_at(a.ids, a.wide, t), a.first, a.vocab);
+    Bytes<B> x[U];
+    memset(x, 0, sizeof(x));
+    if (row >= 0) {
+        const uint8_t *src = a.w + row * a.stride;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (v0 + 32 * u < a.nvec) ld(x[u], src + (int64_t)(v0 + 32 * u) * B);
+    }
+    uint8_t *dst = a.out + t * a.nvec * B;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (v0 + 32 * u < a.nvec) {
+            if (kScale) {
+                float f[B / sizeof(T)];
+                unpack<T, B>(x[u], f);
+                x[u] = pack<T, B>(f, a.scale);
+            }
+            st(dst + (int64_t)(v0 + 32 * u) * B, x[u]);
+        }
+}
+
+// ---------------------------------------------------------------------------------------------------- stable sort by id
+// Radix sort from the least significant digit.  A pair is (row of the table, token); rows outside the table sort behind all
+// others as `vocab`.  A warp takes consecutive stretches of 32 pairs; __match_any_sync gives the lanes of one digit, the
+// warp's counters in shared memory the earlier stretches, so equal digits keep their order.
+constexpr int kDigitBits = 9, kBins = 1 << kDigitBits;
+constexpr int kSortItems = 8;
+constexpr int kOneThreads = 1024, kTileThreads = 256;
+constexpr int kOneMost = kOneThreads * kSortItems;    // tokens that one CTA sorts
+constexpr int kTile = kTileThreads * kSortItems;
+
+struct SortArgs {
+    const void *ids;                 // first pass
+    int wide;
+    int64_t vocab, first;
+    const uint2 *in;                 // later passes
+    uint2 *out;
+    int32_t *hist;                   // [tile][bin]
+    int64_t tokens;
+    int tiles, shift, bits, passes, digit;
+};
+
+// Ranks of a warp's pairs within (warp, digit); counts[warp][bin] end up holding the warp's pairs of each digit.
+__device__ __forceinline__ void warp_ranks(const uint32_t (&key)[kSortItems], int items, int shift, uint32_t mask, int32_t *counts, int (&rank)[kSortItems])
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int32_t *mine = counts + warp * kBins;
+#pragma unroll
+    for (int i = 0; i < kSortItems; ++i) {
+        if (i >= items) break;
+        const uint32_t d = (key[i] >> shift) & mask;
+        const uint32_t peers = __match_any_sync(0xffffffffu, d);
+        const int before = mine[d], below = __popc(peers & ((1u << lane) - 1));
+        __syncwarp();
+        if (below == 0) mine[d] = before + __popc(peers);
+        __syncwarp();
+        rank[i] = before + below;
+    }
+}
+
+// counts[warp][bin] -> pairs of the bin in earlier warps; returns the bin's total for thread `bin`.
+template <int WARPS> __device__ __forceinline__ int warp_prefix(int32_t *counts, int bin)
+{
+    int t = 0;
+#pragma unroll 8
+    for (int w = 0; w < WARPS; ++w) {
+        const int n = counts[w * kBins + bin];
+        counts[w * kBins + bin] = t;
+        t += n;
+    }
+    return t;
+}
+
+// Exclusive prefix over the bins; thread i of the first kBins / N threads holds N consecutive bins' totals.
+template <int N> __device__ __forceinline__ void bins_prefix(int (&t)[N], int32_t *s_warp)
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int own = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) { const int n = t[i]; t[i] = own; own += n; }
+    int v = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int w = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += w;
+    }
+    if (lane == 31) s_warp[warp] = v;
+    __syncthreads();
+    int base = v - own;
+    for (int w = 0; w < warp; ++w) base += s_warp[w];
+#pragma unroll
+    for (int i = 0; i < N; ++i) t[i] += base;
+}
+
+constexpr size_t kOneSmem = (size_t)(kOneThreads / 32) * kBins * 4 + kBins * 4 + (size_t)kOneMost * 8;
+
+// Up to kOneMost tokens: all passes in one CTA, pairs in registers, exchanged through shared memory.
+__global__ void __launch_bounds__(kOneThreads) embed_sort_one_kernel(const __grid_constant__ SortArgs a)
+{
+    extern __shared__ int32_t sh[];
+    __shared__ int32_t s_warp[kOneThreads / 32];
+    constexpr int W = kOneThreads / 32;
+    int32_t *counts = sh, *base = counts + W * kBins;
+    uint2 *pairs = (uint2 *)(base + kBins);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int n = (int)a.tokens, items = (n + kOneThreads - 1) / kOneThreads, at = warp * items * 32 + lane;
+    pdl_trigger();
+    pdl_wait();
+    uint32_t key[kSortItems], pos[kSortItems];
+#pragma unroll
+    for (int i = 0; i < kSortItems; ++i) {
+        const int t = at + i * 32;
+        pos[i] = (uint32_t)t;
+        key[i] = 0xffffffffu;  // behind everything: pairs that pad the last warps
+        if (i < items && t < n) {
+            const int64_t r = row_of(id_at(a.ids, a.wide, t), a.first, a.vocab);
+            key[i] = r >= 0 ? (uint32_t)r : (uint32_t)a.vocab;
+        }
+    }
+    for (int pass = 0; pass < a.passes; ++pass) {
+        const int shift = pass * a.digit;
+        const uint32_t mask = (1u << a.digit) - 1;
+        for (int i = threadIdx.x; i < W * kBins; i += kOneThreads) counts[i] = 0;
+        __syncthreads();
+        int rank[kSortItems];
+        warp_ranks(key, items, shift, mask, counts, rank);
+        __syncthreads();
+        int t[1] = {threadIdx.x < kBins ? warp_prefix<W>(counts, threadIdx.x) : 0};
+        bins_prefix<1>(t, s_warp);
+        if (threadIdx.x < kBins) base[threadIdx.x] = t[0];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kSortItems; ++i) {
+            if (i >= items) break;
+            const uint32_t d = (key[i] >> shift) & mask;
+            pairs[base[d] + counts[warp * kBins + d] + rank[i]] = make_uint2(key[i], pos[i]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kSortItems; ++i) {
+            if (i >= items) break;
+            const uint2 p = pairs[at + i * 32];
+            key[i] = p.x; pos[i] = p.y;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kSortItems; ++i)
+        if (i < items && at + i * 32 < n) a.out[at + i * 32] = make_uint2(key[i], pos[i]);
+}
+
+__device__ __forceinline__ void load_tile(const SortArgs &a, int64_t tile, uint32_t (&key)[kSortItems], uint32_t (&pos)[kSortItems])
+{
+    const int64_t t0 = tile * kTile + (threadIdx.x >> 5) * (32 * kSortItems) + (threadIdx.x & 31);
+#pragma unroll
+    for (int i = 0; i < kSortItems; ++i) {
+        const int64_t t = t0 + i * 32;
+        key[i] = 0xffffffffu;
+        pos[i] = 0;
+        if (t < a.tokens) {
+            if (a.in) {
+                const uint2 p = a.in[t];
+                key[i] = p.x; pos[i] = p.y;
+            } else {
+                const int64_t r = row_of(id_at(a.ids, a.wide, t), a.first, a.vocab);
+                key[i] = r >= 0 ? (uint32_t)r : (uint32_t)a.vocab;
+                pos[i] = (uint32_t)t;
+            }
+        }
+    }
+}
+
+__global__ void __launch_bounds__(kTileThreads) embed_sort_hist_kernel(const __grid_constant__ SortArgs a)
+{
+    __shared__ int32_t bins[kBins];
+    for (int i = threadIdx.x; i < kBins; i += kTileThreads) bins[i] = 0;
+    __syncthreads();
+    pdl_trigger();
+    pdl_wait();
+    uint32_t key[kSortItems], pos[kSortItems];
+    load_tile(a, blockIdx.x, key, pos);
+    const int64_t t0 = (int64_t)blockIdx.x * kTile + (threadIdx.x >> 5) * (32 * kSortItems) + (threadIdx.x & 31);
+#pragma unroll
+    for (int i = 0; i < kSortItems; ++i)
+        if (t0 + i * 32 < a.tokens) atomicAdd(&bins[(key[i] >> a.shift) & ((1u << a.digit) - 1)], 1);
+    __syncthreads();
+    for (int i = threadIdx.x; i < kBins; i += kTileThreads) a.hist[(int64_t)blockIdx.x * kBins + i] = bins[i];
+}
+
+__global__ void __launch_bounds__(kTileThreads) embed_sort_scatter_kernel(const __grid_constant__ SortArgs a)
+{
+    constexpr int W = kTileThreads / 32, N = kBins / kTileThreads;
+    __shared__ int32_t counts[W * kBins], base[kBins], s_warp[W];
+    for (int i = threadIdx.x; i < W * kBins; i += kTileThreads) counts[i] = 0;
+    __syncthreads();
+    pdl_trigger();
+    pdl_wait();
+    uint32_t key[kSortItems], pos[kSortItems];
+    load_tile(a, blockIdx.x, key, pos);
+    const uint32_t mask = (1u << a.digit) - 1;
+    int rank[kSortItems];
+    warp_ranks(key, kSortItems, a.shift, mask, counts, rank);
+    // pairs of each bin in earlier tiles, and of all smaller bins in all tiles
+    int before[N], total[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) before[j] = total[j] = 0;
+#pragma unroll 8
+    for (int q = 0; q < a.tiles; ++q)
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int h = a.hist[(int64_t)q * kBins + threadIdx.x * N + j];
+            total[j] += h;
+            before[j] += q < (int)blockIdx.x ? h : 0;
+        }
+    bins_prefix<N>(total, s_warp);  // its barrier puts all warps' counters before warp_prefix
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        base[threadIdx.x * N + j] = total[j] + before[j];
+        warp_prefix<W>(counts, threadIdx.x * N + j);
+    }
+    __syncthreads();
+    const int64_t t0 = (int64_t)blockIdx.x * kTile + (threadIdx.x >> 5) * (32 * kSortItems) + (threadIdx.x & 31);
+#pragma unroll
+    for (int i = 0; i < kSortItems; ++i)
+        if (t0 + i * 32 < a.tokens) {  // pairs that pad the tile are last in it: they displace none of the others
+            const uint32_t d = (key[i] >> a.shift) & mask;
+            a.out[base[d] + counts[(threadIdx.x >> 5) * kBins + d] + rank[i]] = make_uint2(key[i], pos[i]);
+        }
+}
+
+// ---------------------------------------------------------------------------------------------------- sums by row
+struct SumArgs {
+    const uint2 *pairs;              // sorted
+    const uint8_t *dy;
+    void *out;
+    float *pieces;                   // [tile][2][nvec * per]: run from an earlier tile, run that goes on behind the tile
+    int64_t tokens, vocab, stride;   // stride: bytes between rows of dy
+    int64_t tiles, zero_ctas;
+    int rows, nvec, nslice, add;     // rows: tokens of a tile
+    float scale;
+};
+constexpr int kSumThreads = 256, kSumBatch = 4, kZeroRows = 32, kMostRows = 256;
+
+template <class T, int B> __device__ __forceinline__ void put_row(const SumArgs &a, int64_t row, int v, const float (&acc)[B / sizeof(T)])
+{
+    constexpr int N = B / sizeof(T);
+    const int64_t at = (row * a.nvec + v) * N;
+    if (a.add) {
+        float *p = (float *)a.out + at;
+#pragma unroll
+        for (int i = 0; i < N; ++i) p[i] += acc[i] * a.scale;
+    } else
+        st((T *)a.out + at, pack<T, B>(acc, a.scale));
+}
+
+// First place in the sorted list whose row is not below `row`.
+__device__ __forceinline__ int64_t lower_bound(const uint2 *pairs, int64_t n, uint32_t row)
+{
+    int64_t lo = 0, hi = n;
+    while (lo < hi) {
+        const int64_t mid = (lo + hi) >> 1;
+        if (pairs[mid].x < row) lo = mid + 1; else hi = mid;
+    }
+    return lo;
+}
+
+// grid: tiles x slices of a row, then CTAs that zero kZeroRows rows of the table each where they have no token
+template <class T, int B>
+__global__ void __launch_bounds__(kSumThreads) embed_sum_kernel(const __grid_constant__ SumArgs a)
+{
+    constexpr int N = B / sizeof(T);
+    __shared__ uint2 s_pair[kMostRows];
+    __shared__ uint32_t s_edge[2], s_has;
+    pdl_trigger();
+    pdl_wait();
+    const int64_t sums = a.tiles * a.nslice;
+    if ((int64_t)blockIdx.x >= sums) {
+        const int64_t r0 = ((int64_t)blockIdx.x - sums) * kZeroRows;
+        if (threadIdx.x < 32) {
+            const int64_t r = r0 + threadIdx.x;
+            bool has = true;
+            if (r < a.vocab) {
+                const int64_t at = lower_bound(a.pairs, a.tokens, (uint32_t)r);
+                has = at < a.tokens && a.pairs[at].x == (uint32_t)r;
+            }
+            const uint32_t mask = __ballot_sync(0xffffffffu, has);
+            if (threadIdx.x == 0) s_has = mask;
+        }
+        __syncthreads();
+        Bytes<B> zero;
+        memset(&zero, 0, sizeof(zero));
+        for (int i = 0; i < kZeroRows; ++i)
+            if (!(s_has >> i & 1)) {
+                uint8_t *p = (uint8_t *)a.out + (r0 + i) * a.nvec * B;
+                for (int v = threadIdx.x; v < a.nvec; v += blockDim.x) st(p + (int64_t)v * B, zero);
+            }
+        return;
+    }
+    const int64_t tile = blockIdx.x / a.nslice, t0 = tile * a.rows;
+    const int v = (int)(blockIdx.x - tile * a.nslice) * (int)blockDim.x + threadIdx.x, n = (int)min((int64_t)a.rows, a.tokens - t0);
+    for (int i = threadIdx.x; i < n; i += blockDim.x) s_pair[i] = a.pairs[t0 + i];
+    if (threadIdx.x == 0) {
+        s_edge[0] = t0 > 0 ? a.pairs[t0 - 1].x : 0xffffffffu;
+        s_edge[1] = t0 + n < a.tokens ? a.pairs[t0 + n].x : 0xffffffffu;
+    }
+    __syncthreads();
+    if (v >= a.nvec) return;
+    float acc[N];
+    uint32_t cur = s_pair[0].x;
+    bool head = cur == s_edge[0];  // the run in hand came in from an earlier tile
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = 0.f;
+    const uint8_t *src = a.dy + (int64_t)v * B;
+    for (int i0 = 0; i0 < n; i0 += kSumBatch) {
+        Bytes<B> x[kSumBatch];
+#pragma unroll
+        for (int j = 0; j < kSumBatch; ++j)
+            if (i0 + j < n && s_pair[i0 + j].x < (uint32_t)a.vocab) ld(x[j], src + (int64_t)s_pair[i0 + j].y * a.stride);
+#pragma unroll
+        for (int j = 0; j < kSumBatch; ++j) {
+            if (i0 + j >= n) break;
+            const uint32_t key = s_pair[i0 + j].x;
+            if (key != cur) {
+                if (head) {
+                    float *p = a.pieces + ((tile * 2) * a.nvec + v) * N;
+#pragma unroll
+                    for (int i = 0; i < N; ++i) p[i] = acc[i];
+                } else
+                    put_row<T, B>(a, cur, v, acc);
+                cur = key;
+                head = false;
+#pragma unroll
+                for (int i = 0; i < N; ++i) acc[i] = 0.f;
+            }
+            if (key >= (uint32_t)a.vocab) return;  // outside the table: nothing but such tokens follows
+            float f[N];
+            unpack<T, B>(x[j], f);
+#pragma unroll
+            for (int i = 0; i < N; ++i) acc[i] += f[i];
+        }
+    }
+    const bool tail = cur == s_edge[1];
+    if (head || tail) {
+        float *p = a.pieces + ((tile * 2 + (head ? 0 : 1)) * a.nvec + v) * N;
+#pragma unroll
+        for (int i = 0; i < N; ++i) p[i] = acc[i];
+    } else
+        put_row<T, B>(a, cur, v, acc);
+}
+
+// The runs that begin in a tile and go on behind it: their pieces, in order.
+template <class T, int B>
+__global__ void __launch_bounds__(kSumThreads) embed_join_kernel(const __grid_constant__ SumArgs a)
+{
+    constexpr int N = B / sizeof(T);
+    pdl_trigger();
+    const int64_t tile = blockIdx.x / a.nslice, t1 = (tile + 1) * a.rows;  // not the last tile
+    const int v = (int)(blockIdx.x - tile * a.nslice) * (int)blockDim.x + threadIdx.x;
+    pdl_wait();
+    const uint32_t key = a.pairs[t1 - 1].x;
+    if (key >= (uint32_t)a.vocab || a.pairs[t1].x != key || (tile > 0 && a.pairs[tile * a.rows - 1].x == key)) return;
+    const int64_t last = (lower_bound(a.pairs, a.tokens, key + 1) - 1) / a.rows;  // tile in which the run ends
+    if (v >= a.nvec) return;
+    float acc[N];
+    const float *p = a.pieces + ((tile * 2 + 1) * a.nvec + v) * N;
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = p[i];
+    for (int64_t q = tile + 1; q <= last; ++q) {
+        const float *h = a.pieces + (q * 2 * a.nvec + v) * N;
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] += h[i];
+    }
+    put_row<T, B>(a, key, v, acc);
+}
+
+// ---------------------------------------------------------------------------------------------------- launches
+template <class K> HcclResult grid_of(int64_t ctas, K *out, const char *what)
+{
+    CHK_RET_LOG(ctas > 0x7fffffff, HCCL_E_PARA, "%s: too many rows for one launch (%lld CTAs)", what, (long long)ctas);
+    *out = (K)ctas;
+    return HCCL_SUCCESS;
+}
+
+// Widest vector that every row starts on and is a whole number of; `lanes`: narrower ones where a row has fewer vectors than that.
+int vector_bytes(int64_t row_bytes, uintptr_t bits, int size, int lanes)
+{
+    bits |= (uintptr_t)row_bytes;
+    if (row_bytes < 32 * lanes) bits |= 16;
+    if (row_bytes < 16 * lanes) bits |= 4;
+    return bits % 32 == 0 ? 32 : bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : size;
+}
+
+template <class T, int B> HcclResult lookup(LookupArgs &a, int64_t row_bytes, void *stream)
+{
+    a.nvec = (int)(row_bytes / B);
+    a.nseg = (a.nvec + 32 * kLookupVecs<B> - 1) / (32 * kLookupVecs<B>);
+    a.units = a.tokens * a.nseg;
+    unsigned ctas;
+    CHK_RET(grid_of((a.units + kLookupThreads / 32 - 1) / (kLookupThreads / 32), &ctas, "embedding"));
+    const void *fn = a.scale == 1.f ? (const void *)embed_lookup_kernel<T, B, false> : (const void *)embed_lookup_kernel<T, B, true>;
+    return launch_pdl(fn, dim3(ctas), kLookupThreads, 0, &a, stream, "embedding");
+}
+
+template <class T> HcclResult lookup_typed(LookupArgs &a, int64_t hidden, void *stream)
+{
+    const int64_t row = hidden * (int64_t)sizeof(T);
+    switch (vector_bytes(row, (uintptr_t)a.w | (uintptr_t)a.out | (uintptr_t)a.stride, sizeof(T), 1)) {
+        case 32: return lookup<T, 32>(a, row, stream);
+        case 16: return lookup<T, 16>(a, row, stream);
+        case 4: return lookup<T, 4>(a, row, stream);
+        default: return lookup<T, sizeof(T)>(a, row, stream);
+    }
+}
+
+// Tokens of a tile: short tiles for parallelism, longer ones where there are many tokens, so that a run has few pieces.
+int tile_rows(int64_t tokens) { return (int)std::min<int64_t>(kMostRows, std::max<int64_t>(32, (tokens / 1184 + 31) / 32 * 32)); }
+
+struct Scratch { int64_t pairs, spare, hist, pieces, bytes; };
+Scratch scratch_of(int64_t tokens, int32_t hidden)
+{
+    auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
+    Scratch s;
+    const int64_t tiles = (tokens + tile_rows(tokens) - 1) / tile_rows(tokens);
+    s.pairs = 0;
+    s.spare = s.pairs + up(tokens * 8);
+    s.hist = s.spare + (tokens > kOneMost ? up(tokens * 8) : 0);
+    s.pieces = s.hist + (tokens > kOneMost ? up((tokens + kTile - 1) / kTile * kBins * 4) : 0);
+    s.bytes = s.pieces + (tiles > 1 ? up(tiles * 2 * hidden * 4) : 0);
+    return s;
+}
+
+template <class T, int B> HcclResult sum(SumArgs &a, int64_t row_bytes, void *stream)
+{
+    a.nvec = (int)(row_bytes / B);
+    const int threads = std::min(kSumThreads, (a.nvec + 31) / 32 * 32);
+    a.nslice = (a.nvec + threads - 1) / threads;
+    a.zero_ctas = a.add ? 0 : (a.vocab + kZeroRows - 1) / kZeroRows;
+    unsigned ctas;
+    CHK_RET(grid_of(a.tiles * a.nslice + a.zero_ctas, &ctas, "embedding gradient"));
+    if (ctas) CHK_RET(launch_pdl((const void *)embed_sum_kernel<T, B>, dim3(ctas), (unsigned)threads, 0, &a, stream, "embedding gradient"));
+    if (a.tiles > 1)
+        CHK_RET(launch_pdl((const void *)embed_join_kernel<T, B>, dim3((unsigned)((a.tiles - 1) * a.nslice)), (unsigned)threads, 0, &a, stream, "embedding gradient (join)"));
+    return HCCL_SUCCESS;
+}
+
+template <class T> HcclResult sum_typed(SumArgs &a, int64_t hidden, void *stream)
+{
+    const int64_t row = hidden * (int64_t)sizeof(T);
+    switch (vector_bytes(row, (uintptr_t)a.dy | (uintptr_t)a.stride | (a.add ? 0 : (uintptr_t)a.out), sizeof(T), 32)) {
+        case 32: return sum<T, 32>(a, row, stream);
+        case 16: return sum<T, 16>(a, row, stream);
+        case 4: return sum<T, 4>(a, row, stream);
+        default: return sum<T, sizeof(T)>(a, row, stream);
+    }
+}
+
+HcclResult sort_tokens(const EmbedTable &t, const EmbedIds &ids, const Scratch &s, uint8_t *scratch, void *stream, const uint2 **sorted)
+{
+    SortArgs a;
+    memset(&a, 0, sizeof(a));
+    a.ids = ids.ids; a.wide = ids.wide; a.vocab = t.vocab; a.first = t.first; a.tokens = ids.tokens;
+    int bits = 1;
+    while ((t.vocab >> bits) != 0) ++bits;  // rows 0 .. vocab
+    a.passes = (bits + kDigitBits - 1) / kDigitBits;
+    a.digit = (bits + a.passes - 1) / a.passes;
+    uint2 *buf[2] = {(uint2 *)(scratch + s.pairs), (uint2 *)(scratch + s.spare)};
+    if (ids.tokens <= kOneMost) {
+        const cudaError_t e = cudaFuncSetAttribute((const void *)embed_sort_one_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kOneSmem);
+        CHK_RET_LOG(e != cudaSuccess, HCCL_E_RUNTIME, "embedding gradient set-up failed: %s", cudaGetErrorString(e));
+        a.out = buf[0];
+        *sorted = buf[0];
+        return launch_pdl((const void *)embed_sort_one_kernel, dim3(1), kOneThreads, kOneSmem, &a, stream, "embedding gradient (sort)");
+    }
+    a.hist = (int32_t *)(scratch + s.hist);
+    a.tiles = (int)((ids.tokens + kTile - 1) / kTile);
+    for (int pass = 0; pass < a.passes; ++pass) {
+        a.in = pass ? buf[(pass - 1) & 1] : nullptr;
+        a.out = buf[pass & 1];
+        a.shift = pass * a.digit;
+        CHK_RET(launch_pdl((const void *)embed_sort_hist_kernel, dim3((unsigned)a.tiles), kTileThreads, 0, &a, stream, "embedding gradient (histogram)"));
+        CHK_RET(launch_pdl((const void *)embed_sort_scatter_kernel, dim3((unsigned)a.tiles), kTileThreads, 0, &a, stream, "embedding gradient (scatter)"));
+        *sorted = a.out;
+    }
+    return HCCL_SUCCESS;
+}
+
+}  // namespace
+
+HcclResult embed_lookup(const EmbedTable &t, const EmbedIds &ids, const void *weights, int64_t stride, float scale, void *out, void *stream)
+{
+    if (!ids.tokens) return HCCL_SUCCESS;
+    const int size = dtype_size(t.type);
+    LookupArgs a;
+    memset(&a, 0, sizeof(a));
+    a.ids = ids.ids; a.wide = ids.wide; a.tokens = ids.tokens;
+    a.w = (const uint8_t *)weights; a.out = (uint8_t *)out;
+    a.vocab = t.vocab; a.first = t.first; a.stride = stride * size; a.scale = scale;
+    switch (t.type) {
+        case HCCL_DATA_TYPE_FP32: return lookup_typed<float>(a, t.hidden, stream);
+        case HCCL_DATA_TYPE_FP16: return lookup_typed<__half>(a, t.hidden, stream);
+        default: return lookup_typed<__nv_bfloat16>(a, t.hidden, stream);
+    }
+}
+
+int64_t embed_grad_scratch_bytes(int64_t tokens, int64_t vocab, int32_t hidden) { return std::max<int64_t>(256, scratch_of(tokens, hidden).bytes); }
+
+HcclResult embed_grad(const EmbedTable &t, const EmbedIds &ids, const void *grad, int64_t stride, float scale, void *out, bool add, void *scratch,
+                      void *stream)
+{
+    const Scratch s = scratch_of(ids.tokens, t.hidden);
+    SumArgs a;
+    memset(&a, 0, sizeof(a));
+    if (ids.tokens) CHK_RET(sort_tokens(t, ids, s, (uint8_t *)scratch, stream, &a.pairs));
+    a.dy = (const uint8_t *)grad; a.stride = stride * dtype_size(t.type);
+    a.out = out; a.add = add; a.scale = scale;
+    a.tokens = ids.tokens; a.vocab = t.vocab;
+    a.rows = tile_rows(ids.tokens);
+    a.tiles = (ids.tokens + a.rows - 1) / a.rows;
+    a.pieces = (float *)((uint8_t *)scratch + s.pieces);
+    switch (t.type) {
+        case HCCL_DATA_TYPE_FP32: return sum_typed<float>(a, t.hidden, stream);
+        case HCCL_DATA_TYPE_FP16: return sum_typed<__half>(a, t.hidden, stream);
+        default: return sum_typed<__nv_bfloat16>(a, t.hidden, stream);
+    }
+}
+
+}  // namespace hcclb

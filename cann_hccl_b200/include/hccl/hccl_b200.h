@@ -114,6 +114,38 @@ extern HcclResult HcclB200MatmulReduceScatter(HcclComm comm, void *const *inputs
 extern HcclResult HcclB200GemmBf16Act(const void *A, const void *B, void *C, int32_t M, int32_t N, int32_t K, int32_t act, aclrtStream stream);
 extern HcclResult HcclB200AllGatherMatmulAct(HcclComm comm, void *const *xShards, void *const *weights, void *const *outs, int32_t M, int32_t N,
                                              int32_t K, int32_t act, aclrtStream stream);
+/* ---- model-side operators around the tensor-parallel layers and the MoE exchange: embedding, router ----
+ * All of them run on the current device and in stream order, wait for nothing and keep nothing between calls; `scratch` is the
+ * caller's, needs no contents, and belongs to one call at a time. */
+/* Token embedding, out [tokens, hidden] = scale * weights[ids - firstId], zeros for ids outside firstId .. firstId + vocab - 1 (a
+ * rank's shard of the vocabulary: the sum over the ranks is the whole embedding).  ids: INT32 or INT64; dataType of weights and out:
+ * FP32, FP16 or BFP16; weightStride: elements between rows.  scale is applied in fp32, 1 copies the bits. */
+extern HcclResult HcclB200Embedding(const void *ids, HcclDataType idType, int64_t tokens, const void *weights, int64_t weightStride, int64_t vocab,
+                                    int64_t firstId, int32_t hidden, HcclDataType dataType, float scale, void *out, aclrtStream stream);
+/* Its gradient, out [vocab, hidden] = scale * sum over the tokens of a row of grad [tokens, hidden]: summed in fp32 in the order of
+ * the tokens (the same bits every time).  outType dataType: every row of out is written, rows without a token with zeros.
+ * outType FP32 with accumulate: the sums are added to out, other rows are left alone. */
+extern int64_t HcclB200EmbeddingGradScratchBytes(int64_t tokens, int64_t vocab, int32_t hidden);
+extern HcclResult HcclB200EmbeddingGrad(const void *ids, HcclDataType idType, int64_t tokens, const void *grad, int64_t gradStride, int64_t vocab,
+                                        int64_t firstId, int32_t hidden, HcclDataType dataType, float scale, void *out, HcclDataType outType,
+                                        int32_t accumulate, void *scratch, aclrtStream stream);
+/* Router: idx [tokens, topk] = experts with the largest logits, largest first, equal ones by number (-inf is never chosen: expert -1,
+ * gate 0); gates [tokens, topk] = their softmax probabilities, normalize: divided by their sum.  Tokens with mask 0 (mask may be
+ * null) or with nothing but -inf are not routed: experts -1, gates 0.  Over the routed tokens: counts [experts] = pairs,
+ * probSum [experts] = sums of the probabilities, *routed = their number n, *balance = experts / (topk n^2) * sum counts * probSum
+ * (0 without tokens).  dataType of the logits: FP32, FP16 or BFP16; at most 4096 experts, topk at most 32. */
+extern int64_t HcclB200MoeGateScratchBytes(int64_t tokens, int32_t nExperts);
+extern HcclResult HcclB200MoeGate(const void *logits, HcclDataType dataType, int64_t tokens, int32_t nExperts, int64_t stride, int32_t topk,
+                                  int32_t normalize, const uint8_t *mask, int32_t *idx, float *gates, int32_t *counts, float *probSum, int32_t *routed,
+                                  float *balance, void *scratch, aclrtStream stream);
+/* *balance from counts, sums and token numbers that were summed over ranks. */
+extern HcclResult HcclB200MoeBalance(const int32_t *counts, const float *probSum, const int32_t *routed, int32_t nExperts, int32_t topk,
+                                     float *balance, aclrtStream stream);
+/* dLogits [tokens, nExperts] (of the logits' type) from the gates' gradient (null: none) and the balance loss's, which is the number
+ * dBalance; counts and routed as the loss had them (counts are constants of it). */
+extern HcclResult HcclB200MoeGateGrad(const void *logits, HcclDataType dataType, int64_t tokens, int32_t nExperts, int64_t stride, int32_t topk,
+                                      int32_t normalize, const uint8_t *mask, const int32_t *idx, const float *dGates, const int32_t *counts,
+                                      const int32_t *routed, float dBalance, void *dLogits, aclrtStream stream);
 /* In-kernel timestamps of the newest executor launch (needs HCCL_KERNEL_TRACE=1 at communicator creation):
  * out[0] = kernel start (globaltimer ns), then per step {after wait, after data movement, after signal}. */
 extern HcclResult HcclB200GetKernelTrace(HcclComm comm, uint32_t localRank, uint64_t *out, size_t capWords, int32_t *nsteps);

@@ -6,15 +6,25 @@ expert outputs and form the gate-weighted sum while receiving).
     ... run the local experts on recv[expert_offsets[e]:expert_offsets[e+1]] and write into ex.expert_out ...
     out = ex.combine(gates)                                              # [tokens, hidden]
 
+The router in front of it, with the balance loss and the gradients of both:
+
+    g = gate(logits, topk, mask=None)                                    # Gate(idx, gates, counts, prob_sum, routed, balance)
+    recv, expert_offsets, recv_rows = ex.dispatch(x, g.idx)              # slots without an expert (-1) are skipped
+    ...
+    d_logits = gate_grad(logits, g, d_gates, balance=coefficient)
+
 Counts travel over the device (all-gather of the per-expert histogram); nothing synchronises with the host.  On an
 all-local communicator every tensor argument is a list with one entry per virtual rank.
 """
 import ctypes as C
+from collections import namedtuple
 
 import torch
 
 from .. import _lib as L
 from ..ops.comm import _raw_stream
+from ..utils.dtypes import float_code
+from ..utils.tensors import check_out, on_device_of
 
 
 class _DevPtr:
@@ -134,6 +144,87 @@ class MoEExchange:
         self.recv = self.expert_out = self._topk = None  # nothing reaches the memory given back here
         self.comm.mem_free(self.h_recv)
         self.comm.mem_free(self.h_out)
+
+
+Gate = namedtuple("Gate", "idx gates counts prob_sum routed balance")
+
+
+def _check_gate(logits, topk, mask):
+    if not (torch.is_tensor(logits) and logits.is_cuda and logits.dim() == 2 and logits.shape[1] > 0):
+        raise ValueError("logits must be a CUDA tensor [tokens, experts]")
+    T, E = logits.shape
+    if float_code(logits.dtype) is None:
+        raise TypeError("logits must be fp32, fp16 or bf16, got %s" % logits.dtype)
+    if logits.stride(1) != 1 and E > 1 or logits.stride(0) < E and T > 1:
+        raise ValueError("the experts of a token must lie side by side (strides %s)" % (tuple(logits.stride()),))
+    if not 1 <= topk <= E:
+        raise ValueError("topk %d of %d experts" % (topk, E))
+    if mask is not None and not (mask.device == logits.device and mask.dtype in (torch.bool, torch.uint8) and mask.shape == (T,) and mask.is_contiguous()):
+        raise ValueError("mask must be a contiguous bool tensor [tokens] on the device of the logits")
+    return T, E, max(E, logits.stride(0))
+
+
+def gate(logits, topk, mask=None, normalize=True, comm=None):
+    """Router of a mixture-of-experts layer.  logits [tokens, experts] (fp32, fp16, bf16; rows may be strided); mask [tokens]: tokens that
+    are routed, others (padding) get no expert and count nowhere.  Returns a Gate:
+
+    idx       int32 [tokens, topk]: the experts with the largest logits, largest first, equal ones by number; a logit of -inf is never
+              chosen, slots that stay empty have expert -1 (the exchange skips them) and gate 0
+    gates     fp32 [tokens, topk]: softmax probabilities of the chosen experts, with `normalize` divided by their sum
+    counts    int32 [experts], prob_sum fp32 [experts], routed int32 []: pairs, sums of probabilities and number of the routed tokens
+    balance   fp32 []: experts / (topk * routed^2) * sum(counts * prob_sum), 1 for an even load
+
+    The sums have a fixed order: the same inputs give the same bits.  With `comm` the three sums, and so the loss, are those of all
+    ranks' tokens (on an all-local communicator logits and mask are lists with one tensor per rank, and a list of Gates returns)."""
+    if comm is not None:
+        ls = list(logits) if isinstance(logits, (list, tuple)) else [logits]
+        ms = list(mask) if isinstance(mask, (list, tuple)) else [mask] * len(ls)
+        if len(ls) != comm.nlocal or len(ms) != comm.nlocal:
+            raise ValueError("one tensor per local rank is needed")
+        gs = [gate(l, topk, m, normalize) for l, m in zip(ls, ms)]
+        if comm.nranks > 1:
+            for name in ("counts", "prob_sum", "routed"):
+                ts = [getattr(g, name) for g in gs]
+                comm.all_reduce(ts, ts)
+            for l, g in zip(ls, gs):
+                with on_device_of(l):
+                    L.check(L.lib().HcclB200MoeBalance(g.counts.data_ptr(), g.prob_sum.data_ptr(), g.routed.data_ptr(), l.shape[1], topk,
+                                                       g.balance.data_ptr(), _raw_stream()), "HcclB200MoeBalance")
+        return gs if isinstance(logits, (list, tuple)) else gs[0]
+    T, E, stride = _check_gate(logits, topk, mask)
+    dev = logits.device
+    with on_device_of(logits):
+        idx, gates = torch.empty(T, topk, device=dev, dtype=torch.int32), torch.empty(T, topk, device=dev, dtype=torch.float32)
+        counts, prob_sum = torch.empty(E, device=dev, dtype=torch.int32), torch.empty(E, device=dev, dtype=torch.float32)
+        routed, balance = torch.empty((), device=dev, dtype=torch.int32), torch.empty((), device=dev, dtype=torch.float32)
+        scratch = torch.empty(max(0, L.lib().HcclB200MoeGateScratchBytes(T, E)), device=dev, dtype=torch.uint8)
+        L.check(L.lib().HcclB200MoeGate(logits.data_ptr(), float_code(logits.dtype), T, E, stride, topk, int(normalize),
+                                        None if mask is None else mask.data_ptr(), idx.data_ptr(), gates.data_ptr(), counts.data_ptr(),
+                                        prob_sum.data_ptr(), routed.data_ptr(), balance.data_ptr(), scratch.data_ptr(), _raw_stream()), "HcclB200MoeGate")
+    return Gate(idx, gates, counts, prob_sum, routed, balance)
+
+
+def gate_grad(logits, g, d_gates=None, balance=0.0, mask=None, normalize=True, out=None):
+    """Gradient of the logits: `d_gates` (fp32 [tokens, topk] or None) is the gates' gradient, the number `balance` that of the balance
+    loss.  logits, mask and normalize are those of the gate() call that returned `g`; counts are constants of the loss.  A slot with
+    expert -1 passes nothing on, rows that are not routed get zeros."""
+    if g.idx.dim() != 2:
+        raise ValueError("g must be what gate() returned for these logits")
+    T, E, stride = _check_gate(logits, g.idx.shape[1], mask)
+    dev, topk = logits.device, g.idx.shape[1]
+    if g.idx.shape[0] != T or g.counts.shape != (E,) or g.idx.device != dev or not g.idx.is_contiguous():
+        raise ValueError("g must be what gate() returned for these logits")
+    if d_gates is not None and not (d_gates.device == dev and d_gates.dtype == torch.float32 and d_gates.shape == g.idx.shape and d_gates.is_contiguous()):
+        raise ValueError("d_gates must be a contiguous fp32 tensor [tokens, topk] on the device of the logits")
+    with on_device_of(logits):
+        if out is None:
+            out = torch.empty(T, E, device=dev, dtype=logits.dtype)
+        else:
+            check_out(out, (T, E), logits.dtype, dev)
+        L.check(L.lib().HcclB200MoeGateGrad(logits.data_ptr(), float_code(logits.dtype), T, E, stride, topk, int(normalize),
+                                            None if mask is None else mask.data_ptr(), g.idx.data_ptr(), None if d_gates is None else d_gates.data_ptr(),
+                                            g.counts.data_ptr(), g.routed.data_ptr(), balance, out.data_ptr(), _raw_stream()), "HcclB200MoeGateGrad")
+    return out
 
 
 def route(tokens, n_experts, topk, seed, rank, device="cuda"):

@@ -37,6 +37,15 @@ def hccl_dtype(x):
     return _TORCH[x.dtype]
 
 
+def float_code(t):
+    """HcclDataType of a floating torch type that the model-side operators take (fp32, fp16, bf16), else None."""
+    global _TORCH
+    if _TORCH is None:
+        _TORCH = _torch_map()
+    code = _TORCH.get(t)
+    return code if code in (L.FP32, L.FP16, L.BFP16) else None
+
+
 def data_ptr(x):
     if x is None:
         return None

@@ -1,0 +1,74 @@
+"""What the embedding and the router refuse on the host, before anything is launched."""
+import ctypes as C
+
+import pytest
+
+from cann_hccl_b200 import _lib as L
+
+MEM = C.create_string_buffer(4096)
+AT = (C.addressof(MEM) + 63) // 64 * 64
+
+
+def embed(grad=False, ids=AT, id_type=L.INT64, tokens=4, rows=AT, stride=8, vocab=16, first=0, hidden=8, dtype=L.BFP16, out=AT, out_type=None, add=0, scratch=AT):
+    lib = L.lib()
+    if not grad:
+        return lib.HcclB200Embedding(ids, id_type, tokens, rows, stride, vocab, first, hidden, dtype, 1.0, out, None)
+    return lib.HcclB200EmbeddingGrad(ids, id_type, tokens, rows, stride, vocab, first, hidden, dtype, 1.0, out, dtype if out_type is None else out_type, add,
+                                     scratch, None)
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("bad,want", [({"ids": None}, "PTR"), ({"rows": None}, "PTR"), ({"out": None}, "PTR"), ({"id_type": L.FP32}, "NOT_SUPPORT"),
+                                      ({"dtype": L.INT32}, "NOT_SUPPORT"), ({"dtype": L.FP64}, "NOT_SUPPORT"), ({"tokens": -1}, "PARA"), ({"tokens": 1 << 31}, "PARA"),
+                                      ({"vocab": 0}, "PARA"), ({"vocab": (1 << 31) - 1}, "PARA"), ({"hidden": 0}, "PARA"), ({"first": -1}, "PARA"),
+                                      ({"stride": 7}, "PARA"), ({"ids": AT + 4}, "PARA"), ({"rows": AT + 1}, "PARA"), ({"out": AT + 1}, "PARA")])
+def test_embedding(grad, bad, want):
+    assert embed(grad, **bad) == getattr(L, "E_" + want)
+
+
+def test_embedding_gradient():
+    assert embed(True, scratch=None) == L.E_PTR
+    assert embed(True, scratch=AT + 8) == L.E_PARA
+    assert embed(True, out_type=L.FP32) == L.E_NOT_SUPPORT                 # fp32 sums are added to, or the rows are fp32
+    assert embed(True, add=1) == L.E_NOT_SUPPORT
+    assert embed(True, add=1, out_type=L.FP32, out=AT + 2) == L.E_PARA
+    lib = L.lib()
+    assert lib.HcclB200EmbeddingGradScratchBytes(-1, 10, 8) == -1 and lib.HcclB200EmbeddingGradScratchBytes(10, 0, 8) == -1
+    assert lib.HcclB200EmbeddingGradScratchBytes(10, 10, 0) == -1 and lib.HcclB200EmbeddingGradScratchBytes(0, 10, 8) > 0
+    assert embed(False, tokens=0, ids=None, out=None) == L.SUCCESS
+
+
+def gate(grad=False, logits=AT, dtype=L.FP32, tokens=4, experts=8, stride=8, topk=2, idx=AT, gates=AT, counts=AT, prob=AT, routed=AT, balance=AT, scratch=AT,
+         d_gates=None, out=AT):
+    lib = L.lib()
+    if not grad:
+        return lib.HcclB200MoeGate(logits, dtype, tokens, experts, stride, topk, 1, None, idx, gates, counts, prob, routed, balance, scratch, None)
+    return lib.HcclB200MoeGateGrad(logits, dtype, tokens, experts, stride, topk, 1, None, idx, d_gates, counts, routed, 0.0, out, None)
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("bad,want", [({"logits": None}, "PTR"), ({"idx": None}, "PTR"), ({"counts": None}, "PTR"), ({"routed": None}, "PTR"),
+                                      ({"dtype": L.INT32}, "NOT_SUPPORT"), ({"experts": 4097, "stride": 4097}, "NOT_SUPPORT"), ({"experts": 64, "stride": 64, "topk": 33}, "NOT_SUPPORT"),
+                                      ({"topk": 9}, "PARA"), ({"topk": 0}, "PARA"), ({"experts": 0}, "PARA"), ({"tokens": -1}, "PARA"), ({"stride": 7}, "PARA"),
+                                      ({"logits": AT + 2}, "PARA"), ({"idx": AT + 2}, "PARA"), ({"counts": AT + 1}, "PARA")])
+def test_gate(grad, bad, want):
+    assert gate(grad, **bad) == getattr(L, "E_" + want)
+
+
+def test_gate_outputs():
+    for name in ("gates", "prob", "balance", "scratch"):
+        assert gate(**{name: None}) == L.E_PTR and gate(**{name: AT + 2}) == L.E_PARA, name
+    assert gate(True, out=None) == L.E_PTR and gate(True, out=AT + 2) == L.E_PARA and gate(True, d_gates=AT + 2) == L.E_PARA
+    lib = L.lib()
+    assert lib.HcclB200MoeBalance(None, AT, AT, 8, 2, AT, None) == L.E_PTR and lib.HcclB200MoeBalance(AT, AT, AT, 8, 9, AT, None) == L.E_PARA
+    assert lib.HcclB200MoeGateScratchBytes(4, 0) == -1 and lib.HcclB200MoeGateScratchBytes(4, 5000) == -1 and lib.HcclB200MoeGateScratchBytes(0, 8) > 0
+
+
+def test_python_arguments():
+    torch = pytest.importorskip("torch")
+    from cann_hccl_b200.parallel import moe, vocab
+    w, ids = torch.zeros(10, 8), torch.zeros(3, dtype=torch.int64)        # host tensors are refused whatever they hold
+    for call in (lambda: vocab.embedding(ids, w), lambda: vocab.embedding_grad(ids, torch.zeros(3, 8), 10), lambda: vocab.embedding_grad(ids, torch.zeros(4, 8), 10),
+                 lambda: moe.gate(torch.zeros(4, 8), 2), lambda: moe.gate(None, 2)):
+        with pytest.raises(ValueError):
+            call()
