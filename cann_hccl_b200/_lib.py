@@ -90,6 +90,11 @@ class MoeLayer(C.Structure):
                [("scratch", C.c_void_p)]
 
 
+class VocabLoss(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("w", C.c_void_p), ("xStride", C.c_int64), ("wStride", C.c_int64), ("targets", C.c_void_p), ("weights", C.c_void_p)] + \
+               [(n, C.c_int64) for n in ("tokens", "vocab", "firstId", "wholeVocab", "ignoreId")] + [("hidden", C.c_int32), ("targetType", C.c_int32)]
+
+
 _lib = None
 fast = None  # csrc/python/fastcall.c, bound to the loaded library (or _calls.py in its place)
 
@@ -179,6 +184,11 @@ def lib():
         "HcclB200MatmulReduceScatter": [vp, P(vp), P(vp), P(vp), i32, i32, i32, vp],
         "HcclB200Embedding": [vp, C.c_int, C.c_int64, vp, C.c_int64, C.c_int64, C.c_int64, i32, C.c_int, C.c_float, vp, vp],
         "HcclB200EmbeddingGrad": [vp, C.c_int, C.c_int64, vp, C.c_int64, C.c_int64, C.c_int64, i32, C.c_int, C.c_float, vp, C.c_int, i32, vp, vp],
+        "HcclB200VocabLossScores": [P(VocabLoss), i32, vp, vp, vp, vp, vp],
+        "HcclB200VocabLossCombine": [P(VocabLoss), vp, i32, vp, vp, vp],
+        "HcclB200VocabLossTotal": [P(VocabLoss), vp, vp],
+        "HcclB200VocabLossSum": [P(VocabLoss), vp, vp, vp, vp],
+        "HcclB200VocabLossGrad": [P(VocabLoss), vp, vp, vp, C.c_float, vp, vp, vp, i32, vp, vp],
         "HcclB200MoeGate": [vp, C.c_int, C.c_int64, i32, C.c_int64, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp],
         "HcclB200MoeBalance": [vp, vp, vp, i32, i32, vp, vp],
         "HcclB200MoeGateGrad": [vp, C.c_int, C.c_int64, i32, C.c_int64, i32, i32, vp, vp, vp, vp, vp, C.c_float, vp, vp],
@@ -231,6 +241,9 @@ def lib():
     L.HcclB200MoeScratchBytes.restype = C.c_int64
     L.HcclB200EmbeddingGradScratchBytes.argtypes = [C.c_int64, C.c_int64, i32]
     L.HcclB200MoeGateScratchBytes.argtypes = [C.c_int64, i32]
+    L.HcclB200VocabLossChunk.argtypes = [C.c_int64, i32]
+    L.HcclB200VocabLossScratchBytes.argtypes = [C.c_int64, C.c_int64, i32, i32]
+    L.HcclB200VocabLossChunk.restype = L.HcclB200VocabLossScratchBytes.restype = C.c_int64
     L.HcclB200EmbeddingGradScratchBytes.restype = L.HcclB200MoeGateScratchBytes.restype = C.c_int64
     L.HcclGetErrorString.argtypes = [C.c_int]
     L.HcclGetErrorString.restype = C.c_char_p

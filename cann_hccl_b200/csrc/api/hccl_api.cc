@@ -21,6 +21,7 @@
 #include "health/consistency.h"
 #include "health/fault_inject.h"
 #include "kernels/fused/gemm_local.h"
+#include "kernels/fused/vocab_loss.h"
 #include "kernels/moe_a2a.h"
 #include "kernels/moe_gate.h"
 #include "kernels/vocab_embed.h"
@@ -858,6 +859,84 @@ HcclResult HcclB200MoeGateGrad(const void *logits, HcclDataType dataType, int64_
     CHK_RET(check_gate(logits, dataType, tokens, nExperts, stride, topk, normalize, {counts, routed}, {idx, dLogits}, "HcclB200MoeGateGrad", &s));
     CHK_RET(check_aligned({idx, dGates}, 4, "HcclB200MoeGateGrad"));
     return moe_gate_grad(s, logits, idx, dGates, counts, routed, mask, dBalance, dLogits, stream);
+}
+// targets: only the targets and weights are looked at
+static HcclResult check_vocab_loss(const HcclB200VocabLoss *p, bool targets, std::initializer_list<const void *> words, const char *api, VocabLossCall *c)
+{
+    CHK_RET_LOG(!p, HCCL_E_PTR, "[EI0003] %s: null pointer", api);
+    CHK_RET_LOG(p->targetType != HCCL_DATA_TYPE_INT32 && p->targetType != HCCL_DATA_TYPE_INT64, HCCL_E_NOT_SUPPORT, "%s: targets of type %d are not INT32 or INT64", api,
+                p->targetType);
+    CHK_RET_LOG(p->tokens < 0 || p->tokens > INT32_MAX || p->wholeVocab < 1, HCCL_E_PARA, "%s: %lld tokens, vocabulary of %lld", api, (long long)p->tokens,
+                (long long)p->wholeVocab);
+    bool null = p->tokens > 0 && !p->targets;
+    for (const void *w : words) null = null || !w;
+    if (!targets) {
+        CHK_RET_LOG(p->vocab < 1 || p->vocab >= INT32_MAX - 256 || p->hidden < 8 || p->hidden % 8 || p->firstId < 0 || p->firstId > p->wholeVocab - p->vocab, HCCL_E_PARA,
+                    "%s: vocabulary of %lld from %lld of %lld, rows of %d (a multiple of 8 is needed)", api, (long long)p->vocab, (long long)p->firstId,
+                    (long long)p->wholeVocab, p->hidden);
+        CHK_RET_LOG(p->tokens > (1 << 20), HCCL_E_PARA, "%s: %lld tokens are more than a chunk", api, (long long)p->tokens);
+        CHK_RET_LOG(p->xStride < p->hidden || p->wStride < p->hidden || p->xStride % 8 || p->wStride % 8, HCCL_E_PARA, "%s: strides %lld, %lld of rows of %d", api,
+                    (long long)p->xStride, (long long)p->wStride, p->hidden);
+        null = null || !p->w || (p->tokens > 0 && !p->x);
+    }
+    CHK_RET_LOG(null, HCCL_E_PTR, "[EI0003] %s: null pointer", api);
+    if (!targets) CHK_RET(check_aligned({p->x, p->w}, 16, api));
+    CHK_RET(check_aligned({p->targets}, dtype_size(p->targetType), api));
+    CHK_RET(check_aligned({p->weights}, 4, api));
+    CHK_RET(check_aligned(words, 4, api));
+    *c = VocabLossCall{p->x, p->w, p->xStride, p->wStride, p->targets, p->targetType == HCCL_DATA_TYPE_INT64, p->weights, p->tokens, p->vocab, p->firstId,
+                       p->wholeVocab, p->ignoreId, p->hidden};
+    return HCCL_SUCCESS;
+}
+int64_t HcclB200VocabLossChunk(int64_t vocab, int32_t withGrad) { return vocab < 1 || vocab >= INT32_MAX - 256 ? -1 : vocab_loss_chunk(vocab, withGrad != 0); }
+int64_t HcclB200VocabLossScratchBytes(int64_t tokens, int64_t vocab, int32_t hidden, int32_t withGrad)
+{
+    return tokens < 0 || tokens > (1 << 20) || vocab < 1 || vocab >= INT32_MAX - 256 || hidden < 8 || hidden % 8 ? -1
+           : vocab_loss_scratch_bytes(tokens, vocab, hidden, withGrad != 0);
+}
+HcclResult HcclB200VocabLossScores(const HcclB200VocabLoss *p, int32_t withGrad, float *lse, float *target, float *losses, void *scratch, aclrtStream stream)
+{
+    VocabLossCall c;
+    CHK_RET(check_vocab_loss(p, false, {lse, target, scratch}, "HcclB200VocabLossScores", &c));
+    CHK_RET(check_aligned({losses}, 4, "HcclB200VocabLossScores"));
+    CHK_RET(check_aligned({scratch}, 256, "HcclB200VocabLossScores"));
+    CHK_RET_LOG(losses && p->vocab != p->wholeVocab, HCCL_E_PARA, "HcclB200VocabLossScores: a shard's losses need the other shards");
+    return c.tokens ? vocab_loss_scores(c, withGrad != 0, lse, target, losses, scratch, stream) : HCCL_SUCCESS;
+}
+HcclResult HcclB200VocabLossCombine(const HcclB200VocabLoss *p, const float *parts, int32_t shards, float *lse, float *losses, aclrtStream stream)
+{
+    VocabLossCall c;
+    CHK_RET(check_vocab_loss(p, true, {parts, lse, losses}, "HcclB200VocabLossCombine", &c));
+    CHK_RET_LOG(shards < 1, HCCL_E_PARA, "HcclB200VocabLossCombine: %d shards", shards);
+    return c.tokens ? vocab_loss_combine(c, parts, shards, lse, losses, stream) : HCCL_SUCCESS;
+}
+HcclResult HcclB200VocabLossTotal(const HcclB200VocabLoss *p, float *total, aclrtStream stream)
+{
+    VocabLossCall c;
+    CHK_RET(check_vocab_loss(p, true, {total}, "HcclB200VocabLossTotal", &c));
+    return vocab_loss_total(c, total, stream);
+}
+HcclResult HcclB200VocabLossSum(const HcclB200VocabLoss *p, const float *losses, const float *total, float *loss, aclrtStream stream)
+{
+    VocabLossCall c;
+    CHK_RET(check_vocab_loss(p, true, {loss}, "HcclB200VocabLossSum", &c));
+    CHK_RET_LOG(c.tokens && !losses, HCCL_E_PTR, "[EI0003] HcclB200VocabLossSum: null pointer");
+    CHK_RET(check_aligned({losses, total}, 4, "HcclB200VocabLossSum"));
+    return vocab_loss_sum(c, losses, total, loss, stream);
+}
+HcclResult HcclB200VocabLossGrad(const HcclB200VocabLoss *p, const float *lse, const float *target, const float *total, float scale, void *dx, void *dw,
+                                 float *dwSum, int32_t dwKind, void *scratch, aclrtStream stream)
+{
+    VocabLossCall c;
+    CHK_RET(check_vocab_loss(p, false, {lse, target, scratch}, "HcclB200VocabLossGrad", &c));
+    CHK_RET_LOG(dwKind < VL_BF16 || dwKind > VL_ADD_BF16, HCCL_E_PARA, "HcclB200VocabLossGrad: unknown kind %d of dw", dwKind);
+    CHK_RET_LOG((c.tokens && !dx) || (!dw && (dwKind == VL_BF16 || dwKind == VL_ADD_BF16)) || (!dwSum && dwKind != VL_BF16), HCCL_E_PTR,
+                "[EI0003] HcclB200VocabLossGrad: null pointer");
+    CHK_RET(check_aligned({dx, dw, dwSum}, 16, "HcclB200VocabLossGrad"));
+    CHK_RET(check_aligned({total}, 4, "HcclB200VocabLossGrad"));
+    CHK_RET(check_aligned({scratch}, 256, "HcclB200VocabLossGrad"));
+    CHK_RET_LOG(!c.tokens, HCCL_E_PARA, "HcclB200VocabLossGrad: no tokens");
+    return vocab_loss_grad(c, lse, target, total, scale, dx, dw, dwSum, dwKind, scratch, stream);
 }
 static HcclResult check_act(int32_t act, const char *api)
 {

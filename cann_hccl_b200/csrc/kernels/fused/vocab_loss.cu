@@ -1,0 +1,817 @@
+// Linear layer and softmax cross entropy over the vocabulary, with gradients, without keeping the logits:
+//   s = x W^T;  lse_t = log sum_v exp s_tv;  loss_t = lse_t - s_t,y;  d_tv = g_t (exp(s_tv - lse_t) - [v = y]);  dx = d W;  dW = d^T x
+//
+// scores   tcgen05 product of a chunk of tokens with all tiles of the vocabulary.  The epilogue takes a row's half tile from TMEM,
+//          leaves its maximum m and sum of exp(s - m) (fp32) and, for gradients, 2^15 exp(s - m) in fp16: relative to the half
+//          tile's own maximum 11 bits hold every probability down to 2^-29 of it, so that the one rounding that counts
+//          is the later one of d to bf16.  Logits are never stored, and nothing is computed twice (6 T V H operations in all;
+//          a second product in place of the exponentials would make it 8).
+// rows     lse, target logit and loss of a token from its half tiles.
+// d        exponentials to d in place (bf16), rescaled by exp(m - lse); the target's column is g expm1(s_y - lse), which keeps its
+//          digits for sure guesses.  Tokens that do not count become rows of zeros here, and their x too: 0 x inf is not 0.
+// dx, dW   tcgen05 products that read W, d and x as they lie: an operand whose depth is not its contiguous side goes to the tensor
+//          cores MN-major (boxes of 64 elements x 64 deep).  dx with few tiles is cut along the vocabulary into fp32 shares that a
+//          last launch adds in order; dW over several chunks is summed in fp32.
+//
+// One persistent CTA per SM: warp 0 TMA producer (128-byte swizzle, never multicast), warp 1 MMA issuer into one of two TMEM
+// accumulators, warps 2-9 epilogue of the other.  More than 128 rows: clusters of two CTAs on 256 rows (cta_group::2).
+// A wait that runs out makes what it was for NaN.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <algorithm>
+#include <cstring>
+#include <mutex>
+#include "common/log.h"
+#include "kernels/fused/tc05.cuh"
+#include "kernels/fused/tensor_map.h"
+#include "kernels/fused/vocab_loss.h"
+#include "kernels/pdl.cuh"
+
+namespace hcclb {
+
+namespace {
+using namespace tc05;
+
+enum Mode : int { SCORES = 0, DX = 1, DW = 2 };
+constexpr int kThreads = 320, kEpiWarps = 8;
+constexpr uint32_t kABytes = BM * BK * 2, kStageSpace = 7 * 32768;  // seven stages of a pair
+constexpr uint32_t kTmemCols = 512;
+constexpr int kMaxStages = 8, kMaxCols = BN;
+constexpr uint32_t kChunkBytes = BK * 128;         // MN-major: 64 elements x 64 deep
+constexpr float kExpBits = 15.f, kExpScale = 1.f / 32768.f, kLog2e = 1.4426950408889634f;
+
+struct alignas(64) LossGemm {
+    CUtensorMap tmA, tmB;
+    int M, N;                        // rows and columns of the result
+    int cols, um_tiles, n_tiles, panel;
+    int k_iters, split;              // split: shares along the depth (DX)
+    int units, stages;
+    uint32_t stage_bytes, idesc;
+    // scores
+    float2 *stats;                   // [row][2 * n_tiles]: maximum, sum of exp(s - maximum)
+    float *target;                   // [row]
+    __half *e;                       // [row][ld], may be null
+    const void *y;
+    int64_t first, ignore;
+    int wide_y;
+    // dx, dW
+    __nv_bfloat16 *out;
+    float *sum;                      // shares of dx: [share][row][N]
+    int kind;                        // VocabLossOut
+    int64_t ld;
+    int wide;                        // rows of out and sum start on 32-byte boundaries
+};
+
+struct LossShared {
+    alignas(1024) uint8_t tiles[kStageSpace];
+    alignas(8) uint64_t full_bar[kMaxStages];
+    uint64_t empty_bar[kMaxStages];
+    uint64_t tmem_full[2], tmem_empty[2];
+    uint32_t tmem_base, fail;
+};
+constexpr size_t kSmemBytes = sizeof(LossShared) + 1024;
+static_assert(kSmemBytes <= 227 * 1024, "one CTA per SM");
+
+// MN-major operand, 128-byte swizzle: 64 elements side by side, 8 deep in 1024 bytes, the next 64 elements kChunkBytes on.
+__device__ __forceinline__ uint64_t make_desc_mn(const void *ptr)
+{
+    uint64_t d = 0;
+    d |= (uint64_t)((smem_u32(ptr) & 0x3FFFF) >> 4);
+    d |= (uint64_t)(kChunkBytes >> 4) << 16;           // leading dimension: from 64 elements to the next
+    d |= (uint64_t)(1024 >> 4) << 32;                  // stride dimension: from 8 deep to the next
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+constexpr uint32_t kStepK = 2, kStepMn = (UMMA_K * 128) >> 4;  // 16 deep further, in 16-byte units
+
+struct Tile { int um, nt, share; };
+__device__ __forceinline__ Tile tile_at(const LossGemm &P, int t)
+{
+    Tile w;
+    const int tiles = P.um_tiles * P.n_tiles;
+    w.share = t / tiles;
+    t -= w.share * tiles;
+    const int per = P.um_tiles * P.panel, pn = t / per, n0 = pn * P.panel, width = min(P.panel, P.n_tiles - n0), r = t - pn * per;
+    w.um = r / width;
+    w.nt = n0 + r - w.um * width;
+    return w;
+}
+
+__device__ __forceinline__ void st_v8(void *p, const uint32_t (&v)[8])
+{
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
+__device__ __forceinline__ float exp2_approx(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ int64_t target_of(const void *y, int wide, int64_t t) { return wide ? ((const int64_t *)y)[t] : (int64_t)((const int32_t *)y)[t]; }
+
+// 16 or 32 columns of a row from TMEM
+__device__ __forceinline__ void tmem_cols(uint32_t addr, float (&v)[32])
+{
+    uint32_t r[32];
+    tmem_ld32(addr, r);
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_cols(uint32_t addr, float (&v)[16])
+{
+    uint32_t r[16];
+    tmem_ld16(addr, r);
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+template <int C> __device__ __forceinline__ void row_max(uint32_t taddr, int left, float &m)
+{
+    float v[C];
+    tmem_cols(taddr, v);
+    if (left >= C) {
+#pragma unroll
+        for (int i = 0; i < C; ++i) m = fmaxf(m, v[i]);
+    } else
+#pragma unroll
+        for (int i = 0; i < C; ++i) m = fmaxf(m, i < left ? v[i] : -INFINITY);
+}
+// Exponentials of C columns against m; left: columns that exist; y: the target's column from here; e: where they go (null: nowhere).
+template <int C>
+__device__ __forceinline__ void row_exp(uint32_t taddr, int left, float m, int y, float &z, float &target, __half *e, int room)
+{
+    float v[C];
+    tmem_cols(taddr, v);
+    if ((uint32_t)y < (uint32_t)C)
+#pragma unroll
+        for (int i = 0; i < C; ++i) target = i == y ? v[i] : target;
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+        v[i] = exp2_approx(fmaf(v[i] - m, kLog2e, kExpBits));
+        if (left < C && i >= left) v[i] = 0.f;
+        z += v[i];
+    }
+    if (e)
+#pragma unroll
+        for (int c = 0; c < C; c += 16)
+            if (c < room) {
+                uint32_t o[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const __half2 h = __floats2half2_rn(v[c + 2 * i], v[c + 2 * i + 1]);
+                    o[i] = *(const uint32_t *)&h;
+                }
+                st_v8(e + c, o);
+            }
+}
+
+// 16 results of a row, of which `left` exist (a multiple of 8).
+__device__ __forceinline__ void put16(const LossGemm &P, int64_t at, float *sum, float (&v)[16], int left)
+{
+    if (P.kind == VL_ADD || P.kind == VL_ADD_BF16)
+#pragma unroll
+        for (int c = 0; c < 16; c += 4)
+            if (c < left) {
+                const float4 f = *(const float4 *)(sum + at + c);
+                v[c] += f.x; v[c + 1] += f.y; v[c + 2] += f.z; v[c + 3] += f.w;
+            }
+    if (P.kind == VL_F32 || P.kind == VL_ADD) {
+#pragma unroll
+        for (int c = 0; c < 16; c += 4)
+            if (c < left) *(float4 *)(sum + at + c) = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
+    } else {
+        uint32_t o[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = pack_bf16(__float_as_uint(v[2 * i]), __float_as_uint(v[2 * i + 1]));
+        __nv_bfloat16 *p = P.out + at;
+        if (P.wide && left >= 16) st_v8(p, o);
+        else {
+            if (left >= 8) ((uint4 *)p)[0] = make_uint4(o[0], o[1], o[2], o[3]);
+            if (left >= 16) ((uint4 *)p)[1] = make_uint4(o[4], o[5], o[6], o[7]);
+        }
+    }
+}
+
+template <int MODE, bool kPair>
+__global__ void __launch_bounds__(kThreads, 1) vocab_loss_gemm(const __grid_constant__ LossGemm P)
+{
+    extern __shared__ uint8_t smem_raw[];
+    LossShared &S = *(LossShared *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    constexpr int kCtas = kPair ? 2 : 1;
+    constexpr bool kMnA = MODE == DW, kMnB = MODE != SCORES;
+    const uint32_t stages = (uint32_t)P.stages, stage_bytes = P.stage_bytes;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t cta_r = kPair ? cluster_ctarank() : 0u;
+    const int unit = (int)blockIdx.x / kCtas, total = P.um_tiles * P.n_tiles * P.split;
+    volatile uint32_t *fail = &S.fail;
+
+    pdl_trigger();
+    if (threadIdx.x == 0) {
+        S.fail = 0;
+        for (int i = 0; i < kMaxStages; ++i) { mbar_init(&S.full_bar[i], 1); mbar_init(&S.empty_bar[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&S.tmem_full[i], 1); mbar_init(&S.tmem_empty[i], kCtas * kEpiWarps); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        prefetch_tensormap(&P.tmA);
+        prefetch_tensormap(&P.tmB);
+    }
+    if (warp == 1) {
+        if (kPair) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&S.tmem_base)), "r"(kTmemCols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&S.tmem_base)), "r"(kTmemCols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (kPair) cluster_sync_all();
+    tc_fence_after();
+    const uint32_t tmem_base = S.tmem_base;
+    pdl_wait();
+
+    if (warp == 0) {
+        // ------------------------------------------------------------------ TMA producer
+        if (elect_one()) {
+            uint32_t s = 0, ph = 0;
+            const int bcols = P.cols / kCtas;
+            for (int t = unit; t < total && !*fail; t += P.units) {
+                const Tile w = tile_at(P, t);
+                const int arow = (w.um * kCtas + (int)cta_r) * BM, brow = w.nt * P.cols + (int)cta_r * bcols;
+                const int k0 = (int)((int64_t)P.k_iters * w.share / P.split), k1 = (int)((int64_t)P.k_iters * (w.share + 1) / P.split);
+                for (int k = k0; k < k1; ++k) {
+                    if (!mbar_wait_t<kPair>(&S.empty_bar[s], ph ^ 1, fail)) break;
+                    uint8_t *sa = S.tiles + (size_t)s * stage_bytes, *sb = sa + kABytes;
+                    uint32_t full = smem_u32(&S.full_bar[s]);
+                    if (kPair) {  // the bytes of both CTAs' loads are counted on the leader's barrier
+                        if (cta_r == 0) mbar_expect_tx(&S.full_bar[s], 2 * stage_bytes);
+                        full = mapa_u32(full, 0);
+                    } else
+                        mbar_expect_tx(&S.full_bar[s], stage_bytes);
+                    auto load = [&](uint8_t *dst, const CUtensorMap *map, int x, int y) {
+                        if (kPair) tma_load_2d_pair(dst, map, full, x, y); else tma_load_2d(dst, map, &S.full_bar[s], x, y);
+                    };
+                    if (kMnA) {
+#pragma unroll
+                        for (int c = 0; c < BM / 64; ++c) load(sa + c * kChunkBytes, &P.tmA, arow + c * 64, k * BK);
+                    } else
+                        load(sa, &P.tmA, k * BK, arow);
+                    if (kMnB) {
+                        for (int c = 0; c < bcols / 64; ++c) load(sb + c * kChunkBytes, &P.tmB, brow + c * 64, k * BK);
+                    } else
+                        load(sb, &P.tmB, k * BK, brow);
+                    if (++s == stages) { s = 0; ph ^= 1; }
+                }
+            }
+        }
+        if (*fail)  // loads in flight land before the CTA lets go of its shared memory
+            for (int i = 0; i < 200; ++i) __nanosleep(1000);
+    } else if (warp == 1) {
+        // ------------------------------------------------------------------ MMA issuer (pair: the leader, for both CTAs)
+        if (cta_r == 0 && elect_one()) {
+            uint32_t s = 0, ph = 0, n = 0;
+            for (int t = unit; t < total && !*fail; t += P.units, ++n) {
+                const Tile w = tile_at(P, t);
+                const int k0 = (int)((int64_t)P.k_iters * w.share / P.split), k1 = (int)((int64_t)P.k_iters * (w.share + 1) / P.split);
+                const uint32_t buf = n & 1, use = n >> 1, d = tmem_base + buf * kMaxCols;
+                if (!mbar_wait_t<kPair>(&S.tmem_empty[buf], (use & 1) ^ 1, fail)) break;
+                tc_fence_after();
+                for (int k = k0; k < k1; ++k) {
+                    if (!mbar_wait_t<kPair>(&S.full_bar[s], ph, fail)) break;
+                    tc_fence_after();
+                    const uint8_t *sa = S.tiles + (size_t)s * stage_bytes, *sb = sa + kABytes;
+                    const uint64_t da = kMnA ? make_desc_mn(sa) : make_smem_desc(sa), db = kMnB ? make_desc_mn(sb) : make_smem_desc(sb);
+#pragma unroll
+                    for (int kk = 0; kk < BK / UMMA_K; ++kk) {
+                        const uint64_t a = da + (uint64_t)(kk * (kMnA ? kStepMn : kStepK)), b = db + (uint64_t)(kk * (kMnB ? kStepMn : kStepK));
+                        if (kPair) umma_pair(d, a, b, k != k0 || kk != 0, P.idesc); else umma(d, a, b, k != k0 || kk != 0, P.idesc);
+                    }
+                    if (kPair) umma_commit_pair(&S.empty_bar[s]); else umma_commit(&S.empty_bar[s]);
+                    if (++s == stages) { s = 0; ph ^= 1; }
+                }
+                if (kPair) umma_commit_pair(&S.tmem_full[buf]); else umma_commit(&S.tmem_full[buf]);
+            }
+        }
+    } else {
+        // ------------------------------------------------------------------ epilogue: a warp reaches its TMEM lane quarter, half of the columns
+        const int q4 = warp & 3, half = (warp - 2) >> 2, rl = q4 * 32 + lane;
+        const int mid = (P.cols / 16 + 1) / 2 * 16, c_lo = half ? mid : 0, c_hi = half ? P.cols : mid;
+        uint32_t n = 0;
+        bool bad = false;
+        for (int t = unit; t < total; t += P.units, ++n) {
+            const Tile w = tile_at(P, t);
+            const int row = (w.um * kCtas + (int)cta_r) * BM + rl, col0 = w.nt * P.cols;
+            const uint32_t buf = n & 1, use = n >> 1, taddr = tmem_base + buf * kMaxCols + ((uint32_t)(q4 * 32) << 16);
+            int64_t y = -1;
+            if (MODE == SCORES && row < P.M) {
+                const int64_t id = target_of(P.y, P.wide_y, row);
+                if (id != P.ignore) y = id - P.first - col0;  // of this tile's columns; far outside elsewhere
+            }
+            bad = bad || !mbar_wait_t<kPair>(&S.tmem_full[buf], use & 1, fail);
+            bad = __any_sync(0xffffffffu, bad);
+            tc_fence_after();
+            if (MODE == SCORES) {
+                const int left = P.N - col0;  // columns that exist from the tile's first on
+                float m = -INFINITY, z = 0.f, target = 0.f;
+                if (!bad) {
+                    const int c_end = min(c_hi, (left + 15) / 16 * 16);
+                    int c = c_lo;
+#pragma unroll 1
+                    for (; c + 32 <= c_end; c += 32) row_max<32>(taddr + c, left - c, m);
+                    if (c < c_end) row_max<16>(taddr + c, left - c, m);
+                    const float ref = m == -INFINITY ? 0.f : m;
+                    __half *e = P.e && row < P.M ? P.e + (int64_t)row * P.ld + col0 : nullptr;
+                    const int room = (int)min((int64_t)c_hi, P.ld - col0);  // the row ends behind the last column, on a multiple of 64
+                    const int yl = y >= c_lo && y < c_hi && y < left ? (int)y : -1;
+                    c = c_lo;
+#pragma unroll 1
+                    for (; c + 32 <= c_end; c += 32) row_exp<32>(taddr + c, left - c, ref, yl < 0 ? -1 : yl - c, z, target, e ? e + c : nullptr, room - c);
+                    if (c < c_end) {
+                        row_exp<16>(taddr + c, left - c, ref, yl < 0 ? -1 : yl - c, z, target, e ? e + c : nullptr, room - c);
+                        c += 16;
+                    }
+                    if (e) {
+                        const uint32_t zero[8] = {};
+                        for (; c < room; c += 16) st_v8(e + c, zero);
+                    }
+                    z *= kExpScale;
+                    if (yl >= 0) P.target[row] = target;
+                } else
+                    z = __uint_as_float(0x7fffffffu);
+                if (row < P.M) P.stats[(int64_t)row * (2 * P.n_tiles) + 2 * w.nt + half] = make_float2(m, z);
+            } else {
+                float *sum = P.sum + (P.split > 1 ? (int64_t)w.share * P.M * P.N : 0);
+                const int c_end = min(c_hi, P.N - col0);
+                const int64_t at = (int64_t)row * P.N + col0;
+                int c = c_lo;
+#pragma unroll 1
+                for (; c < c_end; c += 16) {
+                    float v[16];
+                    if (!bad) tmem_cols(taddr + c, v);
+                    else
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(0x7fffffffu);
+                    if (row < P.M) put16(P, at + c, sum, v, c_end - c);
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0 && !bad) {
+                if (kPair) mbar_arrive_cluster(mapa_u32(smem_u32(&S.tmem_empty[buf]), 0)); else mbar_arrive(&S.tmem_empty[buf]);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (kPair) cluster_sync_all();  // the leader's MMAs use both CTAs' stages and TMEM, its commits arrive on both
+    if (warp == 1) {
+        tc_fence_after();
+        if (kPair) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols) : "memory");
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------- rows
+struct RowArgs {
+    const float2 *stats;
+    const float *parts;              // combine: [shards][2][tokens]
+    const void *y;
+    const float *weights, *losses_in, *total;
+    float *lse, *target, *losses, *out;
+    uint8_t *e;                      // [row][ld] 2 bytes each
+    const uint8_t *x;
+    uint8_t *xc;
+    int64_t tokens, first, vocab, whole, ignore, ld, x_stride;
+    int wide, halves, cols, n_tiles, shards, xvec;
+    float scale;
+};
+
+__device__ __forceinline__ bool counts(const RowArgs &a, int64_t id) { return id != a.ignore && id >= 0 && id < a.whole; }
+
+__device__ __forceinline__ float warp_max(float x)
+{
+#pragma unroll
+    for (int o = 16; o; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+    return x;
+}
+__device__ __forceinline__ float warp_sum(float x)
+{
+#pragma unroll
+    for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    return x;
+}
+
+constexpr int kRowThreads = 128, kRowRegs = 8;
+
+// One CTA per token.
+__global__ void __launch_bounds__(kRowThreads) vocab_loss_rows(const __grid_constant__ RowArgs a)
+{
+    __shared__ float s_m[kRowThreads / 32], s_z[kRowThreads / 32];
+    pdl_trigger();
+    pdl_wait();
+    const int64_t t = blockIdx.x;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const float2 *p = a.stats + t * a.halves;
+    float m = -INFINITY, z = 0.f;
+    for (int i0 = 0; i0 < a.halves; i0 += kRowThreads * kRowRegs) {
+        float2 v[kRowRegs];
+        float top = m;
+#pragma unroll
+        for (int k = 0; k < kRowRegs; ++k) {
+            const int i = i0 + k * kRowThreads + threadIdx.x;
+            v[k] = i < a.halves ? p[i] : make_float2(-INFINITY, 0.f);
+            top = fmaxf(top, v[k].x);
+        }
+        const float ref = top == -INFINITY ? 0.f : top;
+        z *= __expf(m - ref);
+#pragma unroll
+        for (int k = 0; k < kRowRegs; ++k) z = fmaf(v[k].y, __expf(v[k].x - ref), z);
+        m = top;
+    }
+    const float wm = warp_max(m);
+    if (lane == 0) s_m[warp] = wm;
+    __syncthreads();
+    float all = s_m[0];
+#pragma unroll
+    for (int w = 1; w < kRowThreads / 32; ++w) all = fmaxf(all, s_m[w]);
+    const float ref = all == -INFINITY ? 0.f : all;
+    z = warp_sum(z * __expf(m - ref));
+    if (lane == 0) s_z[warp] = z;
+    __syncthreads();
+    if (threadIdx.x) return;
+    z = s_z[0];
+#pragma unroll
+    for (int w = 1; w < kRowThreads / 32; ++w) z += s_z[w];
+    const int64_t id = target_of(a.y, a.wide, t);
+    const uint64_t at = (uint64_t)id - (uint64_t)a.first;
+    const bool here = counts(a, id) && at < (uint64_t)a.vocab;
+    const float log_z = logf(z);
+    a.lse[t] = all + log_z;
+    if (!here) a.target[t] = -INFINITY;
+    if (a.losses) a.losses[t] = counts(a, id) ? (all - a.target[t]) + log_z : 0.f;
+}
+
+// Joint lse and loss from the shards'.
+__global__ void __launch_bounds__(kRowThreads) vocab_loss_join(const __grid_constant__ RowArgs a)
+{
+    pdl_trigger();
+    const int64_t t = (int64_t)blockIdx.x * kRowThreads + threadIdx.x;
+    pdl_wait();
+    if (t >= a.tokens) return;
+    float m = -INFINITY, target = -INFINITY;
+    for (int r = 0; r < a.shards; ++r) {
+        m = fmaxf(m, a.parts[(int64_t)(2 * r) * a.tokens + t]);
+        target = fmaxf(target, a.parts[(int64_t)(2 * r + 1) * a.tokens + t]);
+    }
+    const float ref = m == -INFINITY ? 0.f : m;
+    float z = 0.f;
+    for (int r = 0; r < a.shards; ++r) z += expf(a.parts[(int64_t)(2 * r) * a.tokens + t] - ref);
+    const float log_z = logf(z);
+    a.lse[t] = m + log_z;
+    a.losses[t] = counts(a, target_of(a.y, a.wide, t)) ? (m - target) + log_z : 0.f;
+}
+
+constexpr int kSumThreads = 1024;
+// Sum over the tokens that count of the weights (losses_in null) or of weights * losses, in one order.
+__global__ void __launch_bounds__(kSumThreads) vocab_loss_reduce(const __grid_constant__ RowArgs a)
+{
+    __shared__ float s_w[kSumThreads / 32];
+    pdl_trigger();
+    pdl_wait();
+    float sum = 0.f;
+#pragma unroll 4
+    for (int64_t t = threadIdx.x; t < a.tokens; t += kSumThreads) {
+        float v = 0.f;
+        if (counts(a, target_of(a.y, a.wide, t))) {
+            v = a.weights ? a.weights[t] : 1.f;
+            if (a.losses_in) v = v == 0.f ? 0.f : v * a.losses_in[t];
+        }
+        sum += v;
+    }
+    sum = warp_sum(sum);
+    if ((threadIdx.x & 31) == 0) s_w[threadIdx.x >> 5] = sum;
+    __syncthreads();
+    if (threadIdx.x >= 32) return;
+    sum = warp_sum(s_w[threadIdx.x]);
+    if (threadIdx.x) return;
+    if (a.total) sum = *a.total != 0.f ? sum / *a.total : 0.f;
+    *a.out = sum;
+}
+
+constexpr int kDThreads = 256, kDBatch = 4;
+
+// Exponentials -> d, in place; rows of x that count -> xc.  One CTA per token, a warp's lanes share a tile (8 columns each).
+__global__ void __launch_bounds__(kDThreads) vocab_loss_d(const __grid_constant__ RowArgs a)
+{
+    pdl_trigger();
+    pdl_wait();
+    const int64_t t = blockIdx.x;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t id = target_of(a.y, a.wide, t);
+    const float share = !counts(a, id) ? 0.f : a.weights ? a.weights[t] : 1.f;
+    const float total = a.total ? *a.total : 1.f;
+    const float g = share == 0.f || total == 0.f ? 0.f : a.scale * (share / total);
+    uint4 *row = (uint4 *)(a.e + t * a.ld * 2);
+    {
+        const uint4 *src = (const uint4 *)(a.x + t * a.x_stride);
+        uint4 *dst = (uint4 *)a.xc + t * a.xvec;
+        for (int v = threadIdx.x; v < a.xvec; v += kDThreads) dst[v] = share == 0.f ? make_uint4(0, 0, 0, 0) : src[v];
+    }
+    if (share == 0.f) {
+        for (int v = threadIdx.x; v < a.ld / 8; v += kDThreads) row[v] = make_uint4(0, 0, 0, 0);
+        return;
+    }
+    const float lse = a.lse[t];
+    const int64_t y = id - a.first;  // may lie in another shard
+    const float dy = g * expm1f(a.target[t] - lse);
+    const int mid = (a.cols / 16 + 1) / 2 * 16, c = lane * 8, half = c >= mid;
+    const float2 *stats = a.stats + t * a.halves + half;
+    for (int n0 = warp; n0 < a.n_tiles; n0 += kDThreads / 32 * kDBatch) {
+        uint4 v[kDBatch];
+        float f[kDBatch];
+#pragma unroll
+        for (int k = 0; k < kDBatch; ++k) {
+            const int n = n0 + k * (kDThreads / 32);
+            if (n < a.n_tiles && c < a.cols && (int64_t)n * a.cols + c < a.ld) {
+                v[k] = row[(n * (int64_t)a.cols + c) / 8];
+                f[k] = stats[2 * n].x;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kDBatch; ++k) {
+            const int n = n0 + k * (kDThreads / 32);
+            const int64_t col = (int64_t)n * a.cols + c;
+            if (n < a.n_tiles && c < a.cols && col < a.ld) {
+                const float fac = __expf(f[k] - lse) * g * kExpScale;
+                float d[8];
+                const __half2 *h = (const __half2 *)&v[k];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 u = __half22float2(h[i]);
+                    d[2 * i] = u.x * fac; d[2 * i + 1] = u.y * fac;
+                }
+                if (y >= col && y < col + 8 && y < a.vocab)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) d[i] = i == (int)(y - col) ? dy : d[i];
+                uint4 o;
+                o.x = pack_bf16(__float_as_uint(d[0]), __float_as_uint(d[1])); o.y = pack_bf16(__float_as_uint(d[2]), __float_as_uint(d[3]));
+                o.z = pack_bf16(__float_as_uint(d[4]), __float_as_uint(d[5])); o.w = pack_bf16(__float_as_uint(d[6]), __float_as_uint(d[7]));
+                row[col / 8] = o;
+            }
+        }
+    }
+}
+
+struct ShareArgs { const float *shares; __nv_bfloat16 *out; int64_t n; int split; };
+// Shares of dx added in order.
+__global__ void __launch_bounds__(256) vocab_loss_shares(const __grid_constant__ ShareArgs a)
+{
+    pdl_trigger();
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+    pdl_wait();
+    if (i >= a.n) return;
+    float v[8] = {};
+#pragma unroll 4
+    for (int q = 0; q < a.split; ++q) {
+        const float4 *p = (const float4 *)(a.shares + q * a.n + i);
+        const float4 x = p[0], y = p[1];
+        v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+        v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+    }
+    uint4 o;
+    o.x = pack_bf16(__float_as_uint(v[0]), __float_as_uint(v[1])); o.y = pack_bf16(__float_as_uint(v[2]), __float_as_uint(v[3]));
+    o.z = pack_bf16(__float_as_uint(v[4]), __float_as_uint(v[5])); o.w = pack_bf16(__float_as_uint(v[6]), __float_as_uint(v[7]));
+    *(uint4 *)(a.out + i) = o;
+}
+
+// ---------------------------------------------------------------------------------------------------- launches
+const void *gemm_of(int mode, bool pair)
+{
+    if (mode == SCORES) return pair ? (const void *)vocab_loss_gemm<SCORES, true> : (const void *)vocab_loss_gemm<SCORES, false>;
+    if (mode == DX) return pair ? (const void *)vocab_loss_gemm<DX, true> : (const void *)vocab_loss_gemm<DX, false>;
+    return pair ? (const void *)vocab_loss_gemm<DW, true> : (const void *)vocab_loss_gemm<DW, false>;
+}
+
+struct LossDevice { int sms = 0, pairs = 0; };
+
+// Asked once per device; sets the kernels' shared-memory limits on the way.
+HcclResult loss_device(LossDevice *out)
+{
+    static std::mutex mu;
+    static LossDevice known[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return HCCL_E_RUNTIME;
+    std::lock_guard<std::mutex> lk(mu);
+    LossDevice &d = known[dev];
+    if (!d.sms) {
+        int sms = 0, pairs = 0;
+        cudaError_t e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+        for (int mode = SCORES; mode <= DW && e == cudaSuccess; ++mode)
+            for (int pair = 0; pair < 2 && e == cudaSuccess; ++pair)
+                e = cudaFuncSetAttribute(gemm_of(mode, pair), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes);
+        if (e == cudaSuccess) {
+            cudaLaunchConfig_t q;
+            memset(&q, 0, sizeof(q));
+            q.gridDim = dim3((unsigned)(sms / 2 * 2)); q.blockDim = dim3(kThreads); q.dynamicSmemBytes = kSmemBytes;
+            cudaLaunchAttribute at[1];
+            at[0].id = cudaLaunchAttributeClusterDimension;
+            at[0].val.clusterDim.x = 2; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+            q.attrs = at; q.numAttrs = 1;
+            e = cudaOccupancyMaxActiveClusters(&pairs, gemm_of(SCORES, true), &q);
+        }
+        if (e != cudaSuccess || pairs < 1) { HLOG_ERROR("vocabulary loss set-up failed: %s", cudaGetErrorString(e)); return HCCL_E_RUNTIME; }
+        d.pairs = std::min(pairs, sms / 2);
+        d.sms = sms;
+    }
+    *out = d;
+    return HCCL_SUCCESS;
+}
+
+// Tensor map of bf16 [rows, cols], `stride` elements between rows: boxes of 64 columns x box_rows, 128-byte swizzle, zeros outside.
+HcclResult encode(CUtensorMap *map, const void *base, int64_t rows, int64_t cols, int64_t stride, int box_rows)
+{
+    const DriverApi &d = driver_api();
+    if (!d.ok || !d.TensorMapEncodeTiled) return HCCL_E_DRV;
+    cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride * 2};
+    cuuint32_t box[2] = {(cuuint32_t)BK, (cuuint32_t)box_rows}, estr[2] = {1, 1};
+    CUresult r = d.TensorMapEncodeTiled(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(base), dims, strides, box, estr,
+                                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    CHK_RET_LOG(r != CUDA_SUCCESS, HCCL_E_DRV, "cuTensorMapEncodeTiled failed: %s", cu_err(r));
+    return HCCL_SUCCESS;
+}
+
+// Columns of a tile of the scores: whole waves (the widest among equals).
+int score_cols(int64_t um, int64_t vocab, int units)
+{
+    int best = kMaxCols;
+    int64_t least = INT64_MAX;
+    for (int cols = kMaxCols; cols >= 128; cols -= 32) {
+        const int64_t tiles = um * ((vocab + cols - 1) / cols), t = (tiles + units - 1) / units * cols;
+        if (t < least) { least = t; best = cols; }
+    }
+    return best;
+}
+
+struct Layout { int cols, n_tiles; int64_t ld, stats, xc, shares, bytes; bool pair; int split; };
+
+int shares_of(int64_t tokens, int64_t vocab, int32_t hidden, const LossDevice &d, bool pair)
+{
+    const int units = pair ? d.pairs : d.sms;
+    const int64_t tiles = (tokens + (pair ? 255 : 127)) / (pair ? 256 : 128) * ((hidden + kMaxCols - 1) / kMaxCols), k = (vocab + BK - 1) / BK;
+    int best = 1;
+    double least = 1e30;
+    for (int s = 1; s <= 64 && s <= k / 8; ++s) {
+        // ns: waves of k steps, then the shares written and read
+        const double waves = (double)((tiles * s + units - 1) / units);
+        const double t = waves * ((double)(k + s - 1) / s * (pair ? 260. : 290.) + 800.) + (s > 1 ? 3000. + 8. * s * tokens * hidden / 5e3 : 0.);
+        if (t < least) { least = t; best = s; }
+    }
+    return std::max(1, best);
+}
+
+HcclResult layout_of(int64_t tokens, int64_t vocab, int32_t hidden, bool grad, Layout *l)
+{
+    LossDevice d;
+    CHK_RET(loss_device(&d));
+    auto up = [](int64_t n) { return (n + 1023) / 1024 * 1024; };
+    l->pair = tokens > BM;
+    l->cols = score_cols((tokens + (l->pair ? 255 : 127)) / (l->pair ? 256 : 128), vocab, l->pair ? d.pairs : d.sms);
+    l->n_tiles = (int)((vocab + l->cols - 1) / l->cols);
+    l->ld = (vocab + 63) / 64 * 64;
+    l->split = grad ? shares_of(tokens, vocab, hidden, d, l->pair) : 1;
+    l->stats = grad ? up(tokens * l->ld * 2) : 0;
+    l->xc = l->stats + up(tokens * l->n_tiles * 2 * (int64_t)sizeof(float2));
+    l->shares = l->xc + (grad ? up(tokens * hidden * 2) : 0);
+    l->bytes = l->shares + (l->split > 1 ? up((int64_t)l->split * tokens * hidden * 4) : 0);
+    return HCCL_SUCCESS;
+}
+
+HcclResult launch_gemm(int mode, bool pair, LossGemm &P, void *stream)
+{
+    LossDevice d;
+    CHK_RET(loss_device(&d));
+    const int ctas = pair ? 2 : 1;
+    P.um_tiles = (P.M + ctas * BM - 1) / (ctas * BM);
+    P.n_tiles = (P.N + P.cols - 1) / P.cols;
+    P.units = pair ? d.pairs : d.sms;
+    P.stage_bytes = kABytes + (uint32_t)(P.cols / ctas) * BK * 2;
+    P.stages = (int)std::min<uint32_t>(kMaxStages, kStageSpace / P.stage_bytes);
+    P.idesc = instr_desc((uint32_t)(ctas * BM), (uint32_t)P.cols) | (mode == DW ? 1u << 15 : 0u) | (mode != SCORES ? 1u << 16 : 0u);
+    // a panel's columns of B stay in L2 (40 MB of it) while the rows stream past
+    P.panel = (int)std::min<int64_t>(P.n_tiles, std::max<int64_t>(8, (40ll << 20) / ((int64_t)P.cols * P.k_iters * BK * 2)));
+    const int64_t total = (int64_t)P.um_tiles * P.n_tiles * P.split;
+    CHK_RET_LOG(total > INT32_MAX / 2, HCCL_E_PARA, "vocabulary loss: too many tiles");
+    return launch_pdl(gemm_of(mode, pair), dim3((unsigned)(std::min<int64_t>(P.units, total) * ctas)), kThreads, kSmemBytes, &P, stream, "vocabulary loss", ctas);
+}
+
+RowArgs row_args(const VocabLossCall &c)
+{
+    RowArgs a;
+    memset(&a, 0, sizeof(a));
+    a.y = c.targets; a.wide = c.wide; a.weights = c.weights;
+    a.tokens = c.tokens; a.first = c.first; a.vocab = c.vocab; a.whole = c.whole; a.ignore = c.ignore;
+    return a;
+}
+
+}  // namespace
+
+int64_t vocab_loss_chunk(int64_t vocab, bool grad)
+{
+    // two thousand million bytes of exponentials, or 128 MB of sums of half tiles (16 bytes for 256 columns, or for 128 at worst)
+    const int64_t ld = (vocab + 63) / 64 * 64, rows = grad ? (int64_t)(1ll << 31) / (ld * 2) : (int64_t)(128ll << 20) / (ld / 128 * 16 + 16);
+    return std::min<int64_t>(1 << 20, std::max<int64_t>(256, rows / 256 * 256));
+}
+
+int64_t vocab_loss_scratch_bytes(int64_t tokens, int64_t vocab, int32_t hidden, bool grad)
+{
+    Layout l;
+    return layout_of(tokens, vocab, hidden, grad, &l) == HCCL_SUCCESS ? std::max<int64_t>(1024, l.bytes) : -1;
+}
+
+HcclResult vocab_loss_scores(const VocabLossCall &c, bool grad, float *lse, float *target, float *losses, void *scratch, void *stream)
+{
+    Layout l;
+    CHK_RET(layout_of(c.tokens, c.vocab, c.hidden, grad, &l));
+    uint8_t *s = (uint8_t *)scratch;
+    LossGemm P;
+    memset(&P, 0, sizeof(P));
+    P.M = (int)c.tokens; P.N = (int)c.vocab; P.cols = l.cols; P.split = 1;
+    P.k_iters = (c.hidden + BK - 1) / BK;
+    P.stats = (float2 *)(s + l.stats); P.target = target;
+    P.e = grad ? (__half *)s : nullptr; P.ld = l.ld;
+    P.y = c.targets; P.wide_y = c.wide; P.first = c.first; P.ignore = c.ignore;
+    CHK_RET(encode(&P.tmA, c.x, c.tokens, c.hidden, c.x_stride, BM));
+    CHK_RET(encode(&P.tmB, c.w, c.vocab, c.hidden, c.w_stride, l.cols / (l.pair ? 2 : 1)));
+    CHK_RET(launch_gemm(SCORES, l.pair, P, stream));
+    RowArgs a = row_args(c);
+    a.stats = P.stats; a.halves = 2 * l.n_tiles;
+    a.lse = lse; a.target = target; a.losses = losses;
+    return launch_pdl((const void *)vocab_loss_rows, dim3((unsigned)c.tokens), kRowThreads, 0, &a, stream, "vocabulary loss (rows)");
+}
+
+HcclResult vocab_loss_combine(const VocabLossCall &c, const float *parts, int shards, float *lse, float *losses, void *stream)
+{
+    RowArgs a = row_args(c);
+    a.parts = parts; a.shards = shards; a.lse = lse; a.losses = losses;
+    return launch_pdl((const void *)vocab_loss_join, dim3((unsigned)((c.tokens + kRowThreads - 1) / kRowThreads)), kRowThreads, 0, &a, stream, "vocabulary loss (shards)");
+}
+
+HcclResult vocab_loss_total(const VocabLossCall &c, float *total, void *stream)
+{
+    RowArgs a = row_args(c);
+    a.out = total;
+    return launch_pdl((const void *)vocab_loss_reduce, dim3(1), kSumThreads, 0, &a, stream, "vocabulary loss (weights)");
+}
+
+HcclResult vocab_loss_sum(const VocabLossCall &c, const float *losses, const float *total, float *loss, void *stream)
+{
+    RowArgs a = row_args(c);
+    a.losses_in = losses; a.total = total; a.out = loss;
+    return launch_pdl((const void *)vocab_loss_reduce, dim3(1), kSumThreads, 0, &a, stream, "vocabulary loss (sum)");
+}
+
+HcclResult vocab_loss_grad(const VocabLossCall &c, const float *lse, const float *target, const float *total, float scale, void *dx, void *dw, float *dw_sum,
+                           int out, void *scratch, void *stream)
+{
+    Layout l;
+    CHK_RET(layout_of(c.tokens, c.vocab, c.hidden, true, &l));
+    uint8_t *s = (uint8_t *)scratch;
+    RowArgs a = row_args(c);
+    a.stats = (const float2 *)(s + l.stats); a.halves = 2 * l.n_tiles; a.cols = l.cols; a.n_tiles = l.n_tiles;
+    a.e = s; a.ld = l.ld; a.lse = (float *)lse; a.target = (float *)target; a.total = total; a.scale = scale;
+    a.x = (const uint8_t *)c.x; a.x_stride = c.x_stride * 2; a.xc = s + l.xc; a.xvec = c.hidden / 8;
+    CHK_RET(launch_pdl((const void *)vocab_loss_d, dim3((unsigned)c.tokens), kDThreads, 0, &a, stream, "vocabulary loss (d)"));
+
+    LossGemm P;
+    memset(&P, 0, sizeof(P));
+    P.M = (int)c.tokens; P.N = c.hidden; P.cols = kMaxCols;
+    P.k_iters = (int)((c.vocab + BK - 1) / BK);
+    P.split = l.split;
+    P.kind = l.split > 1 ? VL_F32 : VL_BF16;
+    P.out = (__nv_bfloat16 *)dx; P.sum = (float *)(s + l.shares);
+    P.wide = c.hidden % 16 == 0 && ((uintptr_t)dx & 31) == 0;
+    CHK_RET(encode(&P.tmA, s, c.tokens, l.ld, l.ld, BM));
+    CHK_RET(encode(&P.tmB, c.w, c.vocab, c.hidden, c.w_stride, BK));
+    CHK_RET(launch_gemm(DX, l.pair, P, stream));
+    if (l.split > 1) {
+        ShareArgs q = {P.sum, P.out, c.tokens * c.hidden, l.split};
+        CHK_RET(launch_pdl((const void *)vocab_loss_shares, dim3((unsigned)((q.n / 8 + 255) / 256)), 256, 0, &q, stream, "vocabulary loss (dx)"));
+    }
+
+    memset(&P, 0, sizeof(P));
+    P.M = (int)c.vocab; P.N = c.hidden; P.cols = kMaxCols; P.split = 1;
+    P.k_iters = (int)((c.tokens + BK - 1) / BK);
+    P.kind = out; P.out = (__nv_bfloat16 *)dw; P.sum = dw_sum;
+    P.wide = c.hidden % 16 == 0 && ((uintptr_t)dw & 31) == 0;
+    CHK_RET(encode(&P.tmA, s, c.tokens, l.ld, l.ld, BK));
+    CHK_RET(encode(&P.tmB, s + l.xc, c.tokens, c.hidden, c.hidden, BK));
+    return launch_gemm(DW, c.vocab > BM, P, stream);
+}
+
+}  // namespace hcclb

@@ -146,6 +146,36 @@ extern HcclResult HcclB200MoeBalance(const int32_t *counts, const float *probSum
 extern HcclResult HcclB200MoeGateGrad(const void *logits, HcclDataType dataType, int64_t tokens, int32_t nExperts, int64_t stride, int32_t topk,
                                       int32_t normalize, const uint8_t *mask, const int32_t *idx, const float *dGates, const int32_t *counts,
                                       const int32_t *routed, float dBalance, void *dLogits, aclrtStream stream);
+/* Linear layer and softmax cross entropy over the vocabulary, with gradients, without logits in memory: s = x w^T, loss_t = log sum
+ * exp s_t - s_t[target].  One call works on a chunk of at most HcclB200VocabLossChunk() tokens and on one shard of the vocabulary.
+ * A token counts when its target is an id of the whole vocabulary and not ignoreId.  x and w are bf16, their rows 16-byte aligned;
+ * hidden is a multiple of 8. */
+typedef struct HcclB200VocabLossDef {
+    const void *x, *w;                       /* [tokens, hidden], [vocab, hidden] */
+    int64_t xStride, wStride;                /* elements between rows */
+    const void *targets;                     /* [tokens], INT32 or INT64 */
+    const float *weights;                    /* of the tokens; NULL: ones */
+    int64_t tokens, vocab, firstId, wholeVocab, ignoreId;
+    int32_t hidden, targetType;
+} HcclB200VocabLoss;
+extern int64_t HcclB200VocabLossChunk(int64_t vocab, int32_t withGrad);
+extern int64_t HcclB200VocabLossScratchBytes(int64_t tokens, int64_t vocab, int32_t hidden, int32_t withGrad);
+/* lse [tokens] and target [tokens] (the target's logit, -inf where another shard has it) against this shard; losses [tokens] (0 for
+ * tokens that do not count) where the shard is the whole vocabulary, else NULL.  withGrad: scratch then holds what
+ * HcclB200VocabLossGrad needs. */
+extern HcclResult HcclB200VocabLossScores(const HcclB200VocabLoss *p, int32_t withGrad, float *lse, float *target, float *losses, void *scratch,
+                                          aclrtStream stream);
+/* Joint lse and losses from the shards' parts [shards][2][tokens] = (lse, target). */
+extern HcclResult HcclB200VocabLossCombine(const HcclB200VocabLoss *p, const float *parts, int32_t shards, float *lse, float *losses, aclrtStream stream);
+/* *total = sum of the weights of the tokens that count; *loss = sum of weights * losses, divided by *total where total is given (0 where
+ * that is 0).  Only tokens, targets, weights and wholeVocab are looked at, any number of tokens. */
+extern HcclResult HcclB200VocabLossTotal(const HcclB200VocabLoss *p, float *total, aclrtStream stream);
+extern HcclResult HcclB200VocabLossSum(const HcclB200VocabLoss *p, const float *losses, const float *total, float *loss, aclrtStream stream);
+/* Gradients of scale * sum(weights * losses) (divided by *total where given): dx bf16 [tokens, hidden] of this shard alone (sum it over
+ * the shards), and dw [vocab, hidden], by dwKind: 0 bf16 to dw, 1 fp32 to dwSum, 2 added to dwSum, 3 added to dwSum's values and written
+ * to dw as bf16 (dwSum is left as it was).  lse: joint; scratch: as HcclB200VocabLossScores left it for the same p, with withGrad. */
+extern HcclResult HcclB200VocabLossGrad(const HcclB200VocabLoss *p, const float *lse, const float *target, const float *total, float scale, void *dx,
+                                        void *dw, float *dwSum, int32_t dwKind, void *scratch, aclrtStream stream);
 /* In-kernel timestamps of the newest executor launch (needs HCCL_KERNEL_TRACE=1 at communicator creation):
  * out[0] = kernel start (globaltimer ns), then per step {after wait, after data movement, after signal}. */
 extern HcclResult HcclB200GetKernelTrace(HcclComm comm, uint32_t localRank, uint64_t *out, size_t capWords, int32_t *nsteps);

@@ -64,11 +64,61 @@ def test_gate_outputs():
     assert lib.HcclB200MoeGateScratchBytes(4, 0) == -1 and lib.HcclB200MoeGateScratchBytes(4, 5000) == -1 and lib.HcclB200MoeGateScratchBytes(0, 8) > 0
 
 
+def loss(entry="Scores", args=None, **bad):
+    """The entry of a loss call whose structure has the fields `bad`, whose pointers after it those of `args`."""
+    d = dict(x=AT, w=AT, xStride=8, wStride=8, targets=AT, weights=None, tokens=4, vocab=16, firstId=0, wholeVocab=16, ignoreId=-100, hidden=8, targetType=L.INT64)
+    d.update(bad)
+    p = C.byref(L.VocabLoss(**d))
+    a = dict(lse=AT, target=AT, losses=AT, scratch=AT0, parts=AT, shards=2, total=AT, loss=AT, dx=AT, dw=AT, sum=AT, kind=0)
+    a.update(args or {})
+    lib = L.lib()
+    return {"Scores": lambda: lib.HcclB200VocabLossScores(p, 1, a["lse"], a["target"], a["losses"], a["scratch"], None),
+            "Combine": lambda: lib.HcclB200VocabLossCombine(p, a["parts"], a["shards"], a["lse"], a["losses"], None),
+            "Total": lambda: lib.HcclB200VocabLossTotal(p, a["total"], None),
+            "Sum": lambda: lib.HcclB200VocabLossSum(p, a["losses"], a["total"], a["loss"], None),
+            "Grad": lambda: lib.HcclB200VocabLossGrad(p, a["lse"], a["target"], a["total"], 1.0, a["dx"], a["dw"], a["sum"], a["kind"], a["scratch"], None)}[entry]()
+
+
+AT0 = (C.addressof(MEM) + 255) // 256 * 256
+
+
+@pytest.mark.parametrize("entry", ["Scores", "Grad"])
+@pytest.mark.parametrize("bad,want", [({"x": None}, "PTR"), ({"w": None}, "PTR"), ({"targets": None}, "PTR"), ({"targetType": L.FP32}, "NOT_SUPPORT"),
+                                      ({"hidden": 12}, "PARA"), ({"hidden": 0}, "PARA"), ({"hidden": 16}, "PARA"), ({"xStride": 12}, "PARA"), ({"wStride": 0}, "PARA"),
+                                      ({"vocab": 0}, "PARA"), ({"vocab": 17}, "PARA"), ({"firstId": 1}, "PARA"), ({"firstId": -1}, "PARA"), ({"wholeVocab": 15}, "PARA"),
+                                      ({"tokens": -1}, "PARA"), ({"tokens": (1 << 20) + 1}, "PARA"), ({"x": AT + 8}, "PARA"), ({"w": AT + 2}, "PARA"),
+                                      ({"targets": AT + 4}, "PARA"), ({"weights": AT + 2}, "PARA")])
+def test_vocab_loss(entry, bad, want):
+    assert loss(entry, **bad) == getattr(L, "E_" + want)
+
+
+def test_vocab_loss_outputs():
+    assert loss("Scores", vocab=8) == L.E_PARA                              # a shard has no losses of its own
+    for entry, names in (("Scores", ("lse", "target", "scratch")), ("Combine", ("parts", "lse", "losses")), ("Total", ("total",)), ("Sum", ("losses", "loss")),
+                         ("Grad", ("lse", "target", "dx", "dw", "scratch"))):
+        for n in names:
+            assert loss(entry, {n: None}) == L.E_PTR and loss(entry, {n: AT0 + 2}) == L.E_PARA, (entry, n)
+    assert loss("Grad", {"scratch": AT0 + 128}) == L.E_PARA and loss("Combine", {"shards": 0}) == L.E_PARA and loss("Grad", tokens=0) == L.E_PARA
+    assert loss("Grad", {"kind": 4}) == L.E_PARA and loss("Grad", {"kind": -1}) == L.E_PARA
+    for kind in (1, 2, 3):
+        assert loss("Grad", {"kind": kind, "sum": None}) == L.E_PTR
+    assert loss("Grad", {"kind": 3, "dw": None}) == L.E_PTR
+    assert loss("Scores", tokens=0, x=None, targets=None) == L.SUCCESS and loss("Combine", tokens=0, targets=None) == L.SUCCESS
+    lib = L.lib()
+    assert lib.HcclB200VocabLossScores(None, 0, AT, AT, None, AT0, None) == L.E_PTR
+    assert lib.HcclB200VocabLossChunk(0, 1) == -1 and lib.HcclB200VocabLossChunk(1 << 31, 1) == -1
+    for vocab in (1, 1000, 128256, 1 << 24):
+        for grad in (0, 1):
+            assert lib.HcclB200VocabLossChunk(vocab, grad) >= 256 and lib.HcclB200VocabLossChunk(vocab, grad) % 256 == 0
+    assert lib.HcclB200VocabLossScratchBytes(4, 16, 12, 1) == -1 and lib.HcclB200VocabLossScratchBytes((1 << 20) + 1, 16, 8, 1) == -1
+
+
 def test_python_arguments():
     torch = pytest.importorskip("torch")
     from cann_hccl_b200.parallel import moe, vocab
     w, ids = torch.zeros(10, 8), torch.zeros(3, dtype=torch.int64)        # host tensors are refused whatever they hold
     for call in (lambda: vocab.embedding(ids, w), lambda: vocab.embedding_grad(ids, torch.zeros(3, 8), 10), lambda: vocab.embedding_grad(ids, torch.zeros(4, 8), 10),
-                 lambda: moe.gate(torch.zeros(4, 8), 2), lambda: moe.gate(None, 2)):
+                 lambda: moe.gate(torch.zeros(4, 8), 2), lambda: moe.gate(None, 2),
+                 lambda: vocab.linear_cross_entropy(torch.zeros(3, 8), w, ids), lambda: vocab.linear_cross_entropy_grad(torch.zeros(3, 8), w, ids)):
         with pytest.raises(ValueError):
             call()
