@@ -1,14 +1,21 @@
 // Linear layer and softmax cross entropy over the vocabulary, with gradients, without keeping the logits:
-//   s = x W^T;  lse_t = log sum_v exp s_tv;  loss_t = lse_t - s_t,y;  d_tv = g_t (exp(s_tv - lse_t) - [v = y]);  dx = d W;  dW = d^T x
+//   s = x W^T;  lse_t = log sum_v exp s_tv;  loss_t = lse_t - s_t,y;  d_tv = q_t (exp(s_tv - lse_t) - [v = y]);  dx = a d W;  dW = a d^T x
+// (q: weight of the token; a: scale, divided by the sum of the weights for a mean; applied to the fp32 sums, so that the d of a target
+// far from sure is -q and not -q a: an ordinary weight of one is not rounded at all)
+//
+// x        with gradients (or where rows do not start on 128-byte lines) the tokens' rows are copied, those of tokens that do not count as
+//          zeros: 0 x inf is not 0.
 //
 // scores   tcgen05 product of a chunk of tokens with all tiles of the vocabulary.  The epilogue takes a row's half tile from TMEM,
 //          leaves its maximum m and sum of exp(s - m) (fp32) and, for gradients, 2^15 exp(s - m) in fp16: relative to the half
 //          tile's own maximum 11 bits hold every probability down to 2^-29 of it, so that the one rounding that counts
 //          is the later one of d to bf16.  Logits are never stored, and nothing is computed twice (6 T V H operations in all;
 //          a second product in place of the exponentials would make it 8).
-// rows     lse, target logit and loss of a token from its half tiles.
-// d        exponentials to d in place (bf16), rescaled by exp(m - lse); the target's column is g expm1(s_y - lse), which keeps its
-//          digits for sure guesses.  Tokens that do not count become rows of zeros here, and their x too: 0 x inf is not 0.
+// rows     lse and loss of a token from its half tiles.  The target's logit is summed once more in fp32 FMAs of short chains and put in the
+//          place of the tensor cores' one in lse too: their running sum cuts digits off instead of rounding, and a loss near zero is
+//          the difference of two logits that would carry that (8192 tokens of 4096: error of the losses against 64 bits 3.0e-6 before).
+// d        exponentials to d in place (bf16), rescaled by exp(m - lse); the target's column is q expm1(s_y - lse), which keeps its
+//          digits for sure guesses.  Tokens that do not count become rows of zeros.
 // dx, dW   tcgen05 products that read W, d and x as they lie: an operand whose depth is not its contiguous side goes to the tensor
 //          cores MN-major (boxes of 64 elements x 64 deep).  dx with few tiles is cut along the vocabulary into fp32 shares that a
 //          last launch adds in order; dW over several chunks is summed in fp32.
@@ -61,7 +68,9 @@ struct alignas(64) LossGemm {
     float *sum;                      // shares of dx: [share][row][N]
     int kind;                        // VocabLossOut
     int64_t ld;
-    int wide;                        // rows of out and sum start on 32-byte boundaries
+    int wide;                        // rows of out start on 32-byte boundaries
+    const float *total;              // the sums are multiplied by scale / *total (null: scale; a total of 0: 0)
+    float scale;
 };
 
 struct LossShared {
@@ -104,6 +113,10 @@ __device__ __forceinline__ void st_v8(void *p, const uint32_t (&v)[8])
 {
     asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr)
+{
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
 __device__ __forceinline__ float exp2_approx(float x)
 {
     float y;
@@ -112,67 +125,23 @@ __device__ __forceinline__ float exp2_approx(float x)
 }
 __device__ __forceinline__ int64_t target_of(const void *y, int wide, int64_t t) { return wide ? ((const int64_t *)y)[t] : (int64_t)((const int32_t *)y)[t]; }
 
-// 16 or 32 columns of a row from TMEM
-__device__ __forceinline__ void tmem_cols(uint32_t addr, float (&v)[32])
+// Half a tile's columns of a row stay in registers: the accumulator is free again before any of them is worked on.
+constexpr int kHalf = kMaxCols / 2;
+__device__ __forceinline__ void tmem_half(uint32_t addr, float (&v)[kHalf])
 {
-    uint32_t r[32];
-    tmem_ld32(addr, r);
+    uint32_t r[kHalf / 32][32];
+#pragma unroll
+    for (int q = 0; q < kHalf / 32; ++q) tmem_ld32(addr + q * 32, r[q]);
     tmem_ld_wait();
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-}
-__device__ __forceinline__ void tmem_cols(uint32_t addr, float (&v)[16])
-{
-    uint32_t r[16];
-    tmem_ld16(addr, r);
-    tmem_ld_wait();
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
-}
-
-template <int C> __device__ __forceinline__ void row_max(uint32_t taddr, int left, float &m)
-{
-    float v[C];
-    tmem_cols(taddr, v);
-    if (left >= C) {
-#pragma unroll
-        for (int i = 0; i < C; ++i) m = fmaxf(m, v[i]);
-    } else
-#pragma unroll
-        for (int i = 0; i < C; ++i) m = fmaxf(m, i < left ? v[i] : -INFINITY);
-}
-// Exponentials of C columns against m; left: columns that exist; y: the target's column from here; e: where they go (null: nowhere).
-template <int C>
-__device__ __forceinline__ void row_exp(uint32_t taddr, int left, float m, int y, float &z, float &target, __half *e, int room)
-{
-    float v[C];
-    tmem_cols(taddr, v);
-    if ((uint32_t)y < (uint32_t)C)
-#pragma unroll
-        for (int i = 0; i < C; ++i) target = i == y ? v[i] : target;
-#pragma unroll
-    for (int i = 0; i < C; ++i) {
-        v[i] = exp2_approx(fmaf(v[i] - m, kLog2e, kExpBits));
-        if (left < C && i >= left) v[i] = 0.f;
-        z += v[i];
-    }
-    if (e)
-#pragma unroll
-        for (int c = 0; c < C; c += 16)
-            if (c < room) {
-                uint32_t o[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const __half2 h = __floats2half2_rn(v[c + 2 * i], v[c + 2 * i + 1]);
-                    o[i] = *(const uint32_t *)&h;
-                }
-                st_v8(e + c, o);
-            }
+    for (int i = 0; i < kHalf; ++i) v[i] = __uint_as_float(r[i / 32][i % 32]);
 }
 
 // 16 results of a row, of which `left` exist (a multiple of 8).
-__device__ __forceinline__ void put16(const LossGemm &P, int64_t at, float *sum, float (&v)[16], int left)
+__device__ __forceinline__ void put16(const LossGemm &P, int64_t at, float *sum, float *v, int left, float scale)
 {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] *= scale;
     if (P.kind == VL_ADD || P.kind == VL_ADD_BF16)
 #pragma unroll
         for (int c = 0; c < 16; c += 4)
@@ -303,6 +272,17 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_loss_gemm(const __grid_cons
         const int mid = (P.cols / 16 + 1) / 2 * 16, c_lo = half ? mid : 0, c_hi = half ? P.cols : mid;
         uint32_t n = 0;
         bool bad = false;
+        // This warp has read the accumulator.  Relaxed: the loads are complete, and a release would wait for the results stored so far
+        // to reach memory, a microsecond and more on every tile (1531 x 50257 x 1000: scores 153 us, tensor cores busy for 51 %).
+        auto release = [&](uint32_t buf) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0 && !bad) {
+                if (kPair) mbar_arrive_cluster_relaxed(mapa_u32(smem_u32(&S.tmem_empty[buf]), 0)); else mbar_arrive(&S.tmem_empty[buf]);
+            }
+        };
+        float scale = P.scale;
+        if (MODE != SCORES && P.total) scale = *P.total != 0.f ? scale / *P.total : 0.f;
         for (int t = unit; t < total; t += P.units, ++n) {
             const Tile w = tile_at(P, t);
             const int row = (w.um * kCtas + (int)cta_r) * BM + rl, col0 = w.nt * P.cols;
@@ -316,53 +296,61 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_loss_gemm(const __grid_cons
             bad = __any_sync(0xffffffffu, bad);
             tc_fence_after();
             if (MODE == SCORES) {
-                const int left = P.N - col0;  // columns that exist from the tile's first on
-                float m = -INFINITY, z = 0.f, target = 0.f;
-                if (!bad) {
-                    const int c_end = min(c_hi, (left + 15) / 16 * 16);
-                    int c = c_lo;
-#pragma unroll 1
-                    for (; c + 32 <= c_end; c += 32) row_max<32>(taddr + c, left - c, m);
-                    if (c < c_end) row_max<16>(taddr + c, left - c, m);
-                    const float ref = m == -INFINITY ? 0.f : m;
-                    __half *e = P.e && row < P.M ? P.e + (int64_t)row * P.ld + col0 : nullptr;
-                    const int room = (int)min((int64_t)c_hi, P.ld - col0);  // the row ends behind the last column, on a multiple of 64
-                    const int yl = y >= c_lo && y < c_hi && y < left ? (int)y : -1;
-                    c = c_lo;
-#pragma unroll 1
-                    for (; c + 32 <= c_end; c += 32) row_exp<32>(taddr + c, left - c, ref, yl < 0 ? -1 : yl - c, z, target, e ? e + c : nullptr, room - c);
-                    if (c < c_end) {
-                        row_exp<16>(taddr + c, left - c, ref, yl < 0 ? -1 : yl - c, z, target, e ? e + c : nullptr, room - c);
-                        c += 16;
-                    }
-                    if (e) {
-                        const uint32_t zero[8] = {};
-                        for (; c < room; c += 16) st_v8(e + c, zero);
-                    }
-                    z *= kExpScale;
-                    if (yl >= 0) P.target[row] = target;
-                } else
-                    z = __uint_as_float(0x7fffffffu);
-                if (row < P.M) P.stats[(int64_t)row * (2 * P.n_tiles) + 2 * w.nt + half] = make_float2(m, z);
-            } else {
-                float *sum = P.sum + (P.split > 1 ? (int64_t)w.share * P.M * P.N : 0);
-                const int c_end = min(c_hi, P.N - col0);
-                const int64_t at = (int64_t)row * P.N + col0;
-                int c = c_lo;
-#pragma unroll 1
-                for (; c < c_end; c += 16) {
-                    float v[16];
-                    if (!bad) tmem_cols(taddr + c, v);
-                    else
+                float v[kHalf];
+                if (!bad) tmem_half(taddr + c_lo, v);
+                release(buf);
+                const int exist = min(c_hi, P.N - col0) - c_lo;  // columns of this half that exist, the first of them
+                const int yl = y >= c_lo && y < c_lo + exist ? (int)y - c_lo : -1;
+                if (exist < kHalf)
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(0x7fffffffu);
-                    if (row < P.M) put16(P, at + c, sum, v, c_end - c);
+                    for (int i = 0; i < kHalf; ++i) v[i] = i < exist ? v[i] : -INFINITY;
+                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, z4[4] = {}, target = 0.f;
+#pragma unroll
+                for (int i = 0; i < kHalf; ++i) m4[i & 3] = fmaxf(m4[i & 3], v[i]);
+                const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), ref = m == -INFINITY ? 0.f : m;
+                if (yl >= 0) {
+#pragma unroll
+                    for (int i = 0; i < kHalf; ++i) target = i == yl ? v[i] : target;
+                    P.target[row] = target;
                 }
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0 && !bad) {
-                if (kPair) mbar_arrive_cluster(mapa_u32(smem_u32(&S.tmem_empty[buf]), 0)); else mbar_arrive(&S.tmem_empty[buf]);
+                // (v - m first: the product with m alone would carry m's size into every exponent)
+#pragma unroll
+                for (int i = 0; i < kHalf; ++i) {
+                    v[i] = exp2_approx(fmaf(v[i] - ref, kLog2e, kExpBits));
+                    z4[i & 3] += v[i];
+                }
+                const float z = bad ? __uint_as_float(0x7fffffffu) : ((z4[0] + z4[1]) + (z4[2] + z4[3])) * kExpScale;
+                if (row < P.M) {
+                    P.stats[(int64_t)row * (2 * P.n_tiles) + 2 * w.nt + half] = make_float2(m, z);
+                    if (P.e) {
+                        __half *e = P.e + (int64_t)row * P.ld + col0 + c_lo;
+                        const int room = (int)min((int64_t)c_hi, P.ld - col0) - c_lo;  // the row ends on a multiple of 64, in zeros
+#pragma unroll
+                        for (int c = 0; c < kHalf; c += 16)
+                            if (c < room) {
+                                uint32_t o[8];
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) {
+                                    const __half2 h = __floats2half2_rn(v[c + 2 * i], v[c + 2 * i + 1]);
+                                    o[i] = *(const uint32_t *)&h;
+                                }
+                                st_v8(e + c, o);
+                            }
+                    }
+                }
+            } else {
+                float v[kHalf];
+                if (!bad) tmem_half(taddr + c_lo, v);
+                else
+#pragma unroll
+                    for (int i = 0; i < kHalf; ++i) v[i] = __uint_as_float(0x7fffffffu);
+                release(buf);
+                float *sum = P.sum + (P.split > 1 ? (int64_t)w.share * P.M * P.N : 0);
+                const int exist = row < P.M ? min(c_hi, P.N - col0) - c_lo : 0;
+                const int64_t at = (int64_t)row * P.N + col0 + c_lo;
+#pragma unroll
+                for (int c = 0; c < kHalf; c += 16)
+                    if (c < exist) put16(P, at + c, sum, v + c, exist - c, scale);
             }
         }
     }
@@ -384,11 +372,10 @@ struct RowArgs {
     const float *weights, *losses_in, *total;
     float *lse, *target, *losses, *out;
     uint8_t *e;                      // [row][ld] 2 bytes each
-    const uint8_t *x;
+    const uint8_t *x, *w;
     uint8_t *xc;
-    int64_t tokens, first, vocab, whole, ignore, ld, x_stride;
+    int64_t tokens, first, vocab, whole, ignore, ld, x_stride, w_stride;  // strides in bytes
     int wide, halves, cols, n_tiles, shards, xvec;
-    float scale;
 };
 
 __device__ __forceinline__ bool counts(const RowArgs &a, int64_t id) { return id != a.ignore && id >= 0 && id < a.whole; }
@@ -411,11 +398,30 @@ constexpr int kRowThreads = 128, kRowRegs = 8;
 // One CTA per token.
 __global__ void __launch_bounds__(kRowThreads) vocab_loss_rows(const __grid_constant__ RowArgs a)
 {
-    __shared__ float s_m[kRowThreads / 32], s_z[kRowThreads / 32];
+    __shared__ float s_m[kRowThreads / 32], s_z[kRowThreads / 32], s_d[kRowThreads / 32];
     pdl_trigger();
     pdl_wait();
     const int64_t t = blockIdx.x;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t id = target_of(a.y, a.wide, t);
+    const uint64_t at = (uint64_t)id - (uint64_t)a.first;
+    const bool here = counts(a, id) && at < (uint64_t)a.vocab;
+    float dot = 0.f;  // the target's logit
+    if (here) {
+        const uint4 *x = (const uint4 *)(a.x + t * a.x_stride), *w = (const uint4 *)(a.w + (int64_t)at * a.w_stride);
+#pragma unroll 4
+        for (int v = threadIdx.x; v < a.xvec; v += kRowThreads) {
+            const uint4 p = x[v], q = w[v];
+            const uint32_t pw[4] = {p.x, p.y, p.z, p.w}, qw[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {  // bf16 is the upper half of an fp32
+                dot = fmaf(__uint_as_float(pw[i] << 16), __uint_as_float(qw[i] << 16), dot);
+                dot = fmaf(__uint_as_float(pw[i] & 0xffff0000u), __uint_as_float(qw[i] & 0xffff0000u), dot);
+            }
+        }
+        dot = warp_sum(dot);
+        if (lane == 0) s_d[warp] = dot;
+    }
     const float2 *p = a.stats + t * a.halves;
     float m = -INFINITY, z = 0.f;
     for (int i0 = 0; i0 < a.halves; i0 += kRowThreads * kRowRegs) {
@@ -447,13 +453,21 @@ __global__ void __launch_bounds__(kRowThreads) vocab_loss_rows(const __grid_cons
     z = s_z[0];
 #pragma unroll
     for (int w = 1; w < kRowThreads / 32; ++w) z += s_z[w];
-    const int64_t id = target_of(a.y, a.wide, t);
-    const uint64_t at = (uint64_t)id - (uint64_t)a.first;
-    const bool here = counts(a, id) && at < (uint64_t)a.vocab;
-    const float log_z = logf(z);
+    float log_z = logf(z), target = -INFINITY;
+    if (here) {
+        target = a.target[t];
+        dot = s_d[0];
+#pragma unroll
+        for (int w = 1; w < kRowThreads / 32; ++w) dot += s_d[w];
+        const float off = dot - target;  // far off only where logits have no digits behind the point: both stay as they are then
+        if (fabsf(off) < 0.5f) {
+            log_z += log1pf(__expf((target - all) - log_z) * expm1f(off));
+            target = dot;
+        }
+    }
     a.lse[t] = all + log_z;
-    if (!here) a.target[t] = -INFINITY;
-    if (a.losses) a.losses[t] = counts(a, id) ? (all - a.target[t]) + log_z : 0.f;
+    a.target[t] = target;
+    if (a.losses) a.losses[t] = counts(a, id) ? (all - target) + log_z : 0.f;
 }
 
 // Joint lse and loss from the shards'.
@@ -503,9 +517,22 @@ __global__ void __launch_bounds__(kSumThreads) vocab_loss_reduce(const __grid_co
     *a.out = sum;
 }
 
+constexpr int kCopyThreads = 256;
+// Rows of x to rows of xc that start on 128-byte boundaries; zeros for tokens that do not count.
+__global__ void __launch_bounds__(kCopyThreads) vocab_loss_x(const __grid_constant__ RowArgs a)
+{
+    pdl_trigger();
+    const int64_t i = (int64_t)blockIdx.x * kCopyThreads + threadIdx.x, t = i / a.xvec;
+    const int v = (int)(i - t * a.xvec);
+    pdl_wait();
+    if (t >= a.tokens) return;
+    const bool on = counts(a, target_of(a.y, a.wide, t)) && (!a.weights || a.weights[t] != 0.f);
+    ((uint4 *)a.xc)[t * (a.ld / 8) + v] = on ? ((const uint4 *)(a.x + t * a.x_stride))[v] : make_uint4(0, 0, 0, 0);
+}
+
 constexpr int kDThreads = 256, kDBatch = 4;
 
-// Exponentials -> d, in place; rows of x that count -> xc.  One CTA per token, a warp's lanes share a tile (8 columns each).
+// Exponentials -> d, in place.  One CTA per token, a warp's lanes share a tile (8 columns each).
 __global__ void __launch_bounds__(kDThreads) vocab_loss_d(const __grid_constant__ RowArgs a)
 {
     pdl_trigger();
@@ -513,22 +540,15 @@ __global__ void __launch_bounds__(kDThreads) vocab_loss_d(const __grid_constant_
     const int64_t t = blockIdx.x;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t id = target_of(a.y, a.wide, t);
-    const float share = !counts(a, id) ? 0.f : a.weights ? a.weights[t] : 1.f;
-    const float total = a.total ? *a.total : 1.f;
-    const float g = share == 0.f || total == 0.f ? 0.f : a.scale * (share / total);
+    const float q = !counts(a, id) ? 0.f : a.weights ? a.weights[t] : 1.f;
     uint4 *row = (uint4 *)(a.e + t * a.ld * 2);
-    {
-        const uint4 *src = (const uint4 *)(a.x + t * a.x_stride);
-        uint4 *dst = (uint4 *)a.xc + t * a.xvec;
-        for (int v = threadIdx.x; v < a.xvec; v += kDThreads) dst[v] = share == 0.f ? make_uint4(0, 0, 0, 0) : src[v];
-    }
-    if (share == 0.f) {
+    if (q == 0.f) {
         for (int v = threadIdx.x; v < a.ld / 8; v += kDThreads) row[v] = make_uint4(0, 0, 0, 0);
         return;
     }
     const float lse = a.lse[t];
     const int64_t y = id - a.first;  // may lie in another shard
-    const float dy = g * expm1f(a.target[t] - lse);
+    const float dy = q * expm1f(a.target[t] - lse);
     const int mid = (a.cols / 16 + 1) / 2 * 16, c = lane * 8, half = c >= mid;
     const float2 *stats = a.stats + t * a.halves + half;
     for (int n0 = warp; n0 < a.n_tiles; n0 += kDThreads / 32 * kDBatch) {
@@ -547,7 +567,7 @@ __global__ void __launch_bounds__(kDThreads) vocab_loss_d(const __grid_constant_
             const int n = n0 + k * (kDThreads / 32);
             const int64_t col = (int64_t)n * a.cols + c;
             if (n < a.n_tiles && c < a.cols && col < a.ld) {
-                const float fac = __expf(f[k] - lse) * g * kExpScale;
+                const float fac = __expf(f[k] - lse) * q * kExpScale;
                 float d[8];
                 const __half2 *h = (const __half2 *)&v[k];
 #pragma unroll
@@ -658,7 +678,7 @@ int score_cols(int64_t um, int64_t vocab, int units)
     return best;
 }
 
-struct Layout { int cols, n_tiles; int64_t ld, stats, xc, shares, bytes; bool pair; int split; };
+struct Layout { int cols, n_tiles; int64_t ld, xld, stats, xc, shares, bytes; bool pair, copy; int split; };
 
 int shares_of(int64_t tokens, int64_t vocab, int32_t hidden, const LossDevice &d, bool pair)
 {
@@ -687,7 +707,11 @@ HcclResult layout_of(int64_t tokens, int64_t vocab, int32_t hidden, bool grad, L
     l->split = grad ? shares_of(tokens, vocab, hidden, d, l->pair) : 1;
     l->stats = grad ? up(tokens * l->ld * 2) : 0;
     l->xc = l->stats + up(tokens * l->n_tiles * 2 * (int64_t)sizeof(float2));
-    l->shares = l->xc + (grad ? up(tokens * hidden * 2) : 0);
+    l->xld = (hidden + 63) / 64 * 64;
+    // Gradients need the copy for the tokens that do not count.  Rows of x that cross 128-byte lines cost the TMA two requests instead of
+    // one, which bounds the product (1531 x 50257 x 1000: scores 150 us, DW 127): more than one row of tiles is worth the copy.
+    l->copy = grad || (hidden % 64 != 0 && l->pair);
+    l->shares = l->xc + (l->copy ? up(tokens * l->xld * 2) : 0);
     l->bytes = l->shares + (l->split > 1 ? up((int64_t)l->split * tokens * hidden * 4) : 0);
     return HCCL_SUCCESS;
 }
@@ -746,12 +770,19 @@ HcclResult vocab_loss_scores(const VocabLossCall &c, bool grad, float *lse, floa
     P.stats = (float2 *)(s + l.stats); P.target = target;
     P.e = grad ? (__half *)s : nullptr; P.ld = l.ld;
     P.y = c.targets; P.wide_y = c.wide; P.first = c.first; P.ignore = c.ignore;
-    CHK_RET(encode(&P.tmA, c.x, c.tokens, c.hidden, c.x_stride, BM));
+    if (l.copy) {
+        RowArgs a = row_args(c);
+        a.x = (const uint8_t *)c.x; a.x_stride = c.x_stride * 2; a.xc = s + l.xc; a.ld = l.xld; a.xvec = c.hidden / 8;
+        CHK_RET(launch_pdl((const void *)vocab_loss_x, dim3((unsigned)((c.tokens * a.xvec + kCopyThreads - 1) / kCopyThreads)), kCopyThreads, 0, &a, stream,
+                           "vocabulary loss (x)"));
+    }
+    CHK_RET(encode(&P.tmA, l.copy ? s + l.xc : c.x, c.tokens, c.hidden, l.copy ? l.xld : c.x_stride, BM));
     CHK_RET(encode(&P.tmB, c.w, c.vocab, c.hidden, c.w_stride, l.cols / (l.pair ? 2 : 1)));
     CHK_RET(launch_gemm(SCORES, l.pair, P, stream));
     RowArgs a = row_args(c);
     a.stats = P.stats; a.halves = 2 * l.n_tiles;
     a.lse = lse; a.target = target; a.losses = losses;
+    a.x = (const uint8_t *)c.x; a.w = (const uint8_t *)c.w; a.x_stride = c.x_stride * 2; a.w_stride = c.w_stride * 2; a.xvec = c.hidden / 8;
     return launch_pdl((const void *)vocab_loss_rows, dim3((unsigned)c.tokens), kRowThreads, 0, &a, stream, "vocabulary loss (rows)");
 }
 
@@ -784,13 +815,13 @@ HcclResult vocab_loss_grad(const VocabLossCall &c, const float *lse, const float
     uint8_t *s = (uint8_t *)scratch;
     RowArgs a = row_args(c);
     a.stats = (const float2 *)(s + l.stats); a.halves = 2 * l.n_tiles; a.cols = l.cols; a.n_tiles = l.n_tiles;
-    a.e = s; a.ld = l.ld; a.lse = (float *)lse; a.target = (float *)target; a.total = total; a.scale = scale;
-    a.x = (const uint8_t *)c.x; a.x_stride = c.x_stride * 2; a.xc = s + l.xc; a.xvec = c.hidden / 8;
+    a.e = s; a.ld = l.ld; a.lse = (float *)lse; a.target = (float *)target;
     CHK_RET(launch_pdl((const void *)vocab_loss_d, dim3((unsigned)c.tokens), kDThreads, 0, &a, stream, "vocabulary loss (d)"));
 
     LossGemm P;
     memset(&P, 0, sizeof(P));
     P.M = (int)c.tokens; P.N = c.hidden; P.cols = kMaxCols;
+    P.total = total; P.scale = scale;
     P.k_iters = (int)((c.vocab + BK - 1) / BK);
     P.split = l.split;
     P.kind = l.split > 1 ? VL_F32 : VL_BF16;
@@ -806,11 +837,12 @@ HcclResult vocab_loss_grad(const VocabLossCall &c, const float *lse, const float
 
     memset(&P, 0, sizeof(P));
     P.M = (int)c.vocab; P.N = c.hidden; P.cols = kMaxCols; P.split = 1;
+    P.total = total; P.scale = scale;
     P.k_iters = (int)((c.tokens + BK - 1) / BK);
     P.kind = out; P.out = (__nv_bfloat16 *)dw; P.sum = dw_sum;
     P.wide = c.hidden % 16 == 0 && ((uintptr_t)dw & 31) == 0;
     CHK_RET(encode(&P.tmA, s, c.tokens, l.ld, l.ld, BK));
-    CHK_RET(encode(&P.tmB, s + l.xc, c.tokens, c.hidden, c.hidden, BK));
+    CHK_RET(encode(&P.tmB, s + l.xc, c.tokens, c.hidden, l.xld, BK));
     return launch_gemm(DW, c.vocab > BM, P, stream);
 }
 

@@ -5,10 +5,12 @@
 // Gradient: counts are constants; dl = p (u - sum_e p_e u_e) with u_e = coef * E / (k n^2) * counts[e], and through the gates
 // g_j (dg_j - sum_i g_i dg_i) at the chosen experts (normalised), or u raised by dg_j there (not normalised).
 //
-// A warp takes a token, a lane the experts lane, lane + 32, ... in registers: one pass over the logits; a round of the top-k is a
-// maximum over the lanes of an order-preserving integer key.  Sums of probabilities and counts stay in the warp and in shared
-// memory, each CTA leaves one partial row, and one cluster adds them in a fixed order (no floating-point atomics).
-// Bound: launches and latency for decode batches, instruction issue of the top-k rounds for large ones.
+// A warp takes a token, a lane the experts lane, lane + 32, ... : one pass over the logits.  A lane knows the largest of its order-
+// preserving integer keys, so a round of the top-k is a maximum over the lanes; the keys of the lane that has it lie in shared memory,
+// where the whole warp finds the expert and that lane's next largest in a few instructions (with every lane searching its own
+// registers: 65536 tokens x 256, top 8, 167 us).  Sums of probabilities stay in registers, counts in shared memory; each CTA leaves one
+// partial row, a second launch adds them in a fixed order (no floating-point atomics).  Up to kOneCta tokens one CTA does it all.
+// Bound: launches and latency for decode batches, instruction issue for large ones.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -24,7 +26,8 @@ namespace hcclb {
 namespace {
 
 constexpr uint32_t kAll = 0xffffffffu;
-constexpr int kGateThreads = 256, kMaxBlocks = 296, kEndThreads = 1024, kEndCluster = 8;
+constexpr int kGateThreads = 256, kMaxBlocks = 592, kOneThreads = 512, kOneCta = 64;
+constexpr int kEndExperts = 8, kEndSlices = 32, kEndThreads = kEndExperts * kEndSlices;
 
 __device__ __forceinline__ float ld_f(const float *p) { return *p; }
 __device__ __forceinline__ float ld_f(const __half *p) { return __half2float(*p); }
@@ -49,6 +52,11 @@ __device__ __forceinline__ float warp_sum(float x)
     return x;
 }
 
+__device__ __forceinline__ float value_of(uint32_t key)
+{
+    return __uint_as_float(key == kAll ? 0x7fffffffu : key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
+
 struct GateArgs {
     const void *logits;
     const uint8_t *mask;
@@ -56,7 +64,9 @@ struct GateArgs {
     float *gates;
     float *part_p;                  // [cta][experts]
     int32_t *part_c, *part_n;       // [cta][experts], [cta]
-    const int32_t *counts, *routed;
+    uint32_t *arrived;              // of the CTAs that add the parts
+    float *prob_sum, *balance;
+    int32_t *counts, *routed;
     const float *d_gates;
     void *d_logits;
     int64_t tokens, stride;
@@ -64,65 +74,98 @@ struct GateArgs {
     float coef;
 };
 
-// V: experts of a lane; kWarps x experts floats and experts words of shared memory
-template <int V> constexpr int kGateWarps = V > 32 ? 4 : kGateThreads / 32;
-
-template <class T, int V>
-__global__ void __launch_bounds__(kGateWarps<V> * 32) moe_gate_kernel(const __grid_constant__ GateArgs a)
+__device__ __forceinline__ float balance_of(float sum, int n, int experts, int topk)
 {
-    constexpr int W = kGateWarps<V>;
-    extern __shared__ float sh[];
+    return n ? sum / (float)n / (float)n * ((float)experts / (float)topk) : 0.f;
+}
+
+// V: experts of a lane.  Sums of probabilities: in registers up to 32 of them, else in the warp's row of shared memory.
+template <int V> constexpr bool kInRegs = V <= 32;
+template <int V> constexpr int kGateMost = V <= 32 ? 512 : 128;      // threads of a CTA
+template <int V> constexpr int kGateCtas = V <= 8 ? 2 : 1;           // CTAs of that size on an SM
+// Dynamic shared memory: [warps][experts] keys, [warps][experts] sums, [experts] counts.
+template <class T, int V>
+__global__ void __launch_bounds__(kGateMost<V>, kGateCtas<V>) moe_gate_kernel(const __grid_constant__ GateArgs a)
+{
+    extern __shared__ uint32_t sh[];
     __shared__ int s_n;
-    const int E = a.experts, k = a.topk, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    float *s_p = sh + warp * E;
-    int32_t *s_c = (int32_t *)(sh + W * E);
-    for (int i = threadIdx.x; i < W * E; i += W * 32) sh[i] = 0.f;
-    for (int i = threadIdx.x; i < E; i += W * 32) s_c[i] = 0;
+    __shared__ float s_b[kOneThreads / 32];
+    const int E = a.experts, k = a.topk, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5;
+    uint32_t *key = sh + warp * E;
+    float *s_p = (float *)(sh + W * E);
+    int32_t *s_c = (int32_t *)(sh + 2 * W * E);
+    if (!kInRegs<V>)
+        for (int i = threadIdx.x; i < W * E; i += blockDim.x) s_p[i] = 0.f;
+    for (int i = threadIdx.x; i < E; i += blockDim.x) s_c[i] = 0;
     if (threadIdx.x == 0) s_n = 0;
     __syncthreads();
     pdl_trigger();
     pdl_wait();
+    if (blockIdx.x == 0 && threadIdx.x == 0 && a.arrived) *a.arrived = 0;
     int mine = 0;  // routed tokens
+    float sums[kInRegs<V> ? V : 1] = {};
     for (int64_t t = (int64_t)blockIdx.x * W + warp; t < a.tokens; t += (int64_t)gridDim.x * W) {
         const T *row = (const T *)a.logits + t * a.stride;
         const bool on = !a.mask || a.mask[t];
         float x[V];
-        uint32_t best = 0, where = 0;  // of this lane's experts: largest key, its place
+        uint32_t best = 0;  // largest key of this lane
+        __syncwarp();       // the keys of the token before are not read any more
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const int e = j * 32 + lane;
             x[j] = e < E ? ld_f(row + e) : -INFINITY;
-            const uint32_t q = e < E ? key_of(x[j]) : 0;
-            if (q > best) { best = q; where = j; }
         }
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int e = j * 32 + lane;
+            const uint32_t q = e < E ? key_of(x[j]) : 0;
+            if (e < E) key[e] = q;
+            best = max(best, q);
+        }
+        __syncwarp();
         uint32_t top = __reduce_max_sync(kAll, best);
         const bool routed = on && top > kInfKey;
-        float m = top == kAll ? __uint_as_float(0x7fffffffu) : 0.f;  // NaN in the row
-        if (top != kAll) m = __uint_as_float(top & 0x80000000u ? top & 0x7fffffffu : ~top);
+        const float m = value_of(top);
         int sel = -1;           // of slot `lane`
         float sel_x = -INFINITY;
         if (routed) {
-            uint32_t taken[(V + 31) / 32];
-#pragma unroll
-            for (int j = 0; j < (V + 31) / 32; ++j) taken[j] = 0;
             for (int s = 0; s < k; ++s) {
                 if (s) top = __reduce_max_sync(kAll, best);
                 if (top <= kInfKey) break;
-                const uint32_t e = __reduce_min_sync(kAll, best == top ? where * 32 + lane : kAll);
-                if (lane == s) {
-                    sel = (int)e;
-                    sel_x = top == kAll ? __uint_as_float(0x7fffffffu) : __uint_as_float(top & 0x80000000u ? top & 0x7fffffffu : ~top);
-                }
-                if ((e & 31) == (uint32_t)lane) {
-                    if (V > 32) taken[(e >> 5) >> 5] |= 1u << ((e >> 5) & 31);
-                    else taken[0] |= 1u << (e >> 5);
-                    best = 0;
-#pragma unroll
-                    for (int j = 0; j < V; ++j) {
-                        const uint32_t q = j * 32 + lane < E && !(taken[j / 32] >> (j & 31) & 1) ? key_of(x[j]) : 0;
-                        if (q > best) { best = q; where = j; }
+                const uint32_t who = __ballot_sync(kAll, best == top);
+                int e;
+                if ((who & (who - 1)) == 0) {  // one lane has it: which of its experts is the first with that key
+                    const int w = __ffs(who) - 1;
+                    e = -1;
+                    uint32_t next = 0;
+                    for (int j0 = 0; j0 < V; j0 += 32) {
+                        const int j = j0 + lane, at = j * 32 + w;
+                        uint32_t q = j < V && at < E ? key[at] : 0;
+                        if (e < 0) {
+                            const uint32_t hit = __ballot_sync(kAll, q == top);
+                            if (hit) {
+                                e = (j0 + __ffs(hit) - 1) * 32 + w;
+                                if (at == e) key[at] = q = 0;
+                            }
+                        }
+                        next = max(next, q);
+                    }
+                    next = __reduce_max_sync(kAll, next);
+                    if (lane == w) best = next;
+                } else {                       // equal keys: the lowest expert of all
+                    uint32_t first = kAll;
+                    if (best == top)
+                        for (int at = lane; at < E; at += 32)
+                            if (key[at] == top) { first = at; break; }
+                    e = (int)__reduce_min_sync(kAll, first);
+                    if (first == (uint32_t)e) {
+                        key[e] = 0;
+                        best = 0;
+                        for (int at = lane; at < E; at += 32) best = max(best, key[at]);
                     }
                 }
+                __syncwarp();
+                if (lane == s) { sel = e; sel_x = value_of(top); }
             }
             float z = 0.f;
 #pragma unroll
@@ -133,8 +176,10 @@ __global__ void __launch_bounds__(kGateWarps<V> * 32) moe_gate_kernel(const __gr
             z = warp_sum(z);
             const float inv = 1.f / z;
 #pragma unroll
-            for (int j = 0; j < V; ++j)
-                if (j * 32 + lane < E) s_p[j * 32 + lane] += x[j] * inv;
+            for (int j = 0; j < V; ++j) {
+                if (kInRegs<V>) sums[kInRegs<V> ? j : 0] += x[j] * inv;
+                else if (j * 32 + lane < E) s_p[warp * E + j * 32 + lane] += x[j] * inv;
+            }
             const float g = sel >= 0 ? __expf(sel_x - m) : 0.f;
             const float whole = a.normalize ? warp_sum(g) : z;
             if (lane < k) a.gates[t * k + lane] = g / whole;
@@ -144,16 +189,37 @@ __global__ void __launch_bounds__(kGateWarps<V> * 32) moe_gate_kernel(const __gr
             a.gates[t * k + lane] = 0.f;
         if (lane < k) a.idx[t * k + lane] = sel;
     }
+    if (kInRegs<V>)
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (j * 32 + lane < E) s_p[warp * E + j * 32 + lane] = sums[kInRegs<V> ? j : 0];
     if (lane == 0) atomicAdd(&s_n, mine);
     __syncthreads();
-    for (int e = threadIdx.x; e < E; e += W * 32) {
+    const bool alone = gridDim.x == 1;
+    float sum = 0.f;
+    for (int e = threadIdx.x; e < E; e += blockDim.x) {
         float p = 0.f;
-#pragma unroll
-        for (int w = 0; w < W; ++w) p += sh[w * E + e];
-        a.part_p[(int64_t)blockIdx.x * E + e] = p;
-        a.part_c[(int64_t)blockIdx.x * E + e] = s_c[e];
+        for (int w = 0; w < W; ++w) p += s_p[w * E + e];
+        if (alone) {
+            a.prob_sum[e] = p;
+            a.counts[e] = s_c[e];
+            sum += (float)s_c[e] * p;
+        } else {
+            a.part_p[(int64_t)blockIdx.x * E + e] = p;
+            a.part_c[(int64_t)blockIdx.x * E + e] = s_c[e];
+        }
     }
-    if (threadIdx.x == 0) a.part_n[blockIdx.x] = s_n;
+    if (!alone) {
+        if (threadIdx.x == 0) a.part_n[blockIdx.x] = s_n;
+        return;
+    }
+    sum = warp_sum(sum);
+    if (lane == 0) s_b[warp] = sum;
+    __syncthreads();
+    if (threadIdx.x) return;
+    for (int w = 1; w < W; ++w) sum += s_b[w];
+    *a.routed = s_n;
+    *a.balance = balance_of(sum, s_n, E, k);
 }
 
 struct EndArgs {
@@ -161,92 +227,98 @@ struct EndArgs {
     const int32_t *part_c, *part_n;
     float *prob_sum, *balance;      // prob_sum, counts, routed: null where the parts are the sums
     int32_t *counts, *routed;
+    float *shares;                  // [cta] of sum_e counts * prob_sum
+    uint32_t *arrived;              // 0 before the launch; null for one CTA
     int parts, experts, topk;
 };
 
-__device__ __forceinline__ float load_cluster_f(const float *own, int cta)
-{
-    uint32_t at;
-    float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(own)), "r"(cta));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
-    return v;
-}
-
-// One cluster: a warp's lanes hold 32 consecutive experts, the warps of such a group share the parts.
+// A CTA adds the parts of kEndExperts experts at a time, kEndSlices threads for each; the one that arrives last adds the shares, in
+// the order of the CTAs.
 __global__ void __launch_bounds__(kEndThreads) moe_gate_end_kernel(const __grid_constant__ EndArgs a)
 {
-    __shared__ float s_p[32][33], s_b;
-    __shared__ int s_c[32][33], s_n[32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, E = a.experts, cta = blockIdx.x;
+    __shared__ float s_p[kEndSlices][kEndExperts + 1], s_w[kEndThreads / 32];
+    __shared__ int s_c[kEndSlices][kEndExperts + 1], s_n[kEndThreads / 32], s_last;
+    const int x = threadIdx.x % kEndExperts, slice = threadIdx.x / kEndExperts, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, E = a.experts;
     pdl_trigger();
     pdl_wait();
-    int n = 0;
-    for (int i = threadIdx.x; i < a.parts; i += kEndThreads) n += a.part_n[i];
-    n = __reduce_add_sync(kAll, n);
-    if (lane == 0) s_n[warp] = n;
-    float sum = 0.f;  // thread's share of sum_e counts * prob_sum
-    for (int e0 = cta * 32; e0 < E; e0 += kEndCluster * 32) {
-        const int e = e0 + lane;
+    float sum = 0.f;
+    for (int e0 = blockIdx.x * kEndExperts; e0 < E; e0 += gridDim.x * kEndExperts) {
+        const int e = e0 + x;
         float p = 0.f;
         int c = 0;
         if (e < E)
-#pragma unroll 4
-            for (int i = warp; i < a.parts; i += kEndThreads / 32) { p += a.part_p[(int64_t)i * E + e]; c += a.part_c[(int64_t)i * E + e]; }
-        s_p[warp][lane] = p;
-        s_c[warp][lane] = c;
+#pragma unroll 8
+            for (int i = slice; i < a.parts; i += kEndSlices) { p += a.part_p[(int64_t)i * E + e]; c += a.part_c[(int64_t)i * E + e]; }
+        s_p[slice][x] = p;
+        s_c[slice][x] = c;
         __syncthreads();
-        if (warp == 0) {
+        if (threadIdx.x < kEndExperts && e < E) {
             p = 0.f; c = 0;
 #pragma unroll
-            for (int w = 0; w < kEndThreads / 32; ++w) { p += s_p[w][lane]; c += s_c[w][lane]; }
-            if (e < E) {
-                if (a.counts) { a.counts[e] = c; a.prob_sum[e] = p; }
-                sum += (float)c * p;
-            }
+            for (int q = 0; q < kEndSlices; ++q) { p += s_p[q][x]; c += s_c[q][x]; }
+            if (a.counts) { a.counts[e] = c; a.prob_sum[e] = p; }
+            sum += (float)c * p;
         }
         __syncthreads();
     }
-    if (warp == 0) {
-        sum = warp_sum(sum);
-        if (lane == 0) s_b = sum;
+    if (warp == 0) sum = warp_sum(sum);  // lanes behind the experts hold 0
+    if (threadIdx.x == 0) {
+        s_last = 1;
+        if (a.arrived) {
+            a.shares[blockIdx.x] = sum;
+            __threadfence();
+            s_last = atomicAdd(a.arrived, 1u) == gridDim.x - 1;
+            __threadfence();
+        }
     }
-    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    if (cta == 0 && threadIdx.x == 0) {
-        float b = 0.f;
-        for (int q = 0; q < kEndCluster; ++q) b += load_cluster_f(&s_b, q);
-        int all = 0;
-        for (int w = 0; w < kEndThreads / 32; ++w) all += s_n[w];
-        if (a.routed) *a.routed = all;
-        // n^2 leaves 32 bits for a few thousand million tokens only, but counts * p / n / n keeps its digits either way
-        *a.balance = all ? b / (float)all / (float)all * ((float)E / (float)a.topk) : 0.f;
-    }
-    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    __syncthreads();
+    if (!s_last) return;
+    int n = 0;
+    for (int i = threadIdx.x; i < a.parts; i += kEndThreads) n += a.part_n[i];
+    n = __reduce_add_sync(kAll, n);
+    float all = 0.f;
+    if (a.arrived)
+        for (int i = threadIdx.x; i < (int)gridDim.x; i += kEndThreads) all += __ldcg(a.shares + i);
+    all = warp_sum(all);
+    if (lane == 0) { s_n[warp] = n; s_w[warp] = all; }
+    __syncthreads();
+    if (threadIdx.x) return;
+    n = 0; all = 0.f;
+    for (int w = 0; w < kEndThreads / 32; ++w) { n += s_n[w]; all += s_w[w]; }
+    if (a.routed) *a.routed = n;
+    *a.balance = balance_of(a.arrived ? all : sum, n, E, a.topk);
 }
 
+// Dynamic shared memory: [experts] u, [warps][experts] what the gates add at the chosen experts.
 template <class T, int V>
-__global__ void __launch_bounds__(kGateWarps<V> * 32) moe_gate_grad_kernel(const __grid_constant__ GateArgs a)
+__global__ void __launch_bounds__(kGateMost<V>, kGateCtas<V>) moe_gate_grad_kernel(const __grid_constant__ GateArgs a)
 {
-    constexpr int W = kGateWarps<V>;
-    extern __shared__ float s_u[];
-    const int E = a.experts, k = a.topk, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    extern __shared__ uint32_t sh[];
+    const int E = a.experts, k = a.topk, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5;
+    float *s_u = (float *)sh, *extra = s_u + E + warp * E;
+    for (int i = lane; i < E; i += 32) extra[i] = 0.f;
     pdl_trigger();
     pdl_wait();
     const int n = *a.routed;
     const float per = n ? a.coef * ((float)E / (float)k) / (float)n / (float)n : 0.f;
-    for (int e = threadIdx.x; e < E; e += W * 32) s_u[e] = per * (float)a.counts[e];
+    for (int e = threadIdx.x; e < E; e += blockDim.x) s_u[e] = per * (float)a.counts[e];
     __syncthreads();
     for (int64_t t = (int64_t)blockIdx.x * W + warp; t < a.tokens; t += (int64_t)gridDim.x * W) {
         const T *row = (const T *)a.logits + t * a.stride;
         T *out = (T *)a.d_logits + t * E;
-        const int sel = lane < k ? a.idx[t * k + lane] : -1;
-        const float dg = a.d_gates && sel >= 0 && sel < E ? a.d_gates[t * k + lane] : 0.f;
+        int sel = lane < k ? a.idx[t * k + lane] : -1;
+        if (sel >= E) sel = -1;
+        const float dg = a.d_gates && sel >= 0 ? a.d_gates[t * k + lane] : 0.f;
         float x[V], m = -INFINITY;
         bool nan = false;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const int e = j * 32 + lane;
             x[j] = e < E ? ld_f(row + e) : -INFINITY;
+        }
+        const float sel_x = sel >= 0 ? ld_f(row + sel) : -INFINITY;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
             m = fmaxf(m, x[j]);
             nan = nan || x[j] != x[j];
         }
@@ -259,8 +331,6 @@ __global__ void __launch_bounds__(kGateWarps<V> * 32) moe_gate_grad_kernel(const
                 if (j * 32 + lane < E) st_f(out + j * 32 + lane, 0.f);
             continue;
         }
-        float sel_x = -INFINITY;
-        if (sel >= 0 && sel < E) sel_x = ld_f(row + sel);
         float z = 0.f;
 #pragma unroll
         for (int j = 0; j < V; ++j) { x[j] = __expf(x[j] - m); z += x[j]; }
@@ -270,6 +340,7 @@ __global__ void __launch_bounds__(kGateWarps<V> * 32) moe_gate_grad_kernel(const
         const float whole = a.normalize ? warp_sum(g) : z;
         g = g > 0.f ? g / whole : g;
         const float gd = warp_sum(g * dg);
+        if (sel >= 0) extra[sel] = a.normalize ? g * (dg - gd) : g * dg;
         float dot = 0.f;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -277,40 +348,41 @@ __global__ void __launch_bounds__(kGateWarps<V> * 32) moe_gate_grad_kernel(const
             x[j] *= inv;
             if (e < E) dot += x[j] * s_u[e];
         }
-        dot = warp_sum(dot);
+        dot = warp_sum(dot);  // its shuffles also put `extra` before the reads below
+        __syncwarp();
         if (!a.normalize) dot += gd;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const int e = j * 32 + lane;
-            if (e < E) x[j] *= s_u[e] - dot;
+            if (e < E) st_f(out + e, fmaf(x[j], s_u[e] - dot, extra[e]));
         }
-        const float add = a.normalize ? g * (dg - gd) : g * dg;  // at the chosen expert
-        for (int s = 0; s < k; ++s) {
-            const int e = __shfl_sync(kAll, sel, s);
-            const float v = __shfl_sync(kAll, add, s);
-            if (e >= 0 && (e & 31) == lane)
-#pragma unroll
-                for (int j = 0; j < V; ++j) x[j] += j == e >> 5 ? v : 0.f;
-        }
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-            if (j * 32 + lane < E) st_f(out + j * 32 + lane, x[j]);
+        __syncwarp();
+        if (sel >= 0) extra[sel] = 0.f;
+        __syncwarp();
     }
 }
 
-int gate_blocks(int64_t tokens, int warps) { return (int)std::min<int64_t>(kMaxBlocks, std::max<int64_t>(1, (tokens + warps - 1) / warps)); }
+// Threads and CTAs of a call.
+struct GateGrid { int threads, ctas; };
+GateGrid gate_grid(int64_t tokens, int experts, bool grad)
+{
+    const int most = experts > 1024 ? 128 : kOneThreads;
+    if (!grad && tokens <= kOneCta) return {(int)std::min<int64_t>(most, std::max<int64_t>(1, tokens) * 32), 1};
+    const int threads = std::min(kGateThreads, most), warps = threads / 32;
+    return {threads, (int)std::min<int64_t>(grad ? 148 * 6 : kMaxBlocks, (tokens + warps - 1) / warps)};
+}
 
 template <class T, int V> HcclResult run_gate(GateArgs &a, bool grad, void *stream)
 {
-    constexpr int W = kGateWarps<V>;
-    const size_t smem = grad ? (size_t)a.experts * 4 : (size_t)(W + 1) * a.experts * 4;
+    const GateGrid g = gate_grid(a.tokens, a.experts, grad);
+    const int W = g.threads / 32;
+    const size_t smem = (size_t)(grad ? W + 1 : 2 * W + 1) * a.experts * 4;
     const void *fn = grad ? (const void *)moe_gate_grad_kernel<T, V> : (const void *)moe_gate_kernel<T, V>;
     if (smem > 48 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         CHK_RET_LOG(e != cudaSuccess, HCCL_E_RUNTIME, "router set-up failed: %s", cudaGetErrorString(e));
     }
-    const unsigned blocks = grad ? (unsigned)std::min<int64_t>(148 * 8, (a.tokens + W - 1) / W) : (unsigned)gate_blocks(a.tokens, W);
-    return launch_pdl(fn, dim3(blocks), W * 32, smem, &a, stream, grad ? "router gradient" : "router");
+    return launch_pdl(fn, dim3((unsigned)g.ctas), (unsigned)g.threads, smem, &a, stream, grad ? "router gradient" : "router");
 }
 
 template <class T> HcclResult gate_typed(GateArgs &a, bool grad, void *stream)
@@ -337,7 +409,12 @@ HcclResult gate_any(const GateShape &s, GateArgs &a, bool grad, void *stream)
 
 }  // namespace
 
-int64_t moe_gate_scratch_bytes(int64_t, int32_t experts) { return (int64_t)kMaxBlocks * (experts * 8 + 4); }
+// [cta][experts] sums and counts, [cta] tokens, shares of the CTAs that add them, arrivals
+int64_t moe_gate_scratch_bytes(int64_t tokens, int32_t experts)
+{
+    const int ctas = gate_grid(tokens, experts, false).ctas;
+    return ctas == 1 ? 16 : (int64_t)ctas * (experts * 8 + 4) + kGateMaxExperts / kEndExperts * 4 + 16;
+}
 
 HcclResult moe_gate(const GateShape &s, const void *logits, const uint8_t *mask, int32_t *idx, float *gates, int32_t *counts, float *prob_sum,
                     int32_t *routed, float *balance, void *scratch, void *stream)
@@ -345,17 +422,23 @@ HcclResult moe_gate(const GateShape &s, const void *logits, const uint8_t *mask,
     GateArgs a;
     memset(&a, 0, sizeof(a));
     a.logits = logits; a.mask = mask; a.idx = idx; a.gates = gates;
-    a.part_p = (float *)scratch;
-    a.part_c = (int32_t *)scratch + (int64_t)kMaxBlocks * s.experts;
-    a.part_n = a.part_c + (int64_t)kMaxBlocks * s.experts;
-    CHK_RET(gate_any(s, a, false, stream));
+    a.prob_sum = prob_sum; a.balance = balance; a.counts = counts; a.routed = routed;
+    const int ctas = gate_grid(s.tokens, s.experts, false).ctas;
+    if (ctas == 1) return gate_any(s, a, false, stream);
     EndArgs e;
     memset(&e, 0, sizeof(e));
+    a.part_p = (float *)scratch;
+    a.part_c = (int32_t *)scratch + (int64_t)ctas * s.experts;
+    a.part_n = a.part_c + (int64_t)ctas * s.experts;
+    e.shares = (float *)(a.part_n + ctas);
+    e.arrived = (uint32_t *)(e.shares + kGateMaxExperts / kEndExperts);
+    a.arrived = e.arrived;
+    CHK_RET(gate_any(s, a, false, stream));
     e.part_p = a.part_p; e.part_c = a.part_c; e.part_n = a.part_n;
     e.prob_sum = prob_sum; e.balance = balance; e.counts = counts; e.routed = routed;
-    e.parts = gate_blocks(s.tokens, s.experts > 1024 ? 4 : kGateThreads / 32);
+    e.parts = ctas;
     e.experts = s.experts; e.topk = s.topk;
-    return launch_pdl((const void *)moe_gate_end_kernel, dim3(kEndCluster), kEndThreads, 0, &e, stream, "router (sums)", kEndCluster);
+    return launch_pdl((const void *)moe_gate_end_kernel, dim3((unsigned)((s.experts + kEndExperts - 1) / kEndExperts)), kEndThreads, 0, &e, stream, "router (sums)");
 }
 
 HcclResult moe_balance(const int32_t *counts, const float *prob_sum, const int32_t *routed, int32_t experts, int32_t topk, float *balance, void *stream)
@@ -364,7 +447,7 @@ HcclResult moe_balance(const int32_t *counts, const float *prob_sum, const int32
     memset(&e, 0, sizeof(e));
     e.part_p = prob_sum; e.part_c = counts; e.part_n = routed; e.balance = balance;
     e.parts = 1; e.experts = experts; e.topk = topk;
-    return launch_pdl((const void *)moe_gate_end_kernel, dim3(kEndCluster), kEndThreads, 0, &e, stream, "router (balance)", kEndCluster);
+    return launch_pdl((const void *)moe_gate_end_kernel, dim3(1), kEndThreads, 0, &e, stream, "router (balance)");
 }
 
 HcclResult moe_gate_grad(const GateShape &s, const void *logits, const int32_t *idx, const float *d_gates, const int32_t *counts, const int32_t *routed,
@@ -373,7 +456,8 @@ HcclResult moe_gate_grad(const GateShape &s, const void *logits, const int32_t *
     if (!s.tokens) return HCCL_SUCCESS;
     GateArgs a;
     memset(&a, 0, sizeof(a));
-    a.logits = logits; a.mask = mask; a.idx = (int32_t *)idx; a.d_gates = d_gates; a.counts = counts; a.routed = routed; a.coef = coef; a.d_logits = d_logits;
+    a.logits = logits; a.mask = mask; a.idx = (int32_t *)idx; a.d_gates = d_gates; a.counts = (int32_t *)counts; a.routed = (int32_t *)routed;
+    a.coef = coef; a.d_logits = d_logits;
     return gate_any(s, a, true, stream);
 }
 

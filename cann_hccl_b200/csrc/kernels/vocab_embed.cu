@@ -135,8 +135,8 @@ __global__ void __launch_bounds__(kLookupThreads) embed_lookup_kernel(const __gr
 // warp's counters in shared memory the earlier stretches, so equal digits keep their order.
 constexpr int kDigitBits = 9, kBins = 1 << kDigitBits;
 constexpr int kSortItems = 8;
-constexpr int kOneThreads = 1024, kTileThreads = 256;
-constexpr int kOneMost = kOneThreads * kSortItems;    // tokens that one CTA sorts
+constexpr int kTileThreads = 256;
+constexpr int kOneMost = 1024 * kSortItems;           // tokens that one CTA sorts
 constexpr int kTile = kTileThreads * kSortItems;
 
 struct SortArgs {
@@ -202,18 +202,20 @@ template <int N> __device__ __forceinline__ void bins_prefix(int (&t)[N], int32_
     for (int i = 0; i < N; ++i) t[i] += base;
 }
 
-constexpr size_t kOneSmem = (size_t)(kOneThreads / 32) * kBins * 4 + kBins * 4 + (size_t)kOneMost * 8;
+template <int THREADS> constexpr size_t kOneSmem = (size_t)(THREADS / 32) * kBins * 4 + kBins * 4 + (size_t)THREADS * kSortItems * 8;
 
-// Up to kOneMost tokens: all passes in one CTA, pairs in registers, exchanged through shared memory.
-__global__ void __launch_bounds__(kOneThreads) embed_sort_one_kernel(const __grid_constant__ SortArgs a)
+// Up to kOneMost tokens: all passes in one CTA, pairs in registers, exchanged through shared memory.  Fewer warps where there are fewer
+// tokens: the prefix over the warps' counters is the longest step of a pass.
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) embed_sort_one_kernel(const __grid_constant__ SortArgs a)
 {
     extern __shared__ int32_t sh[];
-    __shared__ int32_t s_warp[kOneThreads / 32];
-    constexpr int W = kOneThreads / 32;
+    constexpr int W = THREADS / 32, N = kBins > THREADS ? kBins / THREADS : 1;  // N bins of a thread
+    __shared__ int32_t s_warp[W];
     int32_t *counts = sh, *base = counts + W * kBins;
     uint2 *pairs = (uint2 *)(base + kBins);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int n = (int)a.tokens, items = (n + kOneThreads - 1) / kOneThreads, at = warp * items * 32 + lane;
+    const int n = (int)a.tokens, items = (n + THREADS - 1) / THREADS, at = warp * items * 32 + lane;
     pdl_trigger();
     pdl_wait();
     uint32_t key[kSortItems], pos[kSortItems];
@@ -230,14 +232,18 @@ __global__ void __launch_bounds__(kOneThreads) embed_sort_one_kernel(const __gri
     for (int pass = 0; pass < a.passes; ++pass) {
         const int shift = pass * a.digit;
         const uint32_t mask = (1u << a.digit) - 1;
-        for (int i = threadIdx.x; i < W * kBins; i += kOneThreads) counts[i] = 0;
+        for (int i = threadIdx.x; i < W * kBins; i += THREADS) counts[i] = 0;
         __syncthreads();
         int rank[kSortItems];
         warp_ranks(key, items, shift, mask, counts, rank);
         __syncthreads();
-        int t[1] = {threadIdx.x < kBins ? warp_prefix<W>(counts, threadIdx.x) : 0};
-        bins_prefix<1>(t, s_warp);
-        if (threadIdx.x < kBins) base[threadIdx.x] = t[0];
+        int t[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) t[j] = (int)threadIdx.x * N + j < kBins ? warp_prefix<W>(counts, threadIdx.x * N + j) : 0;
+        bins_prefix<N>(t, s_warp);
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if ((int)threadIdx.x * N + j < kBins) base[threadIdx.x * N + j] = t[j];
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < kSortItems; ++i) {
@@ -362,6 +368,19 @@ template <class T, int B> __device__ __forceinline__ void put_row(const SumArgs 
         st((T *)a.out + at, pack<T, B>(acc, a.scale));
 }
 
+// Zeros over `bytes` bytes from p, by the whole CTA: 32-byte stores whatever the rows' own alignment is.
+template <int SIZE> __device__ __forceinline__ void zero_bytes(uint8_t *p, int64_t bytes)
+{
+    const int64_t head = min(bytes, (int64_t)(-(uintptr_t)p & 31)), body = (bytes - head) / 32, tail = bytes - head - body * 32;
+    Bytes<32> zero;
+    memset(&zero, 0, sizeof(zero));
+    Bytes<SIZE> one;
+    memset(&one, 0, sizeof(one));
+    for (int64_t i = (int64_t)threadIdx.x * SIZE; i < head; i += blockDim.x * SIZE) st(p + i, one);
+    for (int64_t i = threadIdx.x; i < body; i += blockDim.x) st(p + head + i * 32, zero);
+    for (int64_t i = (int64_t)threadIdx.x * SIZE; i < tail; i += blockDim.x * SIZE) st(p + head + body * 32 + i, one);
+}
+
 // First place in the sorted list whose row is not below `row`.
 __device__ __forceinline__ int64_t lower_bound(const uint2 *pairs, int64_t n, uint32_t row)
 {
@@ -396,13 +415,12 @@ __global__ void __launch_bounds__(kSumThreads) embed_sum_kernel(const __grid_con
             if (threadIdx.x == 0) s_has = mask;
         }
         __syncthreads();
-        Bytes<B> zero;
-        memset(&zero, 0, sizeof(zero));
-        for (int i = 0; i < kZeroRows; ++i)
-            if (!(s_has >> i & 1)) {
-                uint8_t *p = (uint8_t *)a.out + (r0 + i) * a.nvec * B;
-                for (int v = threadIdx.x; v < a.nvec; v += blockDim.x) st(p + (int64_t)v * B, zero);
-            }
+        for (int i = 0; i < kZeroRows;) {
+            if (s_has >> i & 1) { ++i; continue; }
+            const int from = i;
+            while (i < kZeroRows && !(s_has >> i & 1)) ++i;
+            zero_bytes<sizeof(T)>((uint8_t *)a.out + (r0 + from) * a.nvec * B, (int64_t)(i - from) * a.nvec * B);
+        }
         return;
     }
     const int64_t tile = blockIdx.x / a.nslice, t0 = tile * a.rows;
@@ -457,29 +475,46 @@ __global__ void __launch_bounds__(kSumThreads) embed_sum_kernel(const __grid_con
         put_row<T, B>(a, cur, v, acc);
 }
 
-// The runs that begin in a tile and go on behind it: their pieces, in order.
-template <class T, int B>
+// The runs that begin in a tile and go on behind it: their pieces, in order.  N columns of a thread, eight pieces in flight (with one at
+// a time, and 16 columns: 32768 tokens x 4096, the most frequent one 1900 times, 72 us).
+template <class T, int N>
 __global__ void __launch_bounds__(kSumThreads) embed_join_kernel(const __grid_constant__ SumArgs a)
 {
-    constexpr int N = B / sizeof(T);
+    constexpr int kBatch = 8;
     pdl_trigger();
     const int64_t tile = blockIdx.x / a.nslice, t1 = (tile + 1) * a.rows;  // not the last tile
-    const int v = (int)(blockIdx.x - tile * a.nslice) * (int)blockDim.x + threadIdx.x;
+    const int64_t c = ((int64_t)(blockIdx.x - tile * a.nslice) * blockDim.x + threadIdx.x) * N, hidden = a.nvec;
     pdl_wait();
     const uint32_t key = a.pairs[t1 - 1].x;
     if (key >= (uint32_t)a.vocab || a.pairs[t1].x != key || (tile > 0 && a.pairs[tile * a.rows - 1].x == key)) return;
     const int64_t last = (lower_bound(a.pairs, a.tokens, key + 1) - 1) / a.rows;  // tile in which the run ends
-    if (v >= a.nvec) return;
+    if (c >= hidden) return;
     float acc[N];
-    const float *p = a.pieces + ((tile * 2 + 1) * a.nvec + v) * N;
+    const float *p = a.pieces + (tile * 2 + 1) * hidden + c;
 #pragma unroll
     for (int i = 0; i < N; ++i) acc[i] = p[i];
-    for (int64_t q = tile + 1; q <= last; ++q) {
-        const float *h = a.pieces + (q * 2 * a.nvec + v) * N;
+    for (int64_t q0 = tile + 1; q0 <= last; q0 += kBatch) {
+        float h[kBatch][N];
 #pragma unroll
-        for (int i = 0; i < N; ++i) acc[i] += h[i];
+        for (int j = 0; j < kBatch; ++j) {
+            const float *src = a.pieces + (q0 + j) * 2 * hidden + c;
+            if (q0 + j <= last) {
+                if (N == 4) *(float4 *)h[j] = *(const float4 *)src;
+                else h[j][0] = src[0];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j)
+            if (q0 + j <= last)
+#pragma unroll
+                for (int i = 0; i < N; ++i) acc[i] += h[j][i];
     }
-    put_row<T, B>(a, key, v, acc);
+    const int64_t at = (int64_t)key * hidden + c;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (a.add) ((float *)a.out)[at + i] += acc[i] * a.scale;
+        else ((T *)a.out)[at + i] = from_f<T>(acc[i] * a.scale);
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------- launches
@@ -547,9 +582,13 @@ template <class T, int B> HcclResult sum(SumArgs &a, int64_t row_bytes, void *st
     unsigned ctas;
     CHK_RET(grid_of(a.tiles * a.nslice + a.zero_ctas, &ctas, "embedding gradient"));
     if (ctas) CHK_RET(launch_pdl((const void *)embed_sum_kernel<T, B>, dim3(ctas), (unsigned)threads, 0, &a, stream, "embedding gradient"));
-    if (a.tiles > 1)
-        CHK_RET(launch_pdl((const void *)embed_join_kernel<T, B>, dim3((unsigned)((a.tiles - 1) * a.nslice)), (unsigned)threads, 0, &a, stream, "embedding gradient (join)"));
-    return HCCL_SUCCESS;
+    if (a.tiles <= 1) return HCCL_SUCCESS;
+    const int hidden = (int)(row_bytes / (int64_t)sizeof(T)), n = hidden % 4 ? 1 : 4, join = std::min(kSumThreads, (hidden / n + 31) / 32 * 32);
+    a.nvec = hidden;
+    a.nslice = (hidden / n + join - 1) / join;
+    CHK_RET(grid_of((a.tiles - 1) * a.nslice, &ctas, "embedding gradient (join)"));
+    return launch_pdl(n == 4 ? (const void *)embed_join_kernel<T, 4> : (const void *)embed_join_kernel<T, 1>, dim3(ctas), (unsigned)join, 0, &a, stream,
+                      "embedding gradient (join)");
 }
 
 template <class T> HcclResult sum_typed(SumArgs &a, int64_t hidden, void *stream)
@@ -563,6 +602,16 @@ template <class T> HcclResult sum_typed(SumArgs &a, int64_t hidden, void *stream
     }
 }
 
+template <int THREADS> HcclResult sort_one(SortArgs &a, void *stream)
+{
+    const void *fn = (const void *)embed_sort_one_kernel<THREADS>;
+    if (kOneSmem<THREADS> > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kOneSmem<THREADS>);
+        CHK_RET_LOG(e != cudaSuccess, HCCL_E_RUNTIME, "embedding gradient set-up failed: %s", cudaGetErrorString(e));
+    }
+    return launch_pdl(fn, dim3(1), THREADS, kOneSmem<THREADS>, &a, stream, "embedding gradient (sort)");
+}
+
 HcclResult sort_tokens(const EmbedTable &t, const EmbedIds &ids, const Scratch &s, uint8_t *scratch, void *stream, const uint2 **sorted)
 {
     SortArgs a;
@@ -574,11 +623,11 @@ HcclResult sort_tokens(const EmbedTable &t, const EmbedIds &ids, const Scratch &
     a.digit = (bits + a.passes - 1) / a.passes;
     uint2 *buf[2] = {(uint2 *)(scratch + s.pairs), (uint2 *)(scratch + s.spare)};
     if (ids.tokens <= kOneMost) {
-        const cudaError_t e = cudaFuncSetAttribute((const void *)embed_sort_one_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kOneSmem);
-        CHK_RET_LOG(e != cudaSuccess, HCCL_E_RUNTIME, "embedding gradient set-up failed: %s", cudaGetErrorString(e));
         a.out = buf[0];
         *sorted = buf[0];
-        return launch_pdl((const void *)embed_sort_one_kernel, dim3(1), kOneThreads, kOneSmem, &a, stream, "embedding gradient (sort)");
+        if (ids.tokens <= 1024) return sort_one<256>(a, stream);
+        if (ids.tokens <= 4096) return sort_one<512>(a, stream);
+        return sort_one<1024>(a, stream);
     }
     a.hist = (int32_t *)(scratch + s.hist);
     a.tiles = (int)((ids.tokens + kTile - 1) / kTile);
