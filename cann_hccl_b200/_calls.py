@@ -51,3 +51,19 @@ class Calls:
         at = [_addresses(t, nlocal, True) for t in (topk_idx, gates, out)]
         rows = C.cast(C.c_void_p(rows), C.POINTER(C.c_void_p)) if rows else None
         return self._lib.HcclB200MoeCombineLocal(comm, _layer(layer), rows, *at, stream)
+
+    # model-side operators: tensors by their addresses, everything else as it is
+    def _model(self, fn, a, tensors):
+        return fn(*[data_ptr(x) if i in tensors else x for i, x in enumerate(a)])
+
+    def embedding(self, *a):
+        return self._model(self._lib.HcclB200Embedding, a, (0, 3, 10))
+
+    def embedding_grad(self, *a):
+        return self._model(self._lib.HcclB200EmbeddingGrad, a, (0, 3, 10, 13))
+
+    def gate(self, *a):
+        return self._model(self._lib.HcclB200MoeGate, a, (0, *range(7, 15)))
+
+    def gate_grad(self, *a):
+        return self._model(self._lib.HcclB200MoeGateGrad, a, (0, 7, 8, 9, 10, 11, 13))

@@ -274,6 +274,7 @@ def _load_fast(L):
         warnings.warn("calls go through ctypes, which costs several microseconds each: %s" % (str(e).splitlines() or [type(e).__name__])[0])
         return Calls(L)
     m.bind(*[C.cast(f, C.c_void_p).value for f in (L.HcclB200Collective, L.HcclB200MoeDispatchLocal, L.HcclB200MoeCombineLocal)])
+    m.bind_model(*[C.cast(f, C.c_void_p).value for f in (L.HcclB200Embedding, L.HcclB200EmbeddingGrad, L.HcclB200MoeGate, L.HcclB200MoeGateGrad)])
     return m
 
 

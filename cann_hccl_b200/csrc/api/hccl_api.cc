@@ -840,8 +840,9 @@ HcclResult HcclB200MoeGate(const void *logits, HcclDataType dataType, int64_t to
                            aclrtStream stream)
 {
     GateShape s;
-    CHK_RET(check_gate(logits, dataType, tokens, nExperts, stride, topk, normalize, {counts, probSum, routed, balance, scratch}, {idx, gates}, "HcclB200MoeGate", &s));
-    CHK_RET(check_aligned({idx, gates}, 4, "HcclB200MoeGate"));
+    CHK_RET(check_gate(logits, dataType, tokens, nExperts, stride, topk, normalize, {counts, probSum, routed, balance}, {idx, gates}, "HcclB200MoeGate", &s));
+    CHK_RET_LOG(!scratch && moe_gate_scratch_bytes(tokens, nExperts) > 0, HCCL_E_PTR, "[EI0003] HcclB200MoeGate: null pointer");
+    CHK_RET(check_aligned({idx, gates, scratch}, 4, "HcclB200MoeGate"));
     return moe_gate(s, logits, mask, idx, gates, counts, probSum, routed, balance, scratch, stream);
 }
 HcclResult HcclB200MoeBalance(const int32_t *counts, const float *probSum, const int32_t *routed, int32_t nExperts, int32_t topk, float *balance,

@@ -45,7 +45,7 @@ enum Mode : int { SCORES = 0, DX = 1, DW = 2 };
 constexpr int kThreads = 320, kEpiWarps = 8;
 constexpr uint32_t kABytes = BM * BK * 2, kStageSpace = 7 * 32768;  // seven stages of a pair
 constexpr uint32_t kTmemCols = 512;
-constexpr int kMaxStages = 8, kMaxCols = BN;
+constexpr int kMaxStages = 8, kMinCols = 128, kMaxCols = BN;
 constexpr uint32_t kChunkBytes = BK * 128;         // MN-major: 64 elements x 64 deep
 constexpr float kExpBits = 15.f, kExpScale = 1.f / 32768.f, kLog2e = 1.4426950408889634f;
 
@@ -55,7 +55,7 @@ struct alignas(64) LossGemm {
     int cols, um_tiles, n_tiles, panel;
     int k_iters, split;              // split: shares along the depth (DX)
     int units, stages;
-    uint32_t stage_bytes, idesc;
+    uint32_t stage_bytes, a_bytes, idesc;  // of a stage, of A in it
     // scores
     float2 *stats;                   // [row][2 * n_tiles]: maximum, sum of exp(s - maximum)
     float *target;                   // [row]
@@ -137,6 +137,27 @@ __device__ __forceinline__ void tmem_half(uint32_t addr, float (&v)[kHalf])
     for (int i = 0; i < kHalf; ++i) v[i] = __uint_as_float(r[i / 32][i % 32]);
 }
 
+// The same in steps of 32 columns, for single CTAs: each of them has a few tiles at most, the code above would come from memory once for
+// every tile (7 tokens x 32000 x 4096: 55 against 50 us), and memory sets the pace anyway.
+__device__ __forceinline__ void tmem_32(uint32_t addr, int left, float (&v)[32])
+{
+    uint32_t r[32];
+    tmem_ld32(addr, r);
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = i < left ? __uint_as_float(r[i]) : -INFINITY;
+}
+__device__ __forceinline__ void put_exp(__half *e, const float *v)
+{
+    uint32_t o[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+        o[i] = *(const uint32_t *)&h;
+    }
+    st_v8(e, o);
+}
+
 // 16 results of a row, of which `left` exist (a multiple of 8).
 __device__ __forceinline__ void put16(const LossGemm &P, int64_t at, float *sum, float *v, int left, float scale)
 {
@@ -173,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_loss_gemm(const __grid_cons
     LossShared &S = *(LossShared *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     constexpr int kCtas = kPair ? 2 : 1;
     constexpr bool kMnA = MODE == DW, kMnB = MODE != SCORES;
-    const uint32_t stages = (uint32_t)P.stages, stage_bytes = P.stage_bytes;
+    const uint32_t stages = (uint32_t)P.stages, stage_bytes = P.stage_bytes, a_bytes = P.a_bytes;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t cta_r = kPair ? cluster_ctarank() : 0u;
     const int unit = (int)blockIdx.x / kCtas, total = P.um_tiles * P.n_tiles * P.split;
@@ -215,7 +236,7 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_loss_gemm(const __grid_cons
                 const int k0 = (int)((int64_t)P.k_iters * w.share / P.split), k1 = (int)((int64_t)P.k_iters * (w.share + 1) / P.split);
                 for (int k = k0; k < k1; ++k) {
                     if (!mbar_wait_t<kPair>(&S.empty_bar[s], ph ^ 1, fail)) break;
-                    uint8_t *sa = S.tiles + (size_t)s * stage_bytes, *sb = sa + kABytes;
+                    uint8_t *sa = S.tiles + (size_t)s * stage_bytes, *sb = sa + a_bytes;
                     uint32_t full = smem_u32(&S.full_bar[s]);
                     if (kPair) {  // the bytes of both CTAs' loads are counted on the leader's barrier
                         if (cta_r == 0) mbar_expect_tx(&S.full_bar[s], 2 * stage_bytes);
@@ -253,7 +274,7 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_loss_gemm(const __grid_cons
                 for (int k = k0; k < k1; ++k) {
                     if (!mbar_wait_t<kPair>(&S.full_bar[s], ph, fail)) break;
                     tc_fence_after();
-                    const uint8_t *sa = S.tiles + (size_t)s * stage_bytes, *sb = sa + kABytes;
+                    const uint8_t *sa = S.tiles + (size_t)s * stage_bytes, *sb = sa + a_bytes;
                     const uint64_t da = kMnA ? make_desc_mn(sa) : make_smem_desc(sa), db = kMnB ? make_desc_mn(sb) : make_smem_desc(sb);
 #pragma unroll
                     for (int kk = 0; kk < BK / UMMA_K; ++kk) {
@@ -296,47 +317,66 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_loss_gemm(const __grid_cons
             bad = __any_sync(0xffffffffu, bad);
             tc_fence_after();
             if (MODE == SCORES) {
-                float v[kHalf];
-                if (!bad) tmem_half(taddr + c_lo, v);
-                release(buf);
                 const int exist = min(c_hi, P.N - col0) - c_lo;  // columns of this half that exist, the first of them
+                const int room = row < P.M && P.e ? (int)min((int64_t)c_hi, P.ld - col0) - c_lo : 0;  // the row ends on a multiple of 64, in zeros
                 const int yl = y >= c_lo && y < c_lo + exist ? (int)y - c_lo : -1;
-                if (exist < kHalf)
+                __half *e = P.e + (int64_t)row * P.ld + col0 + c_lo;
+                float m = -INFINITY, z = 0.f, target = 0.f;
+                if constexpr (kPair) {
+                    float v[kHalf];
+                    if (!bad) tmem_half(taddr + c_lo, v);
+                    release(buf);
+                    if (exist < kHalf)
 #pragma unroll
-                    for (int i = 0; i < kHalf; ++i) v[i] = i < exist ? v[i] : -INFINITY;
-                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, z4[4] = {}, target = 0.f;
+                        for (int i = 0; i < kHalf; ++i) v[i] = i < exist ? v[i] : -INFINITY;
+                    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, z4[4] = {};
 #pragma unroll
-                for (int i = 0; i < kHalf; ++i) m4[i & 3] = fmaxf(m4[i & 3], v[i]);
-                const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), ref = m == -INFINITY ? 0.f : m;
-                if (yl >= 0) {
+                    for (int i = 0; i < kHalf; ++i) m4[i & 3] = fmaxf(m4[i & 3], v[i]);
+                    m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+                    const float ref = m == -INFINITY ? 0.f : m;
+                    if (yl >= 0)
 #pragma unroll
-                    for (int i = 0; i < kHalf; ++i) target = i == yl ? v[i] : target;
-                    P.target[row] = target;
-                }
-                // (v - m first: the product with m alone would carry m's size into every exponent)
+                        for (int i = 0; i < kHalf; ++i) target = i == yl ? v[i] : target;
+                    // (v - m first: the product with m alone would carry m's size into every exponent)
 #pragma unroll
-                for (int i = 0; i < kHalf; ++i) {
-                    v[i] = exp2_approx(fmaf(v[i] - ref, kLog2e, kExpBits));
-                    z4[i & 3] += v[i];
-                }
-                const float z = bad ? __uint_as_float(0x7fffffffu) : ((z4[0] + z4[1]) + (z4[2] + z4[3])) * kExpScale;
-                if (row < P.M) {
-                    P.stats[(int64_t)row * (2 * P.n_tiles) + 2 * w.nt + half] = make_float2(m, z);
-                    if (P.e) {
-                        __half *e = P.e + (int64_t)row * P.ld + col0 + c_lo;
-                        const int room = (int)min((int64_t)c_hi, P.ld - col0) - c_lo;  // the row ends on a multiple of 64, in zeros
-#pragma unroll
-                        for (int c = 0; c < kHalf; c += 16)
-                            if (c < room) {
-                                uint32_t o[8];
-#pragma unroll
-                                for (int i = 0; i < 8; ++i) {
-                                    const __half2 h = __floats2half2_rn(v[c + 2 * i], v[c + 2 * i + 1]);
-                                    o[i] = *(const uint32_t *)&h;
-                                }
-                                st_v8(e + c, o);
-                            }
+                    for (int i = 0; i < kHalf; ++i) {
+                        v[i] = exp2_approx(fmaf(v[i] - ref, kLog2e, kExpBits));
+                        z4[i & 3] += v[i];
                     }
+                    z = (z4[0] + z4[1]) + (z4[2] + z4[3]);
+#pragma unroll
+                    for (int c = 0; c < kHalf; c += 16)
+                        if (c < room) put_exp(e + c, v + c);
+                } else {
+                    float v[32];
+                    if (!bad) {
+#pragma unroll 1
+                        for (int c = 0; c < exist; c += 32) {
+                            tmem_32(taddr + c_lo + c, exist - c, v);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) m = fmaxf(m, v[i]);
+                        }
+                        const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll 1
+                        for (int c = 0; c < c_hi - c_lo; c += 32) {
+                            tmem_32(taddr + c_lo + c, exist - c, v);
+                            if (yl >= c && yl < c + 32)
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) target = i == yl - c ? v[i] : target;
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) {
+                                v[i] = exp2_approx(fmaf(v[i] - ref, kLog2e, kExpBits));
+                                z += v[i];
+                            }
+                            if (c < room) put_exp(e + c, v);
+                            if (c + 16 < room) put_exp(e + c + 16, v + 16);
+                        }
+                    }
+                    release(buf);
+                }
+                if (row < P.M) {
+                    if (yl >= 0) P.target[row] = target;
+                    P.stats[(int64_t)row * (2 * P.n_tiles) + 2 * w.nt + half] = make_float2(m, bad ? __uint_as_float(0x7fffffffu) : z * kExpScale);
                 }
             } else {
                 float v[kHalf];
@@ -671,7 +711,7 @@ int score_cols(int64_t um, int64_t vocab, int units)
 {
     int best = kMaxCols;
     int64_t least = INT64_MAX;
-    for (int cols = kMaxCols; cols >= 128; cols -= 32) {
+    for (int cols = kMaxCols; cols >= kMinCols; cols -= 32) {
         const int64_t tiles = um * ((vocab + cols - 1) / cols), t = (tiles + units - 1) / units * cols;
         if (t < least) { least = t; best = cols; }
     }
@@ -716,6 +756,9 @@ HcclResult layout_of(int64_t tokens, int64_t vocab, int32_t hidden, bool grad, L
     return HCCL_SUCCESS;
 }
 
+// Rows of A in a stage.
+int a_rows(int mode, int m) { return mode == DW || m >= BM ? BM : (m + 7) / 8 * 8; }
+
 HcclResult launch_gemm(int mode, bool pair, LossGemm &P, void *stream)
 {
     LossDevice d;
@@ -724,7 +767,11 @@ HcclResult launch_gemm(int mode, bool pair, LossGemm &P, void *stream)
     P.um_tiles = (P.M + ctas * BM - 1) / (ctas * BM);
     P.n_tiles = (P.N + P.cols - 1) / P.cols;
     P.units = pair ? d.pairs : d.sms;
-    P.stage_bytes = kABytes + (uint32_t)(P.cols / ctas) * BK * 2;
+    // Of fewer than 128 rows only those that exist are loaded (in eights, the swizzle's period): the tensor cores read what follows them
+    // in shared memory instead, for results that nobody reads.  A stage behind which less than that follows does not exist.
+    P.a_bytes = (uint32_t)a_rows(mode, P.M) * BK * 2;
+    P.stage_bytes = P.a_bytes + (uint32_t)(P.cols / ctas) * BK * 2;
+    static_assert(kABytes <= kMinCols * BK * 2, "A's rows end inside the stage's B");
     P.stages = (int)std::min<uint32_t>(kMaxStages, kStageSpace / P.stage_bytes);
     P.idesc = instr_desc((uint32_t)(ctas * BM), (uint32_t)P.cols) | (mode == DW ? 1u << 15 : 0u) | (mode != SCORES ? 1u << 16 : 0u);
     // a panel's columns of B stay in L2 (40 MB of it) while the rows stream past
@@ -776,7 +823,7 @@ HcclResult vocab_loss_scores(const VocabLossCall &c, bool grad, float *lse, floa
         CHK_RET(launch_pdl((const void *)vocab_loss_x, dim3((unsigned)((c.tokens * a.xvec + kCopyThreads - 1) / kCopyThreads)), kCopyThreads, 0, &a, stream,
                            "vocabulary loss (x)"));
     }
-    CHK_RET(encode(&P.tmA, l.copy ? s + l.xc : c.x, c.tokens, c.hidden, l.copy ? l.xld : c.x_stride, BM));
+    CHK_RET(encode(&P.tmA, l.copy ? s + l.xc : c.x, c.tokens, c.hidden, l.copy ? l.xld : c.x_stride, a_rows(SCORES, (int)c.tokens)));
     CHK_RET(encode(&P.tmB, c.w, c.vocab, c.hidden, c.w_stride, l.cols / (l.pair ? 2 : 1)));
     CHK_RET(launch_gemm(SCORES, l.pair, P, stream));
     RowArgs a = row_args(c);
@@ -827,7 +874,7 @@ HcclResult vocab_loss_grad(const VocabLossCall &c, const float *lse, const float
     P.kind = l.split > 1 ? VL_F32 : VL_BF16;
     P.out = (__nv_bfloat16 *)dx; P.sum = (float *)(s + l.shares);
     P.wide = c.hidden % 16 == 0 && ((uintptr_t)dx & 31) == 0;
-    CHK_RET(encode(&P.tmA, s, c.tokens, l.ld, l.ld, BM));
+    CHK_RET(encode(&P.tmA, s, c.tokens, l.ld, l.ld, a_rows(DX, (int)c.tokens)));
     CHK_RET(encode(&P.tmB, c.w, c.vocab, c.hidden, c.w_stride, BK));
     CHK_RET(launch_gemm(DX, l.pair, P, stream));
     if (l.split > 1) {

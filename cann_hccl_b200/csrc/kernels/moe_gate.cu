@@ -26,7 +26,7 @@ namespace hcclb {
 namespace {
 
 constexpr uint32_t kAll = 0xffffffffu;
-constexpr int kGateThreads = 256, kMaxBlocks = 592, kOneThreads = 512, kOneCta = 64;
+constexpr int kGateThreads = 512, kMaxBlocks = 296, kGradThreads = 256, kOneThreads = 512, kOneCta = 64;
 constexpr int kEndExperts = 8, kEndSlices = 32, kEndThreads = kEndExperts * kEndSlices;
 
 __device__ __forceinline__ float ld_f(const float *p) { return *p; }
@@ -40,10 +40,17 @@ __device__ __forceinline__ void st_f(__nv_bfloat16 *p, float x) { *p = __float2b
 __device__ __forceinline__ uint32_t key_of(float x)
 {
     const uint32_t b = __float_as_uint(x + 0.f);
-    if (x != x) return kAll;
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
+    return x != x ? kAll : b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
 constexpr uint32_t kInfKey = 0x007fffffu;  // ~bits(-inf)
+
+// e^x, from ex2 with its smallest results cut to zero
+__device__ __forceinline__ float exp_of(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+    return y;
+}
 
 __device__ __forceinline__ float warp_sum(float x)
 {
@@ -83,7 +90,7 @@ __device__ __forceinline__ float balance_of(float sum, int n, int experts, int t
 template <int V> constexpr bool kInRegs = V <= 32;
 template <int V> constexpr int kGateMost = V <= 32 ? 512 : 128;      // threads of a CTA
 template <int V> constexpr int kGateCtas = V <= 8 ? 2 : 1;           // CTAs of that size on an SM
-// Dynamic shared memory: [warps][experts] keys, [warps][experts] sums, [experts] counts.
+// Dynamic shared memory: [warps][32 V] keys, [warps][experts] sums, [experts] counts.
 template <class T, int V>
 __global__ void __launch_bounds__(kGateMost<V>, kGateCtas<V>) moe_gate_kernel(const __grid_constant__ GateArgs a)
 {
@@ -91,9 +98,10 @@ __global__ void __launch_bounds__(kGateMost<V>, kGateCtas<V>) moe_gate_kernel(co
     __shared__ int s_n;
     __shared__ float s_b[kOneThreads / 32];
     const int E = a.experts, k = a.topk, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5;
-    uint32_t *key = sh + warp * E;
-    float *s_p = (float *)(sh + W * E);
-    int32_t *s_c = (int32_t *)(sh + 2 * W * E);
+    constexpr int S = V * 32;  // keys of a row: zeros behind the experts
+    uint32_t *key = sh + warp * S;
+    float *s_p = (float *)(sh + W * S);
+    int32_t *s_c = (int32_t *)(sh + W * (S + E));
     if (!kInRegs<V>)
         for (int i = threadIdx.x; i < W * E; i += blockDim.x) s_p[i] = 0.f;
     for (int i = threadIdx.x; i < E; i += blockDim.x) s_c[i] = 0;
@@ -119,7 +127,7 @@ __global__ void __launch_bounds__(kGateMost<V>, kGateCtas<V>) moe_gate_kernel(co
         for (int j = 0; j < V; ++j) {
             const int e = j * 32 + lane;
             const uint32_t q = e < E ? key_of(x[j]) : 0;
-            if (e < E) key[e] = q;
+            key[e] = q;
             best = max(best, q);
         }
         __syncwarp();
@@ -127,28 +135,35 @@ __global__ void __launch_bounds__(kGateMost<V>, kGateCtas<V>) moe_gate_kernel(co
         const bool routed = on && top > kInfKey;
         const float m = value_of(top);
         int sel = -1;           // of slot `lane`
-        float sel_x = -INFINITY;
+        uint32_t sel_key = kInfKey;
         if (routed) {
             for (int s = 0; s < k; ++s) {
                 if (s) top = __reduce_max_sync(kAll, best);
                 if (top <= kInfKey) break;
                 const uint32_t who = __ballot_sync(kAll, best == top);
                 int e;
-                if ((who & (who - 1)) == 0) {  // one lane has it: which of its experts is the first with that key
+                if ((who & (who - 1)) == 0) {  // one lane has it: which of its experts is the first with that key, what is left
                     const int w = __ffs(who) - 1;
-                    e = -1;
                     uint32_t next = 0;
-                    for (int j0 = 0; j0 < V; j0 += 32) {
-                        const int j = j0 + lane, at = j * 32 + w;
-                        uint32_t q = j < V && at < E ? key[at] : 0;
-                        if (e < 0) {
+                    if (V <= 32) {
+                        uint32_t *at = key + lane * 32 + w;
+                        if (lane < V) next = *at;
+                        const int j = __ffs(__ballot_sync(kAll, next == top)) - 1;
+                        if (lane == j) *at = next = 0;
+                        e = j * 32 + w;
+                    } else {
+                        e = -1;
+#pragma unroll 1
+                        for (int j0 = 0; j0 < V; j0 += 32) {
+                            uint32_t *at = key + (j0 + lane) * 32 + w, q = *at;
                             const uint32_t hit = __ballot_sync(kAll, q == top);
-                            if (hit) {
-                                e = (j0 + __ffs(hit) - 1) * 32 + w;
-                                if (at == e) key[at] = q = 0;
+                            if (e < 0 && hit) {
+                                const int j = __ffs(hit) - 1;
+                                if (lane == j) *at = q = 0;
+                                e = (j0 + j) * 32 + w;
                             }
+                            next = max(next, q);
                         }
-                        next = max(next, q);
                     }
                     next = __reduce_max_sync(kAll, next);
                     if (lane == w) best = next;
@@ -165,12 +180,12 @@ __global__ void __launch_bounds__(kGateMost<V>, kGateCtas<V>) moe_gate_kernel(co
                     }
                 }
                 __syncwarp();
-                if (lane == s) { sel = e; sel_x = value_of(top); }
+                if (lane == s) { sel = e; sel_key = top; }
             }
             float z = 0.f;
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                x[j] = __expf(x[j] - m);  // experts outside are -inf
+                x[j] = exp_of(x[j] - m);  // experts outside are -inf
                 z += x[j];
             }
             z = warp_sum(z);
@@ -180,7 +195,7 @@ __global__ void __launch_bounds__(kGateMost<V>, kGateCtas<V>) moe_gate_kernel(co
                 if (kInRegs<V>) sums[kInRegs<V> ? j : 0] += x[j] * inv;
                 else if (j * 32 + lane < E) s_p[warp * E + j * 32 + lane] += x[j] * inv;
             }
-            const float g = sel >= 0 ? __expf(sel_x - m) : 0.f;
+            const float g = sel >= 0 ? exp_of(value_of(sel_key) - m) : 0.f;
             const float whole = a.normalize ? warp_sum(g) : z;
             if (lane < k) a.gates[t * k + lane] = g / whole;
             if (sel >= 0) atomicAdd(&s_c[sel], 1);
@@ -333,10 +348,10 @@ __global__ void __launch_bounds__(kGateMost<V>, kGateCtas<V>) moe_gate_grad_kern
         }
         float z = 0.f;
 #pragma unroll
-        for (int j = 0; j < V; ++j) { x[j] = __expf(x[j] - m); z += x[j]; }
+        for (int j = 0; j < V; ++j) { x[j] = exp_of(x[j] - m); z += x[j]; }
         z = warp_sum(z);
         const float inv = 1.f / z;
-        float g = __expf(sel_x - m);   // 0 where the slot is empty
+        float g = exp_of(sel_x - m);   // 0 where the slot is empty
         const float whole = a.normalize ? warp_sum(g) : z;
         g = g > 0.f ? g / whole : g;
         const float gd = warp_sum(g * dg);
@@ -368,15 +383,16 @@ GateGrid gate_grid(int64_t tokens, int experts, bool grad)
 {
     const int most = experts > 1024 ? 128 : kOneThreads;
     if (!grad && tokens <= kOneCta) return {(int)std::min<int64_t>(most, std::max<int64_t>(1, tokens) * 32), 1};
-    const int threads = std::min(kGateThreads, most), warps = threads / 32;
-    return {threads, (int)std::min<int64_t>(grad ? 148 * 6 : kMaxBlocks, (tokens + warps - 1) / warps)};
+    // a token for every warp, until the CTAs are as many as run at once
+    const int threads = std::min(grad ? kGradThreads : tokens >= (int64_t)kMaxBlocks * 16 ? kGateThreads : 128, most), warps = threads / 32;
+    return {threads, (int)std::min<int64_t>(grad ? 148 * 4 : kMaxBlocks, (tokens + warps - 1) / warps)};
 }
 
 template <class T, int V> HcclResult run_gate(GateArgs &a, bool grad, void *stream)
 {
     const GateGrid g = gate_grid(a.tokens, a.experts, grad);
     const int W = g.threads / 32;
-    const size_t smem = (size_t)(grad ? W + 1 : 2 * W + 1) * a.experts * 4;
+    const size_t smem = grad ? (size_t)(W + 1) * a.experts * 4 : (size_t)W * V * 128 + (size_t)(W + 1) * a.experts * 4;
     const void *fn = grad ? (const void *)moe_gate_grad_kernel<T, V> : (const void *)moe_gate_kernel<T, V>;
     if (smem > 48 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
@@ -413,7 +429,7 @@ HcclResult gate_any(const GateShape &s, GateArgs &a, bool grad, void *stream)
 int64_t moe_gate_scratch_bytes(int64_t tokens, int32_t experts)
 {
     const int ctas = gate_grid(tokens, experts, false).ctas;
-    return ctas == 1 ? 16 : (int64_t)ctas * (experts * 8 + 4) + kGateMaxExperts / kEndExperts * 4 + 16;
+    return ctas == 1 ? 0 : (int64_t)ctas * (experts * 8 + 4) + kGateMaxExperts / kEndExperts * 4 + 16;
 }
 
 HcclResult moe_gate(const GateShape &s, const void *logits, const uint8_t *mask, int32_t *idx, float *gates, int32_t *counts, float *prob_sum,

@@ -6,9 +6,10 @@
 //
 // Gradient: the tokens are sorted by id (stable, so that the sums have one order whatever ran before), then a CTA walks a tile of
 // the sorted list, keeps the running row in fp32 registers and writes it when the id changes: every row of dY is read once and
-// every row of the table written once, without atomics.  A run of one id that crosses tiles leaves fp32 pieces, which a second
-// launch adds in order, so that a token that makes up a large part of a text is summed by many CTAs.  Rows of the table without a
-// token are zeroed by the same launch as the sums.
+// every row of the table written once, without atomics on sums.  A run of one id that crosses tiles leaves fp32 pieces, which a last
+// launch adds in order, so that a token that makes up a large part of a text is summed by many CTAs.  The sort leaves a bit for each
+// row that has a token; the launch that sums also zeroes the others (reads and writes together run at 7.0 TB/s; the table zeroed by
+// the SMs that the sort leaves idle, and its rows written twice: 185 + 70 us instead of 188 for 32768 tokens, 128256 x 4096).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -130,14 +131,17 @@ __global__ void __launch_bounds__(kLookupThreads) embed_lookup_kernel(const __gr
 }
 
 // ---------------------------------------------------------------------------------------------------- stable sort by id
-// Radix sort from the least significant digit.  A pair is (row of the table, token); rows outside the table sort behind all
-// others as `vocab`.  A warp takes consecutive stretches of 32 pairs; __match_any_sync gives the lanes of one digit, the
-// warp's counters in shared memory the earlier stretches, so equal digits keep their order.
+// A pair is (row of the table, token); rows outside the table sort behind all others as `vocab`.  Few tokens: a token's place is the
+// number of tokens that belong before it, counted by comparing with all of them.  More: radix sort from the least significant digit;
+// a warp takes consecutive stretches of 32 pairs, __match_any_sync gives the lanes of one digit, the warp's counters in shared
+// memory the earlier stretches, so equal digits keep their order.
+// (1531 tokens: one CTA of a radix sort 8.1 us, one cluster 13 us, both exchanging through shared memory; 32768 tokens: a cluster 25
+// us, the tiles below 20 us.)
+constexpr int kCountMost = 8192, kCountTokens = 32, kCountThreads = 256;  // tokens that are sorted by counting, tokens of a CTA
+constexpr int kWindow = 1 << 18;                                          // rows whose bits a CTA makes
 constexpr int kDigitBits = 9, kBins = 1 << kDigitBits;
 constexpr int kSortItems = 8;
-constexpr int kTileThreads = 256;
-constexpr int kOneMost = 1024 * kSortItems;           // tokens that one CTA sorts
-constexpr int kTile = kTileThreads * kSortItems;
+constexpr int kTileThreads = 256, kTile = kTileThreads * kSortItems;
 
 struct SortArgs {
     const void *ids;                 // first pass
@@ -147,7 +151,8 @@ struct SortArgs {
     uint2 *out;
     int32_t *hist;                   // [tile][bin]
     int64_t tokens;
-    int tiles, shift, bits, passes, digit;
+    uint32_t *has;                   // a bit for each row with a token, cleared and set on the way (null: not wanted)
+    int tiles, shift, passes, digit, last;
 };
 
 // Ranks of a warp's pairs within (warp, digit); counts[warp][bin] end up holding the warp's pairs of each digit.
@@ -202,66 +207,59 @@ template <int N> __device__ __forceinline__ void bins_prefix(int (&t)[N], int32_
     for (int i = 0; i < N; ++i) t[i] += base;
 }
 
-template <int THREADS> constexpr size_t kOneSmem = (size_t)(THREADS / 32) * kBins * 4 + kBins * 4 + (size_t)THREADS * kSortItems * 8;
-
-// Up to kOneMost tokens: all passes in one CTA, pairs in registers, exchanged through shared memory.  Fewer warps where there are fewer
-// tokens: the prefix over the warps' counters is the longest step of a pass.
-template <int THREADS>
-__global__ void __launch_bounds__(THREADS) embed_sort_one_kernel(const __grid_constant__ SortArgs a)
+__device__ __forceinline__ void mark_row(const SortArgs &a, uint32_t row)
 {
-    extern __shared__ int32_t sh[];
-    constexpr int W = THREADS / 32, N = kBins > THREADS ? kBins / THREADS : 1;  // N bins of a thread
-    __shared__ int32_t s_warp[W];
-    int32_t *counts = sh, *base = counts + W * kBins;
-    uint2 *pairs = (uint2 *)(base + kBins);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int n = (int)a.tokens, items = (n + THREADS - 1) / THREADS, at = warp * items * 32 + lane;
+    if (a.has && row < (uint32_t)a.vocab) atomicOr(a.has + (row >> 5), 1u << (row & 31));
+}
+
+__device__ __forceinline__ uint32_t key_at(const SortArgs &a, int64_t t)
+{
+    const int64_t r = row_of(id_at(a.ids, a.wide, t), a.first, a.vocab);
+    return r >= 0 ? (uint32_t)r : (uint32_t)a.vocab;
+}
+
+// Up to kCountMost tokens: grid of token groups, then of windows of the table's bits.  Dynamic shared memory: keys of all tokens (a
+// multiple of 4, those behind the last one above every other), bits of a window.
+__global__ void __launch_bounds__(kCountThreads) embed_sort_count_kernel(const __grid_constant__ SortArgs a)
+{
+    extern __shared__ uint4 sh4[];
+    __shared__ int s_rank[kCountThreads / 32][kCountTokens];
+    uint32_t *keys = (uint32_t *)sh4;
+    const int n = (int)a.tokens, padded = (n + 3) / 4 * 4, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     pdl_trigger();
     pdl_wait();
-    uint32_t key[kSortItems], pos[kSortItems];
-#pragma unroll
-    for (int i = 0; i < kSortItems; ++i) {
-        const int t = at + i * 32;
-        pos[i] = (uint32_t)t;
-        key[i] = 0xffffffffu;  // behind everything: pairs that pad the last warps
-        if (i < items && t < n) {
-            const int64_t r = row_of(id_at(a.ids, a.wide, t), a.first, a.vocab);
-            key[i] = r >= 0 ? (uint32_t)r : (uint32_t)a.vocab;
+    for (int t = threadIdx.x; t < padded; t += kCountThreads) keys[t] = t < n ? key_at(a, t) : 0xffffffffu;
+    if ((int)blockIdx.x >= a.tiles) {
+        uint32_t *bits = keys + padded;
+        const uint32_t r0 = (uint32_t)(blockIdx.x - a.tiles) * kWindow, rows = (uint32_t)min((int64_t)kWindow, a.vocab - r0), words = (rows + 31) / 32;
+        for (uint32_t i = threadIdx.x; i < words; i += kCountThreads) bits[i] = 0;
+        __syncthreads();
+        for (int t = threadIdx.x; t < n; t += kCountThreads) {
+            const uint32_t r = keys[t] - r0;
+            if (r < rows) atomicOr(bits + (r >> 5), 1u << (r & 31));
         }
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < words; i += kCountThreads) a.has[(r0 >> 5) + i] = bits[i];
+        return;
     }
-    for (int pass = 0; pass < a.passes; ++pass) {
-        const int shift = pass * a.digit;
-        const uint32_t mask = (1u << a.digit) - 1;
-        for (int i = threadIdx.x; i < W * kBins; i += THREADS) counts[i] = 0;
-        __syncthreads();
-        int rank[kSortItems];
-        warp_ranks(key, items, shift, mask, counts, rank);
-        __syncthreads();
-        int t[N];
-#pragma unroll
-        for (int j = 0; j < N; ++j) t[j] = (int)threadIdx.x * N + j < kBins ? warp_prefix<W>(counts, threadIdx.x * N + j) : 0;
-        bins_prefix<N>(t, s_warp);
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-            if ((int)threadIdx.x * N + j < kBins) base[threadIdx.x * N + j] = t[j];
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < kSortItems; ++i) {
-            if (i >= items) break;
-            const uint32_t d = (key[i] >> shift) & mask;
-            pairs[base[d] + counts[warp * kBins + d] + rank[i]] = make_uint2(key[i], pos[i]);
-        }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < kSortItems; ++i) {
-            if (i >= items) break;
-            const uint2 p = pairs[at + i * 32];
-            key[i] = p.x; pos[i] = p.y;
-        }
+    __syncthreads();
+    const int t = (int)blockIdx.x * kCountTokens + lane;
+    const uint32_t mine = t < n ? keys[t] : 0xffffffffu;
+    int rank = 0;
+    const uint4 *k4 = (const uint4 *)keys;
+#pragma unroll 4
+    for (int q = warp; q < padded / 4; q += kCountThreads / 32) {
+        const uint4 k = k4[q];
+        // earlier tokens come before equal ones, later ones do not
+        rank += (k.x < mine + (q * 4 < t)) + (k.y < mine + (q * 4 + 1 < t)) + (k.z < mine + (q * 4 + 2 < t)) + (k.w < mine + (q * 4 + 3 < t));
     }
+    s_rank[warp][lane] = rank;
+    __syncthreads();
+    if (warp || t >= n) return;
+    rank = 0;
 #pragma unroll
-    for (int i = 0; i < kSortItems; ++i)
-        if (i < items && at + i * 32 < n) a.out[at + i * 32] = make_uint2(key[i], pos[i]);
+    for (int w = 0; w < kCountThreads / 32; ++w) rank += s_rank[w][lane];
+    a.out[rank] = make_uint2(mine, (uint32_t)t);
 }
 
 __device__ __forceinline__ void load_tile(const SortArgs &a, int64_t tile, uint32_t (&key)[kSortItems], uint32_t (&pos)[kSortItems])
@@ -277,8 +275,7 @@ __device__ __forceinline__ void load_tile(const SortArgs &a, int64_t tile, uint3
                 const uint2 p = a.in[t];
                 key[i] = p.x; pos[i] = p.y;
             } else {
-                const int64_t r = row_of(id_at(a.ids, a.wide, t), a.first, a.vocab);
-                key[i] = r >= 0 ? (uint32_t)r : (uint32_t)a.vocab;
+                key[i] = key_at(a, t);
                 pos[i] = (uint32_t)t;
             }
         }
@@ -292,6 +289,8 @@ __global__ void __launch_bounds__(kTileThreads) embed_sort_hist_kernel(const __g
     __syncthreads();
     pdl_trigger();
     pdl_wait();
+    if (a.has && !a.in)  // the first pass clears the bits, the last one sets them
+        for (int64_t i = (int64_t)blockIdx.x * kTileThreads + threadIdx.x; i < (a.vocab + 31) / 32; i += (int64_t)gridDim.x * kTileThreads) a.has[i] = 0;
     uint32_t key[kSortItems], pos[kSortItems];
     load_tile(a, blockIdx.x, key, pos);
     const int64_t t0 = (int64_t)blockIdx.x * kTile + (threadIdx.x >> 5) * (32 * kSortItems) + (threadIdx.x & 31);
@@ -340,6 +339,7 @@ __global__ void __launch_bounds__(kTileThreads) embed_sort_scatter_kernel(const 
         if (t0 + i * 32 < a.tokens) {  // pairs that pad the tile are last in it: they displace none of the others
             const uint32_t d = (key[i] >> a.shift) & mask;
             a.out[base[d] + counts[(threadIdx.x >> 5) * kBins + d] + rank[i]] = make_uint2(key[i], pos[i]);
+            if (a.last) mark_row(a, key[i]);
         }
 }
 
@@ -350,11 +350,12 @@ struct SumArgs {
     void *out;
     float *pieces;                   // [tile][2][nvec * per]: run from an earlier tile, run that goes on behind the tile
     int64_t tokens, vocab, stride;   // stride: bytes between rows of dy
-    int64_t tiles, zero_ctas;
-    int rows, nvec, nslice, add;     // rows: tokens of a tile
+    const uint32_t *has;             // bits of the rows with a token (null: none has one)
+    int64_t tiles;
+    int rows, nvec, nslice, add, zero_rows;     // rows: tokens of a tile
     float scale;
 };
-constexpr int kSumThreads = 256, kSumBatch = 4, kZeroRows = 32, kMostRows = 256;
+constexpr int kSumThreads = 256, kSumBatch = 4, kMostRows = 256;
 
 template <class T, int B> __device__ __forceinline__ void put_row(const SumArgs &a, int64_t row, int v, const float (&acc)[B / sizeof(T)])
 {
@@ -381,44 +382,24 @@ template <int SIZE> __device__ __forceinline__ void zero_bytes(uint8_t *p, int64
     for (int64_t i = (int64_t)threadIdx.x * SIZE; i < tail; i += blockDim.x * SIZE) st(p + head + body * 32 + i, one);
 }
 
-// First place in the sorted list whose row is not below `row`.
-__device__ __forceinline__ int64_t lower_bound(const uint2 *pairs, int64_t n, uint32_t row)
-{
-    int64_t lo = 0, hi = n;
-    while (lo < hi) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (pairs[mid].x < row) lo = mid + 1; else hi = mid;
-    }
-    return lo;
-}
-
-// grid: tiles x slices of a row, then CTAs that zero kZeroRows rows of the table each where they have no token
+// grid: tiles x slices of a row, then CTAs that zero zero_rows rows of the table each where they have no token
 template <class T, int B>
 __global__ void __launch_bounds__(kSumThreads) embed_sum_kernel(const __grid_constant__ SumArgs a)
 {
     constexpr int N = B / sizeof(T);
     __shared__ uint2 s_pair[kMostRows];
-    __shared__ uint32_t s_edge[2], s_has;
+    __shared__ uint32_t s_edge[2];
     pdl_trigger();
     pdl_wait();
     const int64_t sums = a.tiles * a.nslice;
     if ((int64_t)blockIdx.x >= sums) {
-        const int64_t r0 = ((int64_t)blockIdx.x - sums) * kZeroRows;
-        if (threadIdx.x < 32) {
-            const int64_t r = r0 + threadIdx.x;
-            bool has = true;
-            if (r < a.vocab) {
-                const int64_t at = lower_bound(a.pairs, a.tokens, (uint32_t)r);
-                has = at < a.tokens && a.pairs[at].x == (uint32_t)r;
-            }
-            const uint32_t mask = __ballot_sync(0xffffffffu, has);
-            if (threadIdx.x == 0) s_has = mask;
-        }
-        __syncthreads();
-        for (int i = 0; i < kZeroRows;) {
-            if (s_has >> i & 1) { ++i; continue; }
+        const int64_t r0 = ((int64_t)blockIdx.x - sums) * a.zero_rows;
+        const int n = (int)min((int64_t)a.zero_rows, a.vocab - r0);
+        const uint32_t has = a.has ? a.has[r0 >> 5] >> (r0 & 31) : 0;
+        for (int i = 0; i < n;) {
+            if (has >> i & 1) { ++i; continue; }
             const int from = i;
-            while (i < kZeroRows && !(s_has >> i & 1)) ++i;
+            while (i < n && !(has >> i & 1)) ++i;
             zero_bytes<sizeof(T)>((uint8_t *)a.out + (r0 + from) * a.nvec * B, (int64_t)(i - from) * a.nvec * B);
         }
         return;
@@ -487,7 +468,12 @@ __global__ void __launch_bounds__(kSumThreads) embed_join_kernel(const __grid_co
     pdl_wait();
     const uint32_t key = a.pairs[t1 - 1].x;
     if (key >= (uint32_t)a.vocab || a.pairs[t1].x != key || (tile > 0 && a.pairs[tile * a.rows - 1].x == key)) return;
-    const int64_t last = (lower_bound(a.pairs, a.tokens, key + 1) - 1) / a.rows;  // tile in which the run ends
+    int64_t last = tile;  // tile in which the run ends: a warp looks at the first rows of 32 tiles at a time
+    for (uint32_t same = ~0u; same == ~0u;) {
+        const int64_t q = last + 1 + (threadIdx.x & 31);
+        same = __ballot_sync(0xffffffffu, q < a.tiles && a.pairs[q * a.rows].x == key);
+        last += same == ~0u ? 32 : __ffs(~same) - 1;
+    }
     if (c >= hidden) return;
     float acc[N];
     const float *p = a.pieces + (tile * 2 + 1) * hidden + c;
@@ -557,18 +543,19 @@ template <class T> HcclResult lookup_typed(LookupArgs &a, int64_t hidden, void *
 }
 
 // Tokens of a tile: short tiles for parallelism, longer ones where there are many tokens, so that a run has few pieces.
-int tile_rows(int64_t tokens) { return (int)std::min<int64_t>(kMostRows, std::max<int64_t>(32, (tokens / 1184 + 31) / 32 * 32)); }
+int tile_rows(int64_t tokens) { return (int)std::min<int64_t>(kMostRows, std::max<int64_t>(32, (tokens / 592 + 31) / 32 * 32)); }
 
-struct Scratch { int64_t pairs, spare, hist, pieces, bytes; };
-Scratch scratch_of(int64_t tokens, int32_t hidden)
+struct Scratch { int64_t pairs, spare, hist, has, pieces, bytes; };
+Scratch scratch_of(int64_t tokens, int64_t vocab, int32_t hidden)
 {
     auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
     Scratch s;
     const int64_t tiles = (tokens + tile_rows(tokens) - 1) / tile_rows(tokens);
     s.pairs = 0;
     s.spare = s.pairs + up(tokens * 8);
-    s.hist = s.spare + (tokens > kOneMost ? up(tokens * 8) : 0);
-    s.pieces = s.hist + (tokens > kOneMost ? up((tokens + kTile - 1) / kTile * kBins * 4) : 0);
+    s.hist = s.spare + (tokens > kCountMost ? up(tokens * 8) : 0);
+    s.has = s.hist + (tokens > kCountMost ? up((tokens + kTile - 1) / kTile * kBins * 4) : 0);
+    s.pieces = s.has + (tokens ? up((vocab + 31) / 32 * 4) : 0);
     s.bytes = s.pieces + (tiles > 1 ? up(tiles * 2 * hidden * 4) : 0);
     return s;
 }
@@ -578,9 +565,10 @@ template <class T, int B> HcclResult sum(SumArgs &a, int64_t row_bytes, void *st
     a.nvec = (int)(row_bytes / B);
     const int threads = std::min(kSumThreads, (a.nvec + 31) / 32 * 32);
     a.nslice = (a.nvec + threads - 1) / threads;
-    a.zero_ctas = a.add ? 0 : (a.vocab + kZeroRows - 1) / kZeroRows;
     unsigned ctas;
-    CHK_RET(grid_of(a.tiles * a.nslice + a.zero_ctas, &ctas, "embedding gradient"));
+    a.zero_rows = 32;  // those of one word, fewer where they are long
+    while (a.zero_rows > 1 && a.zero_rows * row_bytes > 65536) a.zero_rows /= 2;
+    CHK_RET(grid_of(a.tiles * a.nslice + (a.add ? 0 : (a.vocab + a.zero_rows - 1) / a.zero_rows), &ctas, "embedding gradient"));
     if (ctas) CHK_RET(launch_pdl((const void *)embed_sum_kernel<T, B>, dim3(ctas), (unsigned)threads, 0, &a, stream, "embedding gradient"));
     if (a.tiles <= 1) return HCCL_SUCCESS;
     const int hidden = (int)(row_bytes / (int64_t)sizeof(T)), n = hidden % 4 ? 1 : 4, join = std::min(kSumThreads, (hidden / n + 31) / 32 * 32);
@@ -602,32 +590,28 @@ template <class T> HcclResult sum_typed(SumArgs &a, int64_t hidden, void *stream
     }
 }
 
-template <int THREADS> HcclResult sort_one(SortArgs &a, void *stream)
-{
-    const void *fn = (const void *)embed_sort_one_kernel<THREADS>;
-    if (kOneSmem<THREADS> > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kOneSmem<THREADS>);
-        CHK_RET_LOG(e != cudaSuccess, HCCL_E_RUNTIME, "embedding gradient set-up failed: %s", cudaGetErrorString(e));
-    }
-    return launch_pdl(fn, dim3(1), THREADS, kOneSmem<THREADS>, &a, stream, "embedding gradient (sort)");
-}
-
-HcclResult sort_tokens(const EmbedTable &t, const EmbedIds &ids, const Scratch &s, uint8_t *scratch, void *stream, const uint2 **sorted)
+HcclResult sort_tokens(const EmbedTable &t, const EmbedIds &ids, const Scratch &s, uint8_t *scratch, uint32_t *has, void *stream, const uint2 **sorted)
 {
     SortArgs a;
     memset(&a, 0, sizeof(a));
     a.ids = ids.ids; a.wide = ids.wide; a.vocab = t.vocab; a.first = t.first; a.tokens = ids.tokens;
+    a.has = has;
     int bits = 1;
     while ((t.vocab >> bits) != 0) ++bits;  // rows 0 .. vocab
     a.passes = (bits + kDigitBits - 1) / kDigitBits;
     a.digit = (bits + a.passes - 1) / a.passes;
     uint2 *buf[2] = {(uint2 *)(scratch + s.pairs), (uint2 *)(scratch + s.spare)};
-    if (ids.tokens <= kOneMost) {
+    if (ids.tokens <= kCountMost) {
         a.out = buf[0];
         *sorted = buf[0];
-        if (ids.tokens <= 1024) return sort_one<256>(a, stream);
-        if (ids.tokens <= 4096) return sort_one<512>(a, stream);
-        return sort_one<1024>(a, stream);
+        a.tiles = (int)((ids.tokens + kCountTokens - 1) / kCountTokens);
+        const size_t smem = (size_t)(ids.tokens + 3) / 4 * 16 + (has ? kWindow / 8 : 0);
+        if (smem > 48 * 1024) {
+            const cudaError_t e = cudaFuncSetAttribute((const void *)embed_sort_count_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+            CHK_RET_LOG(e != cudaSuccess, HCCL_E_RUNTIME, "embedding gradient set-up failed: %s", cudaGetErrorString(e));
+        }
+        const int64_t windows = has ? (t.vocab + kWindow - 1) / kWindow : 0;
+        return launch_pdl((const void *)embed_sort_count_kernel, dim3((unsigned)(a.tiles + windows)), kCountThreads, smem, &a, stream, "embedding gradient (sort)");
     }
     a.hist = (int32_t *)(scratch + s.hist);
     a.tiles = (int)((ids.tokens + kTile - 1) / kTile);
@@ -635,6 +619,7 @@ HcclResult sort_tokens(const EmbedTable &t, const EmbedIds &ids, const Scratch &
         a.in = pass ? buf[(pass - 1) & 1] : nullptr;
         a.out = buf[pass & 1];
         a.shift = pass * a.digit;
+        a.last = pass == a.passes - 1;
         CHK_RET(launch_pdl((const void *)embed_sort_hist_kernel, dim3((unsigned)a.tiles), kTileThreads, 0, &a, stream, "embedding gradient (histogram)"));
         CHK_RET(launch_pdl((const void *)embed_sort_scatter_kernel, dim3((unsigned)a.tiles), kTileThreads, 0, &a, stream, "embedding gradient (scatter)"));
         *sorted = a.out;
@@ -660,15 +645,19 @@ HcclResult embed_lookup(const EmbedTable &t, const EmbedIds &ids, const void *we
     }
 }
 
-int64_t embed_grad_scratch_bytes(int64_t tokens, int64_t vocab, int32_t hidden) { return std::max<int64_t>(256, scratch_of(tokens, hidden).bytes); }
+int64_t embed_grad_scratch_bytes(int64_t tokens, int64_t vocab, int32_t hidden) { return std::max<int64_t>(256, scratch_of(tokens, vocab, hidden).bytes); }
 
 HcclResult embed_grad(const EmbedTable &t, const EmbedIds &ids, const void *grad, int64_t stride, float scale, void *out, bool add, void *scratch,
                       void *stream)
 {
-    const Scratch s = scratch_of(ids.tokens, t.hidden);
+    const Scratch s = scratch_of(ids.tokens, t.vocab, t.hidden);
     SumArgs a;
     memset(&a, 0, sizeof(a));
-    if (ids.tokens) CHK_RET(sort_tokens(t, ids, s, (uint8_t *)scratch, stream, &a.pairs));
+    uint32_t *has = add ? nullptr : (uint32_t *)((uint8_t *)scratch + s.has);
+    if (ids.tokens) {
+        CHK_RET(sort_tokens(t, ids, s, (uint8_t *)scratch, has, stream, &a.pairs));
+        a.has = has;
+    }
     a.dy = (const uint8_t *)grad; a.stride = stride * dtype_size(t.type);
     a.out = out; a.add = add; a.scale = scale;
     a.tokens = ids.tokens; a.vocab = t.vocab;

@@ -249,12 +249,115 @@ static PyObject *moe_combine(PyObject *self, PyObject *const *a, Py_ssize_t n)
     return PyLong_FromLong((long)rc);
 }
 
+/* ---- model-side operators.  Integers and floats are taken as they come, tensors by their addresses (None: null) ---- */
+typedef HcclResult (*embedding_fn)(const void *, HcclDataType, int64_t, const void *, int64_t, int64_t, int64_t, int32_t, HcclDataType, float, void *, aclrtStream);
+typedef HcclResult (*embedding_grad_fn)(const void *, HcclDataType, int64_t, const void *, int64_t, int64_t, int64_t, int32_t, HcclDataType, float, void *, HcclDataType,
+                                        int32_t, void *, aclrtStream);
+typedef HcclResult (*gate_fn)(const void *, HcclDataType, int64_t, int32_t, int64_t, int32_t, int32_t, const uint8_t *, int32_t *, float *, int32_t *, float *, int32_t *,
+                              float *, void *, aclrtStream);
+typedef HcclResult (*gate_grad_fn)(const void *, HcclDataType, int64_t, int32_t, int64_t, int32_t, int32_t, const uint8_t *, const int32_t *, const float *, const int32_t *,
+                                   const int32_t *, float, void *, aclrtStream);
+static embedding_fn g_embedding;
+static embedding_grad_fn g_embedding_grad;
+static gate_fn g_gate;
+static gate_grad_fn g_gate_grad;
+
+/* bind_model(addresses of HcclB200Embedding, HcclB200EmbeddingGrad, HcclB200MoeGate, HcclB200MoeGateGrad) */
+static PyObject *bind_model(PyObject *self, PyObject *const *a, Py_ssize_t n)
+{
+    if (n != 4) { PyErr_SetString(PyExc_TypeError, "bind_model() takes 4 addresses"); return NULL; }
+    g_embedding = (embedding_fn)PyLong_AsVoidPtr(a[0]);
+    g_embedding_grad = (embedding_grad_fn)PyLong_AsVoidPtr(a[1]);
+    g_gate = (gate_fn)PyLong_AsVoidPtr(a[2]);
+    g_gate_grad = (gate_grad_fn)PyLong_AsVoidPtr(a[3]);
+    if (PyErr_Occurred()) return NULL;
+    Py_RETURN_NONE;
+}
+
+/* embedding(ids, type of ids, tokens, weights, stride, vocab, first id, hidden, type, scale, out, stream) -> result code */
+static PyObject *embedding(PyObject *self, PyObject *const *a, Py_ssize_t n)
+{
+    if (n != 12 || !g_embedding) { PyErr_SetString(PyExc_TypeError, "embedding() takes 12 arguments, after bind_model()"); return NULL; }
+    void *ids, *w, *out, *stream = PyLong_AsVoidPtr(a[11]);
+    const int it = (int)PyLong_AsLong(a[1]), t = (int)PyLong_AsLong(a[8]);
+    const int64_t tokens = PyLong_AsLongLong(a[2]), stride = PyLong_AsLongLong(a[4]), vocab = PyLong_AsLongLong(a[5]), first = PyLong_AsLongLong(a[6]);
+    const int32_t hidden = (int32_t)PyLong_AsLong(a[7]);
+    const float scale = (float)PyFloat_AsDouble(a[9]);
+    if (PyErr_Occurred() || address(a[0], &ids) || address(a[3], &w) || address(a[10], &out)) return NULL;
+    HcclResult rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = g_embedding(ids, (HcclDataType)it, tokens, w, stride, vocab, first, hidden, (HcclDataType)t, scale, out, (aclrtStream)stream);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong((long)rc);
+}
+
+/* embedding_grad(ids, type of ids, tokens, grad, stride, vocab, first id, hidden, type, scale, out, type of out, accumulate, scratch, stream) */
+static PyObject *embedding_grad(PyObject *self, PyObject *const *a, Py_ssize_t n)
+{
+    if (n != 15 || !g_embedding_grad) { PyErr_SetString(PyExc_TypeError, "embedding_grad() takes 15 arguments, after bind_model()"); return NULL; }
+    void *ids, *g, *out, *scratch, *stream = PyLong_AsVoidPtr(a[14]);
+    const int it = (int)PyLong_AsLong(a[1]), t = (int)PyLong_AsLong(a[8]), ot = (int)PyLong_AsLong(a[11]);
+    const int64_t tokens = PyLong_AsLongLong(a[2]), stride = PyLong_AsLongLong(a[4]), vocab = PyLong_AsLongLong(a[5]), first = PyLong_AsLongLong(a[6]);
+    const int32_t hidden = (int32_t)PyLong_AsLong(a[7]), add = (int32_t)PyLong_AsLong(a[12]);
+    const float scale = (float)PyFloat_AsDouble(a[9]);
+    if (PyErr_Occurred() || address(a[0], &ids) || address(a[3], &g) || address(a[10], &out) || address(a[13], &scratch)) return NULL;
+    HcclResult rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = g_embedding_grad(ids, (HcclDataType)it, tokens, g, stride, vocab, first, hidden, (HcclDataType)t, scale, out, (HcclDataType)ot, add, scratch, (aclrtStream)stream);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong((long)rc);
+}
+
+/* gate(logits, type, tokens, experts, stride, topk, normalize, mask, idx, gates, counts, prob_sum, routed, balance, scratch, stream) */
+static PyObject *gate(PyObject *self, PyObject *const *a, Py_ssize_t n)
+{
+    if (n != 16 || !g_gate) { PyErr_SetString(PyExc_TypeError, "gate() takes 16 arguments, after bind_model()"); return NULL; }
+    void *at[9], *stream = PyLong_AsVoidPtr(a[15]);
+    static const int from[9] = {0, 7, 8, 9, 10, 11, 12, 13, 14};
+    const int t = (int)PyLong_AsLong(a[1]);
+    const int64_t tokens = PyLong_AsLongLong(a[2]), stride = PyLong_AsLongLong(a[4]);
+    const int32_t experts = (int32_t)PyLong_AsLong(a[3]), topk = (int32_t)PyLong_AsLong(a[5]), normalize = (int32_t)PyLong_AsLong(a[6]);
+    if (PyErr_Occurred()) return NULL;
+    for (int i = 0; i < 9; ++i)
+        if (address(a[from[i]], &at[i])) return NULL;
+    HcclResult rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = g_gate(at[0], (HcclDataType)t, tokens, experts, stride, topk, normalize, at[1], at[2], at[3], at[4], at[5], at[6], at[7], at[8], (aclrtStream)stream);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong((long)rc);
+}
+
+/* gate_grad(logits, type, tokens, experts, stride, topk, normalize, mask, idx, d_gates, counts, routed, d_balance, d_logits, stream) */
+static PyObject *gate_grad(PyObject *self, PyObject *const *a, Py_ssize_t n)
+{
+    if (n != 15 || !g_gate_grad) { PyErr_SetString(PyExc_TypeError, "gate_grad() takes 15 arguments, after bind_model()"); return NULL; }
+    void *at[7], *stream = PyLong_AsVoidPtr(a[14]);
+    static const int from[7] = {0, 7, 8, 9, 10, 11, 13};
+    const int t = (int)PyLong_AsLong(a[1]);
+    const int64_t tokens = PyLong_AsLongLong(a[2]), stride = PyLong_AsLongLong(a[4]);
+    const int32_t experts = (int32_t)PyLong_AsLong(a[3]), topk = (int32_t)PyLong_AsLong(a[5]), normalize = (int32_t)PyLong_AsLong(a[6]);
+    const float coef = (float)PyFloat_AsDouble(a[12]);
+    if (PyErr_Occurred()) return NULL;
+    for (int i = 0; i < 7; ++i)
+        if (address(a[from[i]], &at[i])) return NULL;
+    HcclResult rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = g_gate_grad(at[0], (HcclDataType)t, tokens, experts, stride, topk, normalize, at[1], at[2], at[3], at[4], at[5], coef, at[6], (aclrtStream)stream);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong((long)rc);
+}
+
 static PyMethodDef methods[] = {{"bind", (PyCFunction)(void (*)(void))bind, METH_FASTCALL, NULL},
                                 {"setup", (PyCFunction)(void (*)(void))setup, METH_FASTCALL, NULL},
                                 {"op", (PyCFunction)(void (*)(void))op, METH_FASTCALL, NULL},
                                 {"moe_dispatch", (PyCFunction)(void (*)(void))moe_dispatch, METH_FASTCALL, NULL},
                                 {"moe_combine", (PyCFunction)(void (*)(void))moe_combine, METH_FASTCALL, NULL},
                                 {"collective", (PyCFunction)(void (*)(void))collective, METH_FASTCALL, NULL},
+                                {"bind_model", (PyCFunction)(void (*)(void))bind_model, METH_FASTCALL, NULL},
+                                {"embedding", (PyCFunction)(void (*)(void))embedding, METH_FASTCALL, NULL},
+                                {"embedding_grad", (PyCFunction)(void (*)(void))embedding_grad, METH_FASTCALL, NULL},
+                                {"gate", (PyCFunction)(void (*)(void))gate, METH_FASTCALL, NULL},
+                                {"gate_grad", (PyCFunction)(void (*)(void))gate_grad, METH_FASTCALL, NULL},
                                 {NULL, NULL, 0, NULL}};
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fastcall", NULL, -1, methods, NULL, NULL, NULL, NULL};
 

@@ -133,7 +133,7 @@ extern HcclResult HcclB200EmbeddingGrad(const void *ids, HcclDataType idType, in
  * gate 0); gates [tokens, topk] = their softmax probabilities, normalize: divided by their sum.  Tokens with mask 0 (mask may be
  * null) or with nothing but -inf are not routed: experts -1, gates 0.  Over the routed tokens: counts [experts] = pairs,
  * probSum [experts] = sums of the probabilities, *routed = their number n, *balance = experts / (topk n^2) * sum counts * probSum
- * (0 without tokens).  dataType of the logits: FP32, FP16 or BFP16; at most 4096 experts, topk at most 32. */
+ * (0 without tokens).  scratch may be null where its size is 0.  dataType of the logits: FP32, FP16 or BFP16; at most 4096 experts, topk at most 32. */
 extern int64_t HcclB200MoeGateScratchBytes(int64_t tokens, int32_t nExperts);
 extern HcclResult HcclB200MoeGate(const void *logits, HcclDataType dataType, int64_t tokens, int32_t nExperts, int64_t stride, int32_t topk,
                                   int32_t normalize, const uint8_t *mask, int32_t *idx, float *gates, int32_t *counts, float *probSum, int32_t *routed,

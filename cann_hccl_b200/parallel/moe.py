@@ -23,7 +23,7 @@ import torch
 
 from .. import _lib as L
 from ..ops.comm import _raw_stream
-from ..utils.dtypes import float_code
+from ..utils.dtypes import float_codes
 from ..utils.tensors import check_out, on_device_of
 
 
@@ -149,19 +149,24 @@ class MoEExchange:
 Gate = namedtuple("Gate", "idx gates counts prob_sum routed balance")
 
 
+_FLOAT = float_codes()
+
+
 def _check_gate(logits, topk, mask):
     if not (torch.is_tensor(logits) and logits.is_cuda and logits.dim() == 2 and logits.shape[1] > 0):
         raise ValueError("logits must be a CUDA tensor [tokens, experts]")
     T, E = logits.shape
-    if float_code(logits.dtype) is None:
+    a, b = logits.stride()
+    code = _FLOAT.get(logits.dtype)
+    if code is None:
         raise TypeError("logits must be fp32, fp16 or bf16, got %s" % logits.dtype)
-    if logits.stride(1) != 1 and E > 1 or logits.stride(0) < E and T > 1:
-        raise ValueError("the experts of a token must lie side by side (strides %s)" % (tuple(logits.stride()),))
+    if b != 1 and E > 1 or a < E and T > 1:
+        raise ValueError("the experts of a token must lie side by side (strides %s)" % ((a, b),))
     if not 1 <= topk <= E:
         raise ValueError("topk %d of %d experts" % (topk, E))
     if mask is not None and not (mask.device == logits.device and mask.dtype in (torch.bool, torch.uint8) and mask.shape == (T,) and mask.is_contiguous()):
         raise ValueError("mask must be a contiguous bool tensor [tokens] on the device of the logits")
-    return T, E, max(E, logits.stride(0))
+    return T, E, max(E, a), code
 
 
 def gate(logits, topk, mask=None, normalize=True, comm=None):
@@ -191,16 +196,16 @@ def gate(logits, topk, mask=None, normalize=True, comm=None):
                     L.check(L.lib().HcclB200MoeBalance(g.counts.data_ptr(), g.prob_sum.data_ptr(), g.routed.data_ptr(), l.shape[1], topk,
                                                        g.balance.data_ptr(), _raw_stream()), "HcclB200MoeBalance")
         return gs if isinstance(logits, (list, tuple)) else gs[0]
-    T, E, stride = _check_gate(logits, topk, mask)
-    dev = logits.device
+    T, E, stride, code = _check_gate(logits, topk, mask)
+    new, i32, f32 = logits.new_empty, torch.int32, torch.float32
     with on_device_of(logits):
-        idx, gates = torch.empty(T, topk, device=dev, dtype=torch.int32), torch.empty(T, topk, device=dev, dtype=torch.float32)
-        counts, prob_sum = torch.empty(E, device=dev, dtype=torch.int32), torch.empty(E, device=dev, dtype=torch.float32)
-        routed, balance = torch.empty((), device=dev, dtype=torch.int32), torch.empty((), device=dev, dtype=torch.float32)
-        scratch = torch.empty(max(0, L.lib().HcclB200MoeGateScratchBytes(T, E)), device=dev, dtype=torch.uint8)
-        L.check(L.lib().HcclB200MoeGate(logits.data_ptr(), float_code(logits.dtype), T, E, stride, topk, int(normalize),
-                                        None if mask is None else mask.data_ptr(), idx.data_ptr(), gates.data_ptr(), counts.data_ptr(),
-                                        prob_sum.data_ptr(), routed.data_ptr(), balance.data_ptr(), scratch.data_ptr(), _raw_stream()), "HcclB200MoeGate")
+        idx, gates = new((T, topk), dtype=i32), new((T, topk), dtype=f32)
+        counts, prob_sum, routed, balance = new(E, dtype=i32), new(E, dtype=f32), new((), dtype=i32), new((), dtype=f32)
+        n = L.lib().HcclB200MoeGateScratchBytes(T, E)
+        scratch = new(n, dtype=torch.uint8) if n > 0 else None
+        rc = L.fast.gate(logits, code, T, E, stride, topk, int(normalize), mask, idx, gates, counts, prob_sum, routed, balance, scratch, _raw_stream())
+        if rc:
+            L.check(rc, "HcclB200MoeGate")
     return Gate(idx, gates, counts, prob_sum, routed, balance)
 
 
@@ -210,7 +215,7 @@ def gate_grad(logits, g, d_gates=None, balance=0.0, mask=None, normalize=True, o
     expert -1 passes nothing on, rows that are not routed get zeros."""
     if g.idx.dim() != 2:
         raise ValueError("g must be what gate() returned for these logits")
-    T, E, stride = _check_gate(logits, g.idx.shape[1], mask)
+    T, E, stride, code = _check_gate(logits, g.idx.shape[1], mask)
     dev, topk = logits.device, g.idx.shape[1]
     if g.idx.shape[0] != T or g.counts.shape != (E,) or g.idx.device != dev or not g.idx.is_contiguous():
         raise ValueError("g must be what gate() returned for these logits")
@@ -218,12 +223,13 @@ def gate_grad(logits, g, d_gates=None, balance=0.0, mask=None, normalize=True, o
         raise ValueError("d_gates must be a contiguous fp32 tensor [tokens, topk] on the device of the logits")
     with on_device_of(logits):
         if out is None:
-            out = torch.empty(T, E, device=dev, dtype=logits.dtype)
+            out = logits.new_empty((T, E))
         else:
             check_out(out, (T, E), logits.dtype, dev)
-        L.check(L.lib().HcclB200MoeGateGrad(logits.data_ptr(), float_code(logits.dtype), T, E, stride, topk, int(normalize),
-                                            None if mask is None else mask.data_ptr(), g.idx.data_ptr(), None if d_gates is None else d_gates.data_ptr(),
-                                            g.counts.data_ptr(), g.routed.data_ptr(), balance, out.data_ptr(), _raw_stream()), "HcclB200MoeGateGrad")
+        L.lib()
+        rc = L.fast.gate_grad(logits, code, T, E, stride, topk, int(normalize), mask, g.idx, d_gates, g.counts, g.routed, balance, out, _raw_stream())
+        if rc:
+            L.check(rc, "HcclB200MoeGateGrad")
     return out
 
 

@@ -16,10 +16,11 @@ import torch
 
 from .. import _lib as L
 from ..ops.comm import _raw_stream
-from ..utils.dtypes import float_code
+from ..utils.dtypes import float_codes
 from ..utils.tensors import check_out, on_device_of
 
 _IDS = {torch.int32: L.INT32, torch.int64: L.INT64}
+_FLOAT = float_codes()
 
 
 def _check_ids(ids, device):
@@ -28,50 +29,54 @@ def _check_ids(ids, device):
 
 
 def _check_rows(t, name):
-    """[rows, hidden] whose rows lie in one piece each; returns the elements between rows."""
+    """[rows, hidden] whose rows lie in one piece each; returns rows, hidden and the elements between rows."""
     if not (torch.is_tensor(t) and t.is_cuda and t.dim() == 2 and t.shape[1] > 0):
         raise ValueError("%s must be a CUDA tensor [rows, hidden]" % name)
-    if float_code(t.dtype) is None:
+    if t.dtype not in _FLOAT:
         raise TypeError("%s must be fp32, fp16 or bf16, got %s" % (name, t.dtype))
-    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
-        raise ValueError("rows of %s must lie in one piece each (strides %s)" % (name, tuple(t.stride())))
-    return max(t.shape[1], t.stride(0))
+    (n, h), (a, b) = t.shape, t.stride()
+    if h > 1 and b != 1 or n > 1 and a < h:
+        raise ValueError("rows of %s must lie in one piece each (strides %s)" % (name, (a, b)))
+    return n, h, a if n > 1 else h
 
 
 def embedding(ids, w, scale=1.0, first_id=0, out=None):
     """scale * w[ids - first_id] -> [*ids.shape, hidden]; ids outside the rows of w give zeros.  The product is rounded once."""
-    stride = _check_rows(w, "w")
+    vocab, hidden, stride = _check_rows(w, "w")
     _check_ids(ids, w.device)
     with on_device_of(w):
         if out is None:
-            out = torch.empty((*ids.shape, w.shape[1]), device=w.device, dtype=w.dtype)
+            out = w.new_empty((*ids.shape, hidden))
         else:
-            check_out(out, (*ids.shape, w.shape[1]), w.dtype, w.device)
-        L.check(L.lib().HcclB200Embedding(ids.data_ptr(), _IDS[ids.dtype], ids.numel(), w.data_ptr(), stride, w.shape[0], first_id, w.shape[1],
-                                          float_code(w.dtype), scale, out.data_ptr(), _raw_stream()), "HcclB200Embedding")
+            check_out(out, (*ids.shape, hidden), w.dtype, w.device)
+        L.lib()
+        rc = L.fast.embedding(ids, _IDS[ids.dtype], ids.numel(), w, stride, vocab, first_id, hidden, _FLOAT[w.dtype], scale, out, _raw_stream())
+        if rc:
+            L.check(rc, "HcclB200Embedding")
     return out
 
 
 def embedding_grad(ids, dy, vocab, scale=1.0, first_id=0, out=None, add=False):
     """Gradient of embedding()'s w: [vocab, hidden] of dy's type, the fp32 sums of dy's rows by token, in token order (the same bits every
     time), times scale.  With `add` the sums are added to `out`, an fp32 tensor (gradients of several batches, or of a tied weight)."""
-    if not (torch.is_tensor(dy) and dy.dim() >= 1) or tuple(dy.shape[:-1]) != tuple(ids.shape):
+    if not (torch.is_tensor(dy) and dy.dim() >= 1) or dy.shape[:-1] != ids.shape:
         raise ValueError("dy must be [*ids.shape, hidden]")
     rows = dy if dy.dim() == 2 else dy.reshape(-1, dy.shape[-1])
-    stride, hidden = _check_rows(rows, "dy"), rows.shape[1]
+    _, hidden, stride = _check_rows(rows, "dy")
     _check_ids(ids, rows.device)
     with on_device_of(rows):
         if out is None:
             if add:
                 raise ValueError("add needs the fp32 tensor to add to")
-            out = torch.empty(vocab, hidden, device=rows.device, dtype=rows.dtype)
+            out = rows.new_empty((vocab, hidden))
         else:
             check_out(out, (vocab, hidden), torch.float32 if add else rows.dtype, rows.device)
-        lib = L.lib()
-        scratch = torch.empty(max(0, lib.HcclB200EmbeddingGradScratchBytes(ids.numel(), vocab, hidden)), device=rows.device, dtype=torch.uint8)
-        L.check(lib.HcclB200EmbeddingGrad(ids.data_ptr(), _IDS[ids.dtype], ids.numel(), rows.data_ptr(), stride, vocab, first_id, hidden,
-                                          float_code(rows.dtype), scale, out.data_ptr(), float_code(out.dtype), int(add), scratch.data_ptr(),
-                                          _raw_stream()), "HcclB200EmbeddingGrad")
+        n, lib = ids.numel(), L.lib()
+        scratch = rows.new_empty(max(0, lib.HcclB200EmbeddingGradScratchBytes(n, vocab, hidden)), dtype=torch.uint8)
+        rc = L.fast.embedding_grad(ids, _IDS[ids.dtype], n, rows, stride, vocab, first_id, hidden, _FLOAT[rows.dtype], scale, out, _FLOAT[out.dtype],
+                                   int(add), scratch, _raw_stream())
+        if rc:
+            L.check(rc, "HcclB200EmbeddingGrad")
     return out
 
 
@@ -105,12 +110,11 @@ _BF16_OUT, _F32_OUT, _ADD, _ADD_BF16 = range(4)
 
 
 def _check_loss(x, w, targets, weights, reduction):
-    """[(x, w, strides)] of one shard; the rest of the arguments."""
     for t, name in ((x, "x"), (w, "w")):
-        stride = _check_rows(t, name)
+        _, h, stride = _check_rows(t, name)
         if t.dtype != torch.bfloat16:
             raise TypeError("%s must be bf16, got %s" % (name, t.dtype))
-        if t.shape[1] % 8 or stride % 8 or t.data_ptr() % 16:
+        if h % 8 or stride % 8 or t.data_ptr() % 16:
             raise ValueError("rows of %s must be multiples of 8 elements that start on 16-byte boundaries" % name)
     if x.shape[1] != w.shape[1] or x.device != w.device or not w.shape[0]:
         raise ValueError("x %s and w %s must have the same hidden size and device" % (tuple(x.shape), tuple(w.shape)))
@@ -128,43 +132,45 @@ class _Shard:
 
     def __init__(self, x, w, targets, weights, first, whole, ignore):
         self.x, self.w, self.targets, self.weights = x, w, targets, weights
-        self.first, self.whole, self.ignore = first, whole, ignore
-        self.T, self.V, self.H = x.shape[0], w.shape[0], w.shape[1]
+        (self.T, self.H), self.V = x.shape, w.shape[0]
+        self._xs, ws = x.stride(0) if self.T > 1 else self.H, w.stride(0) if self.V > 1 else self.H
+        self._x, self._y, self._ysize = x.data_ptr(), targets.data_ptr(), targets.element_size()
+        self._q = None if weights is None else weights.data_ptr()
+        self._call = L.VocabLoss(self._x, w.data_ptr(), self._xs, ws, self._y, self._q, self.T, self.V, first, whole, ignore,
+                                 self.H, _IDS[targets.dtype])
 
     def part(self, a, b):
-        x, w, y, q = self.x, self.w, self.targets, self.weights
-        return C.byref(L.VocabLoss(x=x.data_ptr() + a * x.stride(0) * 2, w=w.data_ptr(), xStride=max(self.H, x.stride(0)), wStride=max(self.H, w.stride(0)),
-                                   targets=y.data_ptr() + a * y.element_size(), weights=None if q is None else q.data_ptr() + a * 4, tokens=b - a,
-                                   vocab=self.V, firstId=self.first, wholeVocab=self.whole, ignoreId=self.ignore, hidden=self.H, targetType=_IDS[y.dtype]))
+        """The call for tokens a to b (the structure is the shard's: valid until the next one)."""
+        c = self._call
+        c.x, c.targets, c.tokens = self._x + a * self._xs * 2, self._y + a * self._ysize, b - a
+        if self._q is not None:
+            c.weights = self._q + a * 4
+        return C.byref(c)
 
     def new(self, shape, dtype=torch.float32):
-        return torch.empty(shape, device=self.x.device, dtype=dtype)
-
-    def scratch(self, tokens, grad):
-        n = L.lib().HcclB200VocabLossScratchBytes(tokens, self.V, self.H, int(grad))
-        if n < 0:
-            raise RuntimeError("no scratch size for %d tokens, %d rows of %d" % (tokens, self.V, self.H))
-        return self.new(n, torch.uint8)
-
-
-def _at(t, a):
-    return None if t is None else t.data_ptr() + a * t.element_size()
+        return self.x.new_empty(shape, dtype=dtype)
 
 
 def _run_loss(shards, comm, reduction, scale=1.0, outs=None, grad=False):
     """The loss of shards that share their tokens (those of this process), chunk by chunk; with `grad` dx and dw of each."""
-    lib, st, s0 = L.lib(), _raw_stream(), shards[0]
-    T, alone = s0.T, comm is None or comm.nranks == 1
+    lib, st, check, s0 = L.lib(), _raw_stream(), L.check, shards[0]
+    T, alone, none = s0.T, comm is None or comm.nranks == 1, reduction == "none"
     chunk = min(max(T, 1), min(lib.HcclB200VocabLossChunk(s.V, int(grad)) for s in shards))
     losses = [s.new(T) for s in shards]
-    total = None
+    # fp32 words of each shard behind its scratch: lse and target logit of a chunk, the joint lse, the sum of the weights
+    mem, words = [], []
+    for s in shards:
+        n = lib.HcclB200VocabLossScratchBytes(chunk if T else 0, s.V, s.H, int(grad))
+        if n < 0:
+            raise RuntimeError("no scratch size for %d tokens, %d rows of %d" % (chunk, s.V, s.H))
+        n = (n + 255) // 256 * 256
+        m = s.new(n + (3 * chunk + 1) * 4, torch.uint8)
+        mem.append(m)
+        words.append(m.data_ptr() + n)
+    totals = [p + 12 * chunk if reduction == "mean" else None for p in words]
     if reduction == "mean":
-        total = [s.new(()) for s in shards]
-        for s, t in zip(shards, total):
-            L.check(lib.HcclB200VocabLossTotal(s.part(0, T), t.data_ptr(), st), "HcclB200VocabLossTotal")
-    parts = [s.new((2, chunk)) for s in shards]                    # lse and target logits of a chunk
-    joint = parts if alone else [s.new(chunk) for s in shards]
-    scratch = [s.scratch(chunk, grad) for s in shards] if T else None
+        for s, p in zip(shards, totals):
+            check(lib.HcclB200VocabLossTotal(s.part(0, T), p, st), "HcclB200VocabLossTotal")
     if grad:
         dxs = [s.new((T, s.H), torch.bfloat16) for s in shards]
         several = T > chunk
@@ -173,31 +179,29 @@ def _run_loss(shards, comm, reduction, scale=1.0, outs=None, grad=False):
     for a in range(0, T, chunk):
         b = min(T, a + chunk)
         n = b - a
-        for s, p, mem, loss in zip(shards, parts, scratch, losses):
-            L.check(lib.HcclB200VocabLossScores(s.part(a, b), int(grad), p.data_ptr(), p.data_ptr() + n * 4, _at(loss, a) if alone else None, mem.data_ptr(), st),
-                    "HcclB200VocabLossScores")
+        for s, m, p, loss in zip(shards, mem, words, losses):
+            check(lib.HcclB200VocabLossScores(s.part(a, b), int(grad), p, p + n * 4, loss.data_ptr() + a * 4 if alone else None, m.data_ptr(), st), "HcclB200VocabLossScores")
         if not alone:
             every = [s.new((comm.nranks, 2, n)) for s in shards]
-            mine = [p.view(-1)[:2 * n] for p in parts]
+            mine = [m[p - m.data_ptr():p - m.data_ptr() + 8 * n].view(torch.float32) for m, p in zip(mem, words)]
             comm.all_gather(mine, every)
-            for s, e, lse, loss in zip(shards, every, joint, losses):
-                L.check(lib.HcclB200VocabLossCombine(s.part(a, b), e.data_ptr(), comm.nranks, lse.data_ptr(), _at(loss, a), st), "HcclB200VocabLossCombine")
+            for s, e, p, loss in zip(shards, every, words, losses):
+                check(lib.HcclB200VocabLossCombine(s.part(a, b), e.data_ptr(), comm.nranks, p + 8 * chunk, loss.data_ptr() + a * 4, st), "HcclB200VocabLossCombine")
         if grad:
-            for i, (s, p, lse, mem) in enumerate(zip(shards, parts, joint, scratch)):
+            for i, (s, m, p) in enumerate(zip(shards, mem, words)):
                 kind = _ADD if outs[i] is not None else _BF16_OUT if not several else _F32_OUT if a == 0 else _ADD if b < T else _ADD_BF16
-                L.check(lib.HcclB200VocabLossGrad(s.part(a, b), lse.data_ptr(), p.data_ptr() + n * 4, _at(total and total[i], 0), scale,
-                                                  dxs[i].data_ptr() + a * s.H * 2, dws[i].data_ptr(), _at(sums[i], 0), kind, mem.data_ptr(), st),
-                        "HcclB200VocabLossGrad")
+                check(lib.HcclB200VocabLossGrad(s.part(a, b), p if alone else p + 8 * chunk, p + n * 4, totals[i], scale, dxs[i].data_ptr() + a * s.H * 2,
+                                                dws[i].data_ptr(), None if sums[i] is None else sums[i].data_ptr(), kind, m.data_ptr(), st), "HcclB200VocabLossGrad")
     if grad and not T:
         for o, d in zip(outs, dws):
             if o is None:
                 d.zero_()
     if grad and not alone and T:
         comm.all_reduce(dxs, dxs)
-    if reduction != "none":
+    if not none:
         for i, (s, loss) in enumerate(zip(shards, losses)):
             out = s.new(())
-            L.check(lib.HcclB200VocabLossSum(s.part(0, T), loss.data_ptr(), _at(total and total[i], 0), out.data_ptr(), st), "HcclB200VocabLossSum")
+            check(lib.HcclB200VocabLossSum(s.part(0, T), loss.data_ptr(), totals[i], out.data_ptr(), st), "HcclB200VocabLossSum")
             losses[i] = out
     return list(zip(losses, dxs, dws)) if grad else losses
 

@@ -37,13 +37,15 @@ def hccl_dtype(x):
     return _TORCH[x.dtype]
 
 
-def float_code(t):
-    """HcclDataType of a floating torch type that the model-side operators take (fp32, fp16, bf16), else None."""
-    global _TORCH
-    if _TORCH is None:
-        _TORCH = _torch_map()
-    code = _TORCH.get(t)
-    return code if code in (L.FP32, L.FP16, L.BFP16) else None
+_FLOATS = {}
+
+
+def float_codes():
+    """{torch type: HcclDataType} of the floating types that the model-side operators take."""
+    if not _FLOATS:
+        import torch
+        _FLOATS.update({torch.float32: L.FP32, torch.float16: L.FP16, torch.bfloat16: L.BFP16})
+    return _FLOATS
 
 
 def data_ptr(x):

@@ -1,14 +1,21 @@
 """Checks and the device guard that the model-side operators share."""
-import contextlib
-
 import torch
 
-_NONE = contextlib.nullcontext()
+class _Nothing:
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *a):
+        return False
+
+
+_NONE = _Nothing()
+_current = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def on_device_of(t):
     """Makes the tensor's device (and with it torch's current stream there) the current one for a call."""
-    return _NONE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _NONE if t.get_device() == _current() else torch.cuda.device(t.device)
 
 
 def check_out(out, shape, dtype, device):

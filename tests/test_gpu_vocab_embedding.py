@@ -126,11 +126,26 @@ def test_gradient(T, V, hidden, kind, dtype):
     assert close(acc, want + start.double(), size + start.double().abs(), count + 1, torch.float32)
 
 
-def test_gradient_of_a_large_batch():
-    T, V, hidden = 300007, 2000, 8                                           # 147 tiles of the sort, long runs
-    ids, dy = text(T, V, "zipf"), torch.randn(T, hidden, device="cuda")
+@pytest.mark.parametrize("T,V,hidden,dtype", [(300007, 2000, 8, torch.float32), (65536, 30000, 40, torch.bfloat16), (65537, 700, 33, torch.float16),
+                                              (70000, 1 << 20, 5, torch.bfloat16)])
+def test_gradient_of_a_large_batch(T, V, hidden, dtype):
+    """Both sides of what one cluster sorts; long runs; three digits."""
+    ids, dy = text(T, V, "zipf"), torch.randn(T, hidden, device="cuda").to(dtype)
     want, size, count = grad64(ids, dy, V, 1.0)
-    assert close(vocab.embedding_grad(ids, dy, V), want, size, count, torch.float32)
+    out = torch.full((V, hidden), 5.0, device="cuda", dtype=dtype)
+    assert close(vocab.embedding_grad(ids, dy, V, out=out), want, size, count, dtype)
+    assert bool((out[(count[:, 0] == 0)] == 0).all())
+
+
+def test_gradient_into_rows_off_a_boundary():
+    """A table that starts between vectors, with something before and behind it."""
+    for dtype, off in ((torch.bfloat16, 1), (torch.bfloat16, 3), (torch.float32, 1), (torch.float16, 17)):
+        room = torch.full((1000 * 33 + 64,), 7.0, device="cuda", dtype=dtype)
+        out = room[off:off + 33000].view(1000, 33)
+        ids, dy = text(200, 1000, "zipf"), torch.randn(200, 33, device="cuda").to(dtype)
+        vocab.embedding_grad(ids, dy, 1000, out=out)
+        assert torch.equal(out, vocab.embedding_grad(ids, dy, 1000))
+        assert bool((room[:off] == 7).all()) and bool((room[off + 33000:] == 7).all())
 
 
 def test_gradient_strides_shards_and_empty():
@@ -215,3 +230,16 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for k in range(2):
         assert all(torch.equal(g, want[k]) for g in got[k])
+
+
+@pytest.mark.parametrize("call", ["vocab.embedding(i, w)", "vocab.embedding_grad(i, w[:3], 5)", "vocab.linear_cross_entropy(w[:3], w, i)", "moe.gate(w, 2)",
+                                  "moe.gate_grad(w, moe.Gate(w[:, :2].int().contiguous(), None, w[0].int(), None, i[0].int(), None))"])
+def test_first_call_of_a_program(call):
+    """Whatever the first call into the package is, it loads the library."""
+    import os
+    import subprocess
+    import sys
+    prog = "import torch; from cann_hccl_b200.parallel import moe, vocab; w = torch.zeros(5, 8, device='cuda', dtype=torch.bfloat16); " \
+           "i = torch.zeros(3, device='cuda', dtype=torch.int64); %s; torch.cuda.synchronize()" % call
+    r = subprocess.run([sys.executable, "-c", prog], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr

@@ -56,12 +56,14 @@ def test_gate(grad, bad, want):
 
 
 def test_gate_outputs():
-    for name in ("gates", "prob", "balance", "scratch"):
+    for name in ("gates", "prob", "balance"):
         assert gate(**{name: None}) == L.E_PTR and gate(**{name: AT + 2}) == L.E_PARA, name
+    assert gate(scratch=AT + 2) == L.E_PARA and gate(scratch=None, tokens=1000) == L.E_PTR   # a decode batch needs none
     assert gate(True, out=None) == L.E_PTR and gate(True, out=AT + 2) == L.E_PARA and gate(True, d_gates=AT + 2) == L.E_PARA
     lib = L.lib()
     assert lib.HcclB200MoeBalance(None, AT, AT, 8, 2, AT, None) == L.E_PTR and lib.HcclB200MoeBalance(AT, AT, AT, 8, 9, AT, None) == L.E_PARA
-    assert lib.HcclB200MoeGateScratchBytes(4, 0) == -1 and lib.HcclB200MoeGateScratchBytes(4, 5000) == -1 and lib.HcclB200MoeGateScratchBytes(0, 8) > 0
+    assert lib.HcclB200MoeGateScratchBytes(4, 0) == -1 and lib.HcclB200MoeGateScratchBytes(4, 5000) == -1 and lib.HcclB200MoeGateScratchBytes(0, 8) == 0
+    assert lib.HcclB200MoeGateScratchBytes(1000, 8) > 0
 
 
 def loss(entry="Scores", args=None, **bad):
