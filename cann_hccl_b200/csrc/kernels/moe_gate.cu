@@ -5,11 +5,12 @@
 // Gradient: counts are constants; dl = p (u - sum_e p_e u_e) with u_e = coef * E / (k n^2) * counts[e], and through the gates
 // g_j (dg_j - sum_i g_i dg_i) at the chosen experts (normalised), or u raised by dg_j there (not normalised).
 //
-// A warp takes a token, a lane the experts lane, lane + 32, ... : one pass over the logits.  A lane knows the largest of its order-
-// preserving integer keys, so a round of the top-k is a maximum over the lanes; the keys of the lane that has it lie in shared memory,
-// where the whole warp finds the expert and that lane's next largest in a few instructions (with every lane searching its own
-// registers: 65536 tokens x 256, top 8, 167 us).  Sums of probabilities stay in registers, counts in shared memory; each CTA leaves one
-// partial row, a second launch adds them in a fixed order (no floating-point atomics).  Up to kOneCta tokens one CTA does it all.
+// A warp takes a token, a lane the experts lane, lane + 32, ... : one pass over the logits, as order-preserving integer keys.  The k-th
+// largest of the lanes' maxima is a bound that at least k experts reach and few more do (about ten for top 8 of 256): these go to a
+// list in shared memory, a lane takes one of them and counts the others before it.  More than 32 of them (many equal logits): k rounds
+// of a maximum over the lanes.  (65536 tokens x 256, top 8: rounds in which every lane searches its registers 167 us, rounds that the
+// warp searches together 63 us.)  Sums of probabilities stay in registers, counts in shared memory; each CTA leaves one partial row,
+// a second launch adds them in a fixed order (no floating-point atomics).  Up to kOneCta tokens one CTA does it all.
 // Bound: launches and latency for decode batches, instruction issue for large ones.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -44,7 +45,7 @@ __device__ __forceinline__ uint32_t key_of(float x)
 }
 constexpr uint32_t kInfKey = 0x007fffffu;  // ~bits(-inf)
 
-// e^x, from ex2 with its smallest results cut to zero
+// e^x from ex2, its smallest results cut to zero
 __device__ __forceinline__ float exp_of(float x)
 {
     float y;
@@ -97,6 +98,7 @@ __global__ void __launch_bounds__(kGateMost<V>, kGateCtas<V>) moe_gate_kernel(co
     extern __shared__ uint32_t sh[];
     __shared__ int s_n;
     __shared__ float s_b[kOneThreads / 32];
+    __shared__ uint64_t s_list[kGateMost<V> / 32][36];
     const int E = a.experts, k = a.topk, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5;
     constexpr int S = V * 32;  // keys of a row: zeros behind the experts
     uint32_t *key = sh + warp * S;
@@ -117,70 +119,81 @@ __global__ void __launch_bounds__(kGateMost<V>, kGateCtas<V>) moe_gate_kernel(co
         const bool on = !a.mask || a.mask[t];
         float x[V];
         uint32_t best = 0;  // largest key of this lane
-        __syncwarp();       // the keys of the token before are not read any more
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const int e = j * 32 + lane;
             x[j] = e < E ? ld_f(row + e) : -INFINITY;
         }
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int e = j * 32 + lane;
-            const uint32_t q = e < E ? key_of(x[j]) : 0;
-            key[e] = q;
-            best = max(best, q);
-        }
-        __syncwarp();
-        uint32_t top = __reduce_max_sync(kAll, best);
+        for (int j = 0; j < V; ++j) best = max(best, key_of(x[j]));  // experts outside count as -inf
+        const uint32_t top = __reduce_max_sync(kAll, best);
         const bool routed = on && top > kInfKey;
         const float m = value_of(top);
-        int sel = -1;           // of slot `lane`
-        uint32_t sel_key = kInfKey;
+        int sel = -1, slot = lane;  // this lane's choice, if it has one, and its place
+        uint32_t sel_key = 0;
         if (routed) {
-            for (int s = 0; s < k; ++s) {
-                if (s) top = __reduce_max_sync(kAll, best);
-                if (top <= kInfKey) break;
-                const uint32_t who = __ballot_sync(kAll, best == top);
-                int e;
-                if ((who & (who - 1)) == 0) {  // one lane has it: which of its experts is the first with that key, what is left
-                    const int w = __ffs(who) - 1;
-                    uint32_t next = 0;
-                    if (V <= 32) {
-                        uint32_t *at = key + lane * 32 + w;
-                        if (lane < V) next = *at;
-                        const int j = __ffs(__ballot_sync(kAll, next == top)) - 1;
-                        if (lane == j) *at = next = 0;
-                        e = j * 32 + w;
-                    } else {
-                        e = -1;
-#pragma unroll 1
-                        for (int j0 = 0; j0 < V; j0 += 32) {
-                            uint32_t *at = key + (j0 + lane) * 32 + w, q = *at;
-                            const uint32_t hit = __ballot_sync(kAll, q == top);
-                            if (e < 0 && hit) {
-                                const int j = __ffs(hit) - 1;
-                                if (lane == j) *at = q = 0;
-                                e = (j0 + j) * 32 + w;
-                            }
-                            next = max(next, q);
-                        }
-                    }
-                    next = __reduce_max_sync(kAll, next);
-                    if (lane == w) best = next;
-                } else {                       // equal keys: the lowest expert of all
-                    uint32_t first = kAll;
-                    if (best == top)
-                        for (int at = lane; at < E; at += 32)
-                            if (key[at] == top) { first = at; break; }
-                    e = (int)__reduce_min_sync(kAll, first);
-                    if (first == (uint32_t)e) {
-                        key[e] = 0;
-                        best = 0;
-                        for (int at = lane; at < E; at += 32) best = max(best, key[at]);
-                    }
+            // the k-th largest of the lanes' maxima (sorted by a bitonic network)
+            uint32_t bound = best;
+#pragma unroll
+            for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+                for (int step = size / 2; step; step /= 2) {
+                    const uint32_t other = __shfl_xor_sync(kAll, bound, step);
+                    bound = ((lane & size) == 0) == ((lane & step) == 0) ? max(bound, other) : min(bound, other);
+                }
+            bound = max(__shfl_sync(kAll, bound, k - 1), kInfKey + 1);
+            int own = 0;
+#pragma unroll
+            for (int j = 0; j < V; ++j) own += key_of(x[j]) >= bound;
+            int at = own;
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) {
+                const int before = __shfl_up_sync(kAll, at, o);
+                if (lane >= o) at += before;
+            }
+            const int c = __shfl_sync(kAll, at, 31);
+            at -= own;
+            if (c <= 32) {
+                uint64_t *list = s_list[warp];  // key, and the expert so that lower ones are larger
+                __syncwarp();                   // the list of the token before is not read any more
+                if (lane < 4) list[c + lane] = 0;
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const uint32_t q = key_of(x[j]);
+                    if (q >= bound) list[at++] = (uint64_t)q << 32 | (uint32_t)~(j * 32 + lane);
                 }
                 __syncwarp();
-                if (lane == s) { sel = e; sel_key = top; }
+                if (lane < c) {
+                    const uint64_t mine = list[lane];
+                    int rank = 0;
+                    for (int i = 0; i < c; i += 4)
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) rank += list[i + u] > mine;
+                    slot = rank;
+                    sel = rank < k ? (int)~(uint32_t)mine : -1;
+                    sel_key = (uint32_t)(mine >> 32);
+                }
+            } else {
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < V; ++j) key[j * 32 + lane] = j * 32 + lane < E ? key_of(x[j]) : 0;
+                __syncwarp();
+                for (int s = 0; s < k; ++s) {
+                    const uint32_t now = __reduce_max_sync(kAll, best);
+                    if (now <= kInfKey) break;
+                    uint32_t first = kAll;  // the lowest expert with that key
+                    if (best == now)
+                        for (int e = lane; e < S; e += 32)
+                            if (key[e] == now) { first = e; break; }
+                    const uint32_t e = __reduce_min_sync(kAll, first);
+                    if (first == e) {
+                        key[e] = 0;
+                        best = 0;
+                        for (int i = lane; i < S; i += 32) best = max(best, key[i]);
+                    }
+                    __syncwarp();
+                    if (lane == s) { sel = (int)e; sel_key = now; }
+                }
             }
             float z = 0.f;
 #pragma unroll
@@ -189,7 +202,7 @@ __global__ void __launch_bounds__(kGateMost<V>, kGateCtas<V>) moe_gate_kernel(co
                 z += x[j];
             }
             z = warp_sum(z);
-            const float inv = 1.f / z;
+            const float inv = __fdividef(1.f, z);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 if (kInRegs<V>) sums[kInRegs<V> ? j : 0] += x[j] * inv;
@@ -197,12 +210,12 @@ __global__ void __launch_bounds__(kGateMost<V>, kGateCtas<V>) moe_gate_kernel(co
             }
             const float g = sel >= 0 ? exp_of(value_of(sel_key) - m) : 0.f;
             const float whole = a.normalize ? warp_sum(g) : z;
-            if (lane < k) a.gates[t * k + lane] = g / whole;
+            if (slot < k) a.gates[t * k + slot] = __fdividef(g, whole);
             if (sel >= 0) atomicAdd(&s_c[sel], 1);
             ++mine;
         } else if (lane < k)
             a.gates[t * k + lane] = 0.f;
-        if (lane < k) a.idx[t * k + lane] = sel;
+        if (slot < k) a.idx[t * k + slot] = sel;
     }
     if (kInRegs<V>)
 #pragma unroll
@@ -350,10 +363,10 @@ __global__ void __launch_bounds__(kGateMost<V>, kGateCtas<V>) moe_gate_grad_kern
 #pragma unroll
         for (int j = 0; j < V; ++j) { x[j] = exp_of(x[j] - m); z += x[j]; }
         z = warp_sum(z);
-        const float inv = 1.f / z;
+        const float inv = __fdividef(1.f, z);
         float g = exp_of(sel_x - m);   // 0 where the slot is empty
         const float whole = a.normalize ? warp_sum(g) : z;
-        g = g > 0.f ? g / whole : g;
+        g = g > 0.f ? __fdividef(g, whole) : g;
         const float gd = warp_sum(g * dg);
         if (sel >= 0) extra[sel] = a.normalize ? g * (dg - gd) : g * dg;
         float dot = 0.f;
