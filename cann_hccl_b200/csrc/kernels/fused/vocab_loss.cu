@@ -45,7 +45,7 @@ enum Mode : int { SCORES = 0, DX = 1, DW = 2 };
 constexpr int kThreads = 320, kEpiWarps = 8;
 constexpr uint32_t kABytes = BM * BK * 2, kStageSpace = 7 * 32768;  // seven stages of a pair
 constexpr uint32_t kTmemCols = 512;
-constexpr int kMaxStages = 8, kMinCols = 128, kMaxCols = BN;
+constexpr int kMaxStages = 8, kMaxCols = BN;
 constexpr uint32_t kChunkBytes = BK * 128;         // MN-major: 64 elements x 64 deep
 constexpr float kExpBits = 15.f, kExpScale = 1.f / 32768.f, kLog2e = 1.4426950408889634f;
 
@@ -59,7 +59,7 @@ struct alignas(64) LossGemm {
     // scores
     float2 *stats;                   // [row][2 * n_tiles]: maximum, sum of exp(s - maximum)
     float *target;                   // [row]
-    __half *e;                       // [row][ld], may be null
+    __half *e;                       // [row][ld], of which `width` columns are written; may be null
     const void *y;
     int64_t first, ignore;
     int wide_y;
@@ -67,8 +67,7 @@ struct alignas(64) LossGemm {
     __nv_bfloat16 *out;
     float *sum;                      // shares of dx: [share][row][N]
     int kind;                        // VocabLossOut
-    int64_t ld;
-    int wide;                        // rows of out start on 32-byte boundaries
+    int64_t ld, width;
     const float *total;              // the sums are multiplied by scale / *total (null: scale; a total of 0: 0)
     float scale;
 };
@@ -82,6 +81,13 @@ struct LossShared {
 };
 constexpr size_t kSmemBytes = sizeof(LossShared) + 1024;
 static_assert(kSmemBytes <= 227 * 1024, "one CTA per SM");
+
+// Pairs turn bf16 dW around in the end of the stages' space, 32 rows x 64 columns of a warp at a time, so that a store covers whole 128-byte
+// lines: a lane's own row in 32-byte stores moves 16 bytes per cycle and SM (1 token, 128256 x 4096: 252 us, 214 this way; as boxes
+// stored by the TMA 335 us).  The exponentials leave in 32-byte stores all the same: beside their 128 values a lane has no
+// registers left for it (1024 tokens, 160000 x 256: 218 against 117 us).
+constexpr uint32_t kTurnWarp = 32 * 128, kTurnSpace = kEpiWarps * kTurnWarp;
+template <int MODE, bool kPair> constexpr bool kTurn = kPair && MODE == DW;
 
 // MN-major operand, 128-byte swizzle: 64 elements side by side, 8 deep in 1024 bytes, the next 64 elements kChunkBytes on.
 __device__ __forceinline__ uint64_t make_desc_mn(const void *ptr)
@@ -137,7 +143,17 @@ __device__ __forceinline__ void tmem_half(uint32_t addr, float (&v)[kHalf])
     for (int i = 0; i < kHalf; ++i) v[i] = __uint_as_float(r[i / 32][i % 32]);
 }
 
-// The same in steps of 32 columns, for single CTAs: each of them has a few tiles at most, the code above would come from memory once for
+__device__ __forceinline__ void tmem_64(uint32_t addr, float (&v)[64])
+{
+    uint32_t r[2][32];
+    tmem_ld32(addr, r[0]);
+    tmem_ld32(addr + 32, r[1]);
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i / 32][i % 32]);
+}
+
+// tmem_half in steps of 32 columns, for single CTAs: each of them has a few tiles at most, the code above would come from memory once for
 // every tile (7 tokens x 32000 x 4096: 55 against 50 us), and memory sets the pace anyway.
 __device__ __forceinline__ void tmem_32(uint32_t addr, int left, float (&v)[32])
 {
@@ -147,44 +163,35 @@ __device__ __forceinline__ void tmem_32(uint32_t addr, int left, float (&v)[32])
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = i < left ? __uint_as_float(r[i]) : -INFINITY;
 }
-__device__ __forceinline__ void put_exp(__half *e, const float *v)
+template <int C> __device__ __forceinline__ void put_exp(__half *e, const float (&v)[C], int room)
 {
-    uint32_t o[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-        o[i] = *(const uint32_t *)&h;
-    }
-    st_v8(e, o);
+    for (int c = 0; c < C; c += 16)
+        if (c < room) {
+            uint32_t o[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const __half2 h = __floats2half2_rn(v[c + 2 * i], v[c + 2 * i + 1]);
+                o[i] = *(const uint32_t *)&h;
+            }
+            st_v8(e + c, o);
+        }
 }
 
-// 16 results of a row, of which `left` exist (a multiple of 8).
-__device__ __forceinline__ void put16(const LossGemm &P, int64_t at, float *sum, float *v, int left, float scale)
+// v: eight 16-byte pieces of the lane's row; to: the first piece of the warp's first row; rows, pieces: that exist.
+__device__ __forceinline__ void turn_store(uint8_t *box, const uint4 (&v)[8], int lane, uint8_t *to, int64_t row_bytes, int rows, int pieces)
 {
+    __syncwarp();  // what was here has been read
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] *= scale;
-    if (P.kind == VL_ADD || P.kind == VL_ADD_BF16)
+    for (int c = 0; c < 8; ++c) *(uint4 *)(box + lane * 128 + (c ^ (lane & 7)) * 16) = v[c];
+    __syncwarp();
+    const int c = lane & 7;
+    if (c < pieces)
 #pragma unroll
-        for (int c = 0; c < 16; c += 4)
-            if (c < left) {
-                const float4 f = *(const float4 *)(sum + at + c);
-                v[c] += f.x; v[c + 1] += f.y; v[c + 2] += f.z; v[c + 3] += f.w;
-            }
-    if (P.kind == VL_F32 || P.kind == VL_ADD) {
-#pragma unroll
-        for (int c = 0; c < 16; c += 4)
-            if (c < left) *(float4 *)(sum + at + c) = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
-    } else {
-        uint32_t o[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = pack_bf16(__float_as_uint(v[2 * i]), __float_as_uint(v[2 * i + 1]));
-        __nv_bfloat16 *p = P.out + at;
-        if (P.wide && left >= 16) st_v8(p, o);
-        else {
-            if (left >= 8) ((uint4 *)p)[0] = make_uint4(o[0], o[1], o[2], o[3]);
-            if (left >= 16) ((uint4 *)p)[1] = make_uint4(o[4], o[5], o[6], o[7]);
+        for (int i = 0; i < 8; ++i) {
+            const int r = i * 4 + (lane >> 3);
+            if (r < rows) *(uint4 *)(to + r * row_bytes + c * 16) = *(const uint4 *)(box + r * 128 + (c ^ (r & 7)) * 16);
         }
-    }
 }
 
 template <int MODE, bool kPair>
@@ -204,7 +211,7 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_loss_gemm(const __grid_cons
     if (threadIdx.x == 0) {
         S.fail = 0;
         for (int i = 0; i < kMaxStages; ++i) { mbar_init(&S.full_bar[i], 1); mbar_init(&S.empty_bar[i], 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&S.tmem_full[i], 1); mbar_init(&S.tmem_empty[i], kCtas * kEpiWarps); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&S.tmem_full[i], 1); mbar_init(&S.tmem_empty[i], kEpiWarps); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         prefetch_tensormap(&P.tmA);
         prefetch_tensormap(&P.tmB);
@@ -288,10 +295,14 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_loss_gemm(const __grid_cons
             }
         }
     } else {
-        // ------------------------------------------------------------------ epilogue: a warp reaches its TMEM lane quarter, half of the columns
-        const int q4 = warp & 3, half = (warp - 2) >> 2, rl = q4 * 32 + lane;
-        const int mid = (P.cols / 16 + 1) / 2 * 16, c_lo = half ? mid : 0, c_hi = half ? P.cols : mid;
-        uint32_t n = 0;
+        // ------------------------------------------------------------------ epilogue: a warp reaches its TMEM lane quarter.  Single: the two
+        // warps of a quarter take half of the columns each.  Pair: they take tiles in turn, one accumulator each, so that one waits for
+        // TMEM while the other stores.
+        const int q4 = warp & 3, group = (warp - 2) >> 2, rl = q4 * 32 + lane;
+        const int mid = (P.cols / 16 + 1) / 2 * 16, half0 = kPair ? 0 : group, halves = kPair ? 2 : 1;
+        const int every = kPair ? 2 : 1;  // tile of this warp
+        uint8_t *box = S.tiles + kStageSpace - kTurnSpace + (warp - 2) * kTurnWarp;
+        uint32_t n = kPair ? group : 0;
         bool bad = false;
         // This warp has read the accumulator.  Relaxed: the loads are complete, and a release would wait for the results stored so far
         // to reach memory, a microsecond and more on every tile (1531 x 50257 x 1000: scores 153 us, tensor cores busy for 51 %).
@@ -304,7 +315,7 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_loss_gemm(const __grid_cons
         };
         float scale = P.scale;
         if (MODE != SCORES && P.total) scale = *P.total != 0.f ? scale / *P.total : 0.f;
-        for (int t = unit; t < total; t += P.units, ++n) {
+        for (int t = unit + (int)n * P.units; t < total; t += every * P.units, n += every) {
             const Tile w = tile_at(P, t);
             const int row = (w.um * kCtas + (int)cta_r) * BM + rl, col0 = w.nt * P.cols;
             const uint32_t buf = n & 1, use = n >> 1, taddr = tmem_base + buf * kMaxCols + ((uint32_t)(q4 * 32) << 16);
@@ -316,81 +327,114 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_loss_gemm(const __grid_cons
             bad = bad || !mbar_wait_t<kPair>(&S.tmem_full[buf], use & 1, fail);
             bad = __any_sync(0xffffffffu, bad);
             tc_fence_after();
-            if (MODE == SCORES) {
-                const int exist = min(c_hi, P.N - col0) - c_lo;  // columns of this half that exist, the first of them
-                const int room = row < P.M && P.e ? (int)min((int64_t)c_hi, P.ld - col0) - c_lo : 0;  // the row ends on a multiple of 64, in zeros
-                const int yl = y >= c_lo && y < c_lo + exist ? (int)y - c_lo : -1;
-                __half *e = P.e + (int64_t)row * P.ld + col0 + c_lo;
-                float m = -INFINITY, z = 0.f, target = 0.f;
-                if constexpr (kPair) {
-                    float v[kHalf];
-                    if (!bad) tmem_half(taddr + c_lo, v);
-                    release(buf);
-                    if (exist < kHalf)
-#pragma unroll
-                        for (int i = 0; i < kHalf; ++i) v[i] = i < exist ? v[i] : -INFINITY;
-                    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, z4[4] = {};
-#pragma unroll
-                    for (int i = 0; i < kHalf; ++i) m4[i & 3] = fmaxf(m4[i & 3], v[i]);
-                    m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-                    const float ref = m == -INFINITY ? 0.f : m;
-                    if (yl >= 0)
-#pragma unroll
-                        for (int i = 0; i < kHalf; ++i) target = i == yl ? v[i] : target;
-                    // (v - m first: the product with m alone would carry m's size into every exponent)
-#pragma unroll
-                    for (int i = 0; i < kHalf; ++i) {
-                        v[i] = exp2_approx(fmaf(v[i] - ref, kLog2e, kExpBits));
-                        z4[i & 3] += v[i];
-                    }
-                    z = (z4[0] + z4[1]) + (z4[2] + z4[3]);
-#pragma unroll
-                    for (int c = 0; c < kHalf; c += 16)
-                        if (c < room) put_exp(e + c, v + c);
-                } else {
-                    float v[32];
-                    if (!bad) {
-#pragma unroll 1
-                        for (int c = 0; c < exist; c += 32) {
-                            tmem_32(taddr + c_lo + c, exist - c, v);
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) m = fmaxf(m, v[i]);
-                        }
-                        const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll 1
-                        for (int c = 0; c < c_hi - c_lo; c += 32) {
-                            tmem_32(taddr + c_lo + c, exist - c, v);
-                            if (yl >= c && yl < c + 32)
-#pragma unroll
-                                for (int i = 0; i < 32; ++i) target = i == yl - c ? v[i] : target;
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) {
-                                v[i] = exp2_approx(fmaf(v[i] - ref, kLog2e, kExpBits));
-                                z += v[i];
-                            }
-                            if (c < room) put_exp(e + c, v);
-                            if (c + 16 < room) put_exp(e + c + 16, v + 16);
-                        }
-                    }
-                    release(buf);
-                }
-                if (row < P.M) {
-                    if (yl >= 0) P.target[row] = target;
-                    P.stats[(int64_t)row * (2 * P.n_tiles) + 2 * w.nt + half] = make_float2(m, bad ? __uint_as_float(0x7fffffffu) : z * kExpScale);
-                }
-            } else {
-                float v[kHalf];
-                if (!bad) tmem_half(taddr + c_lo, v);
-                else
-#pragma unroll
-                    for (int i = 0; i < kHalf; ++i) v[i] = __uint_as_float(0x7fffffffu);
+            if (row - lane >= P.M) {  // a warp of rows that do not exist
                 release(buf);
-                float *sum = P.sum + (P.split > 1 ? (int64_t)w.share * P.M * P.N : 0);
-                const int exist = row < P.M ? min(c_hi, P.N - col0) - c_lo : 0;
-                const int64_t at = (int64_t)row * P.N + col0 + c_lo;
+                continue;
+            }
+#pragma unroll 1
+            for (int half = half0; half < half0 + halves; ++half) {
+                const int c_lo = half ? mid : 0, c_hi = half ? P.cols : mid;
+                const bool last = half == half0 + halves - 1;  // the accumulator is free when its last half is read
+                if (MODE == SCORES) {
+                    const int exist = min(c_hi, P.N - col0) - c_lo;  // columns of this half that exist, the first of them
+                    const int room = (int)min((int64_t)c_hi, P.width - col0) - c_lo;  // the row ends on a multiple of 32, in zeros
+                    const int yl = y >= c_lo && y < c_lo + exist ? (int)y - c_lo : -1;
+                    __half *e = P.e + (int64_t)row * P.ld + col0 + c_lo;
+                    float m = -INFINITY, z = 0.f, target = 0.f;
+                    if constexpr (kPair) {
+                        float v[kHalf];
+                        if (!bad) tmem_half(taddr + c_lo, v);
+                        if (last) release(buf);
+                        if (exist < kHalf)
 #pragma unroll
-                for (int c = 0; c < kHalf; c += 16)
-                    if (c < exist) put16(P, at + c, sum, v + c, exist - c, scale);
+                            for (int i = 0; i < kHalf; ++i) v[i] = i < exist ? v[i] : -INFINITY;
+                        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, z4[4] = {};
+#pragma unroll
+                        for (int i = 0; i < kHalf; ++i) m4[i & 3] = fmaxf(m4[i & 3], v[i]);
+                        m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+                        const float ref = m == -INFINITY ? 0.f : m;
+                        if (yl >= 0)
+#pragma unroll
+                            for (int i = 0; i < kHalf; ++i) target = i == yl ? v[i] : target;
+                        // v - m first: the product with m alone would carry m's size into every exponent
+#pragma unroll
+                        for (int i = 0; i < kHalf; ++i) {
+                            v[i] = exp2_approx(fmaf(v[i] - ref, kLog2e, kExpBits));
+                            z4[i & 3] += v[i];
+                        }
+                        z = (z4[0] + z4[1]) + (z4[2] + z4[3]);
+                        if (P.e && row < P.M) put_exp(e, v, room);
+                    } else {
+                        float v[32];
+                        if (!bad) {
+#pragma unroll 1
+                            for (int c = 0; c < exist; c += 32) {
+                                tmem_32(taddr + c_lo + c, exist - c, v);
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) m = fmaxf(m, v[i]);
+                            }
+                            const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll 1
+                            for (int c = 0; c < c_hi - c_lo; c += 32) {
+                                tmem_32(taddr + c_lo + c, exist - c, v);
+                                if (yl >= c && yl < c + 32)
+#pragma unroll
+                                    for (int i = 0; i < 32; ++i) target = i == yl - c ? v[i] : target;
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) {
+                                    v[i] = exp2_approx(fmaf(v[i] - ref, kLog2e, kExpBits));
+                                    z += v[i];
+                                }
+                                if (P.e && row < P.M) put_exp(e + c, v, room - c);
+                            }
+                        }
+                        if (last) release(buf);
+                    }
+                    if (row < P.M) {
+                        if (yl >= 0) P.target[row] = target;
+                        P.stats[(int64_t)row * (2 * P.n_tiles) + 2 * w.nt + half] = make_float2(m, bad ? __uint_as_float(0x7fffffffu) : z * kExpScale);
+                    }
+                } else {
+                    float *sum = P.sum + (P.split > 1 ? (int64_t)w.share * P.M * P.N : 0);
+                    const int left = min(c_hi, P.N - col0) - c_lo, exist = row < P.M ? left : 0;
+                    const int64_t at = (int64_t)row * P.N + col0 + c_lo;
+#pragma unroll
+                    for (int c = 0; c < kHalf; c += 64) {
+                        float v[64];
+                        if (!bad) tmem_64(taddr + c_lo + c, v);
+                        else
+#pragma unroll
+                            for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(0x7fffffffu);
+                        if (last && c + 64 == kHalf) release(buf);
+#pragma unroll
+                        for (int i = 0; i < 64; ++i) v[i] *= scale;
+                        if (P.kind == VL_ADD || P.kind == VL_ADD_BF16)
+#pragma unroll
+                            for (int i = 0; i < 64; i += 4)
+                                if (c + i < exist) {
+                                    const float4 f = *(const float4 *)(sum + at + c + i);
+                                    v[i] += f.x; v[i + 1] += f.y; v[i + 2] += f.z; v[i + 3] += f.w;
+                                }
+                        if (P.kind == VL_F32 || P.kind == VL_ADD) {
+#pragma unroll
+                            for (int i = 0; i < 64; i += 4)
+                                if (c + i < exist) *(float4 *)(sum + at + c + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                        } else if (c < left) {
+                            uint4 o[8];
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                o[j].x = pack_bf16(__float_as_uint(v[8 * j]), __float_as_uint(v[8 * j + 1])); o[j].y = pack_bf16(__float_as_uint(v[8 * j + 2]), __float_as_uint(v[8 * j + 3]));
+                                o[j].z = pack_bf16(__float_as_uint(v[8 * j + 4]), __float_as_uint(v[8 * j + 5])); o[j].w = pack_bf16(__float_as_uint(v[8 * j + 6]), __float_as_uint(v[8 * j + 7]));
+                            }
+                            if constexpr (kTurn<MODE, kPair>)
+                                turn_store(box, o, lane, (uint8_t *)(P.out + at - (int64_t)lane * P.N + c), (int64_t)P.N * 2, P.M - (row - lane), (left - c) / 8);
+                            else
+#pragma unroll
+                                for (int j = 0; j < 8; ++j)
+                                    if (c + 8 * j < exist) *(uint4 *)(P.out + at + c + 8 * j) = o[j];
+                        }
+                    }
+                }
             }
         }
     }
@@ -414,7 +458,7 @@ struct RowArgs {
     uint8_t *e;                      // [row][ld] 2 bytes each
     const uint8_t *x, *w;
     uint8_t *xc;
-    int64_t tokens, first, vocab, whole, ignore, ld, x_stride, w_stride;  // strides in bytes
+    int64_t tokens, first, vocab, whole, ignore, ld, width, x_stride, w_stride;  // x_stride, w_stride: in bytes
     int wide, halves, cols, n_tiles, shards, xvec;
 };
 
@@ -570,79 +614,86 @@ __global__ void __launch_bounds__(kCopyThreads) vocab_loss_x(const __grid_consta
     ((uint4 *)a.xc)[t * (a.ld / 8) + v] = on ? ((const uint4 *)(a.x + t * a.x_stride))[v] : make_uint4(0, 0, 0, 0);
 }
 
-constexpr int kDThreads = 256, kDBatch = 4;
-
-// Exponentials -> d, in place.  One CTA per token, a warp's lanes share a tile (8 columns each).
+constexpr int kDThreads = 256, kDBatch = 4, kDVecs = kDThreads * kDBatch;
+// Exponentials -> d, in place.  grid (stretches of a row, tokens): kDVecs vectors of 8 columns at a time, in turn.
 __global__ void __launch_bounds__(kDThreads) vocab_loss_d(const __grid_constant__ RowArgs a)
 {
     pdl_trigger();
     pdl_wait();
-    const int64_t t = blockIdx.x;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t t = blockIdx.y;
     const int64_t id = target_of(a.y, a.wide, t);
     const float q = !counts(a, id) ? 0.f : a.weights ? a.weights[t] : 1.f;
     uint4 *row = (uint4 *)(a.e + t * a.ld * 2);
-    if (q == 0.f) {
-        for (int v = threadIdx.x; v < a.ld / 8; v += kDThreads) row[v] = make_uint4(0, 0, 0, 0);
-        return;
-    }
+    const uint32_t vecs = (uint32_t)(a.width / 8), cols = (uint32_t)a.cols, mid = (cols / 16 + 1) / 2 * 16;
     const float lse = a.lse[t];
     const int64_t y = id - a.first;  // may lie in another shard
     const float dy = q * expm1f(a.target[t] - lse);
-    const int mid = (a.cols / 16 + 1) / 2 * 16, c = lane * 8, half = c >= mid;
-    const float2 *stats = a.stats + t * a.halves + half;
-    for (int n0 = warp; n0 < a.n_tiles; n0 += kDThreads / 32 * kDBatch) {
+    const float2 *stats = a.stats + t * a.halves;
+    for (uint32_t v0 = blockIdx.x * kDVecs + threadIdx.x; v0 < vecs; v0 += gridDim.x * kDVecs) {
         uint4 v[kDBatch];
         float f[kDBatch];
+        if (q != 0.f)
 #pragma unroll
-        for (int k = 0; k < kDBatch; ++k) {
-            const int n = n0 + k * (kDThreads / 32);
-            if (n < a.n_tiles && c < a.cols && (int64_t)n * a.cols + c < a.ld) {
-                v[k] = row[(n * (int64_t)a.cols + c) / 8];
-                f[k] = stats[2 * n].x;
+            for (int k = 0; k < kDBatch; ++k) {
+                const uint32_t i = v0 + k * kDThreads, col = i * 8, n = col / cols;
+                if (i < vecs) {
+                    v[k] = row[i];
+                    f[k] = stats[2 * n + (col - n * cols >= mid)].x;
+                }
             }
-        }
 #pragma unroll
         for (int k = 0; k < kDBatch; ++k) {
-            const int n = n0 + k * (kDThreads / 32);
-            const int64_t col = (int64_t)n * a.cols + c;
-            if (n < a.n_tiles && c < a.cols && col < a.ld) {
+            const uint32_t i = v0 + k * kDThreads;
+            if (i >= vecs) break;
+            uint4 o = make_uint4(0, 0, 0, 0);
+            if (q != 0.f) {
                 const float fac = __expf(f[k] - lse) * q * kExpScale;
                 float d[8];
                 const __half2 *h = (const __half2 *)&v[k];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 u = __half22float2(h[i]);
-                    d[2 * i] = u.x * fac; d[2 * i + 1] = u.y * fac;
+                for (int j = 0; j < 4; ++j) {
+                    const float2 u = __half22float2(h[j]);
+                    d[2 * j] = u.x * fac; d[2 * j + 1] = u.y * fac;
                 }
-                if (y >= col && y < col + 8 && y < a.vocab)
+                const int64_t at = y - (int64_t)i * 8;
+                if (at >= 0 && at < 8 && y < a.vocab)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) d[i] = i == (int)(y - col) ? dy : d[i];
-                uint4 o;
+                    for (int j = 0; j < 8; ++j) d[j] = j == (int)at ? dy : d[j];
                 o.x = pack_bf16(__float_as_uint(d[0]), __float_as_uint(d[1])); o.y = pack_bf16(__float_as_uint(d[2]), __float_as_uint(d[3]));
                 o.z = pack_bf16(__float_as_uint(d[4]), __float_as_uint(d[5])); o.w = pack_bf16(__float_as_uint(d[6]), __float_as_uint(d[7]));
-                row[col / 8] = o;
             }
+            row[i] = o;
         }
     }
 }
 
 struct ShareArgs { const float *shares; __nv_bfloat16 *out; int64_t n; int split; };
-// Shares of dx added in order.
-__global__ void __launch_bounds__(256) vocab_loss_shares(const __grid_constant__ ShareArgs a)
+constexpr int kShareSlices = 8;
+// Shares of dx added: a warp's lanes hold 8 values each, the warps of a CTA a part of the shares each, whose sums are added in order.
+__global__ void __launch_bounds__(32 * kShareSlices) vocab_loss_shares(const __grid_constant__ ShareArgs a)
 {
+    __shared__ float s_v[kShareSlices][8][33];
     pdl_trigger();
-    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t i = ((int64_t)blockIdx.x * 32 + lane) * 8;
     pdl_wait();
-    if (i >= a.n) return;
     float v[8] = {};
+    if (i < a.n)
 #pragma unroll 4
-    for (int q = 0; q < a.split; ++q) {
-        const float4 *p = (const float4 *)(a.shares + q * a.n + i);
-        const float4 x = p[0], y = p[1];
-        v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
-        v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
-    }
+        for (int q = warp; q < a.split; q += kShareSlices) {
+            const float4 *p = (const float4 *)(a.shares + q * a.n + i);
+            const float4 x = p[0], y = p[1];
+            v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+            v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+        }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s_v[warp][k][lane] = v[k];
+    __syncthreads();
+    if (warp || i >= a.n) return;
+#pragma unroll
+    for (int w = 1; w < kShareSlices; ++w)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] += s_v[w][k][lane];
     uint4 o;
     o.x = pack_bf16(__float_as_uint(v[0]), __float_as_uint(v[1])); o.y = pack_bf16(__float_as_uint(v[2]), __float_as_uint(v[3]));
     o.z = pack_bf16(__float_as_uint(v[4]), __float_as_uint(v[5])); o.w = pack_bf16(__float_as_uint(v[6]), __float_as_uint(v[7]));
@@ -706,19 +757,19 @@ HcclResult encode(CUtensorMap *map, const void *base, int64_t rows, int64_t cols
     return HCCL_SUCCESS;
 }
 
-// Columns of a tile of the scores: whole waves (the widest among equals).
-int score_cols(int64_t um, int64_t vocab, int units)
+// Columns of a tile of the scores: the fewest columns (and ends of tiles, about 48 columns' worth each) for the busiest unit.
+int score_cols(int64_t um, int64_t vocab, bool pair, int units)
 {
     int best = kMaxCols;
     int64_t least = INT64_MAX;
-    for (int cols = kMaxCols; cols >= kMinCols; cols -= 32) {
-        const int64_t tiles = um * ((vocab + cols - 1) / cols), t = (tiles + units - 1) / units * cols;
+    for (int cols = kMaxCols; cols >= (pair ? 64 : 32); cols -= 32) {
+        const int64_t tiles = um * ((vocab + cols - 1) / cols), t = (tiles + units - 1) / units * (cols + 48);
         if (t < least) { least = t; best = cols; }
     }
     return best;
 }
 
-struct Layout { int cols, n_tiles; int64_t ld, xld, stats, xc, shares, bytes; bool pair, copy; int split; };
+struct Layout { int cols, n_tiles; int64_t ld, width, xld, stats, xc, shares, bytes; bool pair, copy; int split; };
 
 int shares_of(int64_t tokens, int64_t vocab, int32_t hidden, const LossDevice &d, bool pair)
 {
@@ -741,9 +792,10 @@ HcclResult layout_of(int64_t tokens, int64_t vocab, int32_t hidden, bool grad, L
     CHK_RET(loss_device(&d));
     auto up = [](int64_t n) { return (n + 1023) / 1024 * 1024; };
     l->pair = tokens > BM;
-    l->cols = score_cols((tokens + (l->pair ? 255 : 127)) / (l->pair ? 256 : 128), vocab, l->pair ? d.pairs : d.sms);
+    l->cols = score_cols((tokens + (l->pair ? 255 : 127)) / (l->pair ? 256 : 128), vocab, l->pair, l->pair ? d.pairs : d.sms);
     l->n_tiles = (int)((vocab + l->cols - 1) / l->cols);
-    l->ld = (vocab + 63) / 64 * 64;
+    l->ld = (vocab + 63) / 64 * 64;      // rows of the exponentials start on 128-byte lines,
+    l->width = (vocab + 31) / 32 * 32;   // and are written as far as the tiles (multiples of 32 columns) reach for certain
     l->split = grad ? shares_of(tokens, vocab, hidden, d, l->pair) : 1;
     l->stats = grad ? up(tokens * l->ld * 2) : 0;
     l->xc = l->stats + up(tokens * l->n_tiles * 2 * (int64_t)sizeof(float2));
@@ -756,8 +808,9 @@ HcclResult layout_of(int64_t tokens, int64_t vocab, int32_t hidden, bool grad, L
     return HCCL_SUCCESS;
 }
 
-// Rows of A in a stage.
-int a_rows(int mode, int m) { return mode == DW || m >= BM ? BM : (m + 7) / 8 * 8; }
+// Rows of A in a stage.  Of fewer than 128 rows only those that exist are loaded (in eights, the swizzle's period) where B is long enough:
+// the tensor cores read what follows them in shared memory, B, for results that nobody reads (7 tokens x 32000 x 4096: 62 -> 56 us).
+int a_rows(int mode, int m, int cols) { return mode == DW || m >= BM || (uint32_t)cols * BK * 2 < kABytes ? BM : (m + 7) / 8 * 8; }
 
 HcclResult launch_gemm(int mode, bool pair, LossGemm &P, void *stream)
 {
@@ -767,12 +820,10 @@ HcclResult launch_gemm(int mode, bool pair, LossGemm &P, void *stream)
     P.um_tiles = (P.M + ctas * BM - 1) / (ctas * BM);
     P.n_tiles = (P.N + P.cols - 1) / P.cols;
     P.units = pair ? d.pairs : d.sms;
-    // Of fewer than 128 rows only those that exist are loaded (in eights, the swizzle's period): the tensor cores read what follows them
-    // in shared memory instead, for results that nobody reads.  A stage behind which less than that follows does not exist.
-    P.a_bytes = (uint32_t)a_rows(mode, P.M) * BK * 2;
+    P.a_bytes = (uint32_t)a_rows(mode, P.M, P.cols) * BK * 2;
     P.stage_bytes = P.a_bytes + (uint32_t)(P.cols / ctas) * BK * 2;
-    static_assert(kABytes <= kMinCols * BK * 2, "A's rows end inside the stage's B");
-    P.stages = (int)std::min<uint32_t>(kMaxStages, kStageSpace / P.stage_bytes);
+    const bool turned = pair && mode == DW && (P.kind == VL_BF16 || P.kind == VL_ADD_BF16);
+    P.stages = (int)std::min<uint32_t>(kMaxStages, (kStageSpace - (turned ? kTurnSpace : 0)) / P.stage_bytes);
     P.idesc = instr_desc((uint32_t)(ctas * BM), (uint32_t)P.cols) | (mode == DW ? 1u << 15 : 0u) | (mode != SCORES ? 1u << 16 : 0u);
     // a panel's columns of B stay in L2 (40 MB of it) while the rows stream past
     P.panel = (int)std::min<int64_t>(P.n_tiles, std::max<int64_t>(8, (40ll << 20) / ((int64_t)P.cols * P.k_iters * BK * 2)));
@@ -815,7 +866,7 @@ HcclResult vocab_loss_scores(const VocabLossCall &c, bool grad, float *lse, floa
     P.M = (int)c.tokens; P.N = (int)c.vocab; P.cols = l.cols; P.split = 1;
     P.k_iters = (c.hidden + BK - 1) / BK;
     P.stats = (float2 *)(s + l.stats); P.target = target;
-    P.e = grad ? (__half *)s : nullptr; P.ld = l.ld;
+    P.e = grad ? (__half *)s : nullptr; P.ld = l.ld; P.width = l.width;
     P.y = c.targets; P.wide_y = c.wide; P.first = c.first; P.ignore = c.ignore;
     if (l.copy) {
         RowArgs a = row_args(c);
@@ -823,7 +874,7 @@ HcclResult vocab_loss_scores(const VocabLossCall &c, bool grad, float *lse, floa
         CHK_RET(launch_pdl((const void *)vocab_loss_x, dim3((unsigned)((c.tokens * a.xvec + kCopyThreads - 1) / kCopyThreads)), kCopyThreads, 0, &a, stream,
                            "vocabulary loss (x)"));
     }
-    CHK_RET(encode(&P.tmA, l.copy ? s + l.xc : c.x, c.tokens, c.hidden, l.copy ? l.xld : c.x_stride, a_rows(SCORES, (int)c.tokens)));
+    CHK_RET(encode(&P.tmA, l.copy ? s + l.xc : c.x, c.tokens, c.hidden, l.copy ? l.xld : c.x_stride, a_rows(SCORES, (int)c.tokens, l.cols)));
     CHK_RET(encode(&P.tmB, c.w, c.vocab, c.hidden, c.w_stride, l.cols / (l.pair ? 2 : 1)));
     CHK_RET(launch_gemm(SCORES, l.pair, P, stream));
     RowArgs a = row_args(c);
@@ -862,8 +913,18 @@ HcclResult vocab_loss_grad(const VocabLossCall &c, const float *lse, const float
     uint8_t *s = (uint8_t *)scratch;
     RowArgs a = row_args(c);
     a.stats = (const float2 *)(s + l.stats); a.halves = 2 * l.n_tiles; a.cols = l.cols; a.n_tiles = l.n_tiles;
-    a.e = s; a.ld = l.ld; a.lse = (float *)lse; a.target = (float *)target;
-    CHK_RET(launch_pdl((const void *)vocab_loss_d, dim3((unsigned)c.tokens), kDThreads, 0, &a, stream, "vocabulary loss (d)"));
+    a.e = s; a.ld = l.ld; a.width = l.width; a.lse = (float *)lse; a.target = (float *)target;
+    // enough CTAs to fill the GPU a few times, none without work (129 tokens x 160000 by one CTA each: 50 us)
+    const int64_t parts = std::min<int64_t>((l.width / 8 + kDVecs - 1) / kDVecs, std::max<int64_t>(1, 4096 / c.tokens));
+    // tokens along y, 65535 of them at most in a launch
+    for (int64_t t0 = 0; t0 < c.tokens; t0 += 65535) {
+        RowArgs q = a;
+        const int64_t n = std::min<int64_t>(65535, c.tokens - t0);
+        q.y = (const uint8_t *)a.y + t0 * (a.wide ? 8 : 4);
+        q.weights = a.weights ? a.weights + t0 : nullptr;
+        q.e += t0 * a.ld * 2; q.lse += t0; q.target += t0; q.stats += t0 * a.halves;
+        CHK_RET(launch_pdl((const void *)vocab_loss_d, dim3((unsigned)parts, (unsigned)n), kDThreads, 0, &q, stream, "vocabulary loss (d)"));
+    }
 
     LossGemm P;
     memset(&P, 0, sizeof(P));
@@ -873,13 +934,12 @@ HcclResult vocab_loss_grad(const VocabLossCall &c, const float *lse, const float
     P.split = l.split;
     P.kind = l.split > 1 ? VL_F32 : VL_BF16;
     P.out = (__nv_bfloat16 *)dx; P.sum = (float *)(s + l.shares);
-    P.wide = c.hidden % 16 == 0 && ((uintptr_t)dx & 31) == 0;
-    CHK_RET(encode(&P.tmA, s, c.tokens, l.ld, l.ld, a_rows(DX, (int)c.tokens)));
+    CHK_RET(encode(&P.tmA, s, c.tokens, l.width, l.ld, a_rows(DX, (int)c.tokens, kMaxCols)));
     CHK_RET(encode(&P.tmB, c.w, c.vocab, c.hidden, c.w_stride, BK));
     CHK_RET(launch_gemm(DX, l.pair, P, stream));
     if (l.split > 1) {
         ShareArgs q = {P.sum, P.out, c.tokens * c.hidden, l.split};
-        CHK_RET(launch_pdl((const void *)vocab_loss_shares, dim3((unsigned)((q.n / 8 + 255) / 256)), 256, 0, &q, stream, "vocabulary loss (dx)"));
+        CHK_RET(launch_pdl((const void *)vocab_loss_shares, dim3((unsigned)((q.n / 8 + 31) / 32)), 32 * kShareSlices, 0, &q, stream, "vocabulary loss (dx)"));
     }
 
     memset(&P, 0, sizeof(P));
@@ -887,8 +947,7 @@ HcclResult vocab_loss_grad(const VocabLossCall &c, const float *lse, const float
     P.total = total; P.scale = scale;
     P.k_iters = (int)((c.tokens + BK - 1) / BK);
     P.kind = out; P.out = (__nv_bfloat16 *)dw; P.sum = dw_sum;
-    P.wide = c.hidden % 16 == 0 && ((uintptr_t)dw & 31) == 0;
-    CHK_RET(encode(&P.tmA, s, c.tokens, l.ld, l.ld, BK));
+    CHK_RET(encode(&P.tmA, s, c.tokens, l.width, l.ld, BK));
     CHK_RET(encode(&P.tmB, s + l.xc, c.tokens, c.hidden, l.xld, BK));
     return launch_gemm(DW, c.vocab > BM, P, stream);
 }

@@ -84,7 +84,7 @@ class Exact:
 # one row of a tile, single CTAs (128 rows) and pairs, one to several tiles of either side, depths of one step and partly filled ones,
 # vocabularies below a tile, odd, and just beyond a multiple of it; dx cut along the vocabulary
 SHAPES = [(1, 1, 8), (1, 100, 8), (2, 33, 16), (7, 1000, 72), (128, 257, 64), (129, 512, 136), (256, 130, 64), (300, 1003, 1000), (513, 4097, 520), (40, 20001, 264),
-          (1000, 300, 2048), (640, 769, 24), (1531, 2050, 320)]
+          (1000, 300, 2048), (640, 769, 24), (1531, 2050, 320), (60, 4000, 72), (129, 4000, 128), (70001, 100, 8)]
 
 
 @pytest.mark.parametrize("T,V,hidden", SHAPES)
@@ -116,6 +116,17 @@ def test_gradients(T, V, hidden):
     e.dw = e.dw + start
     e.dw_err = e.dw_err + start.abs() * 2.0 ** -24
     e.check((loss, dx, dw), torch.float32)
+
+
+@pytest.mark.parametrize("V", [1, 33, 65, 97, 129, 161, 193, 220, 225, 289, 449, 673, 1345, 3137, 4480, 6657])
+def test_gradients_at_the_end_of_the_vocabulary(V):
+    """Tiles of every width whose last one ends near a multiple of 32 or 64: columns that no tile reaches are not read either (the scratch
+    holds NaN before)."""
+    for T in (5, 200):
+        x, w, y = problem(T, V, 40)
+        junk = torch.full((4 << 20,), 0x7fc0 * 0x10001, device="cuda", dtype=torch.int32)
+        del junk                                    # the allocator hands this memory out again
+        Exact(x, w, y).check(vocab.linear_cross_entropy_grad(x, w, y))
 
 
 def test_gradients_of_norm():
