@@ -123,6 +123,11 @@ __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_add
 {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
+// One of a lane's registers by its number; as a choice in C the registers would become an array in local memory.
+__device__ __forceinline__ void store_if(float *p, float v, bool yes)
+{
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %2, 0;\n @p st.global.f32 [%0], %1;\n}" ::"l"(p), "f"(v), "r"((int)yes) : "memory");
+}
 __device__ __forceinline__ float exp2_approx(float x)
 {
     float y;
@@ -340,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_loss_gemm(const __grid_cons
                     const int room = (int)min((int64_t)c_hi, P.width - col0) - c_lo;  // the row ends on a multiple of 32, in zeros
                     const int yl = y >= c_lo && y < c_lo + exist ? (int)y - c_lo : -1;
                     __half *e = P.e + (int64_t)row * P.ld + col0 + c_lo;
-                    float m = -INFINITY, z = 0.f, target = 0.f;
+                    float m = -INFINITY, z = 0.f;
                     if constexpr (kPair) {
                         float v[kHalf];
                         if (!bad) tmem_half(taddr + c_lo, v);
@@ -355,7 +360,7 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_loss_gemm(const __grid_cons
                         const float ref = m == -INFINITY ? 0.f : m;
                         if (yl >= 0)
 #pragma unroll
-                            for (int i = 0; i < kHalf; ++i) target = i == yl ? v[i] : target;
+                            for (int i = 0; i < kHalf; ++i) store_if(P.target + row, v[i], i == yl);
                         // v - m first: the product with m alone would carry m's size into every exponent
 #pragma unroll
                         for (int i = 0; i < kHalf; ++i) {
@@ -379,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_loss_gemm(const __grid_cons
                                 tmem_32(taddr + c_lo + c, exist - c, v);
                                 if (yl >= c && yl < c + 32)
 #pragma unroll
-                                    for (int i = 0; i < 32; ++i) target = i == yl - c ? v[i] : target;
+                                    for (int i = 0; i < 32; ++i) store_if(P.target + row, v[i], i == yl - c);
 #pragma unroll
                                 for (int i = 0; i < 32; ++i) {
                                     v[i] = exp2_approx(fmaf(v[i] - ref, kLog2e, kExpBits));
@@ -391,7 +396,6 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_loss_gemm(const __grid_cons
                         if (last) release(buf);
                     }
                     if (row < P.M) {
-                        if (yl >= 0) P.target[row] = target;
                         P.stats[(int64_t)row * (2 * P.n_tiles) + 2 * w.nt + half] = make_float2(m, bad ? __uint_as_float(0x7fffffffu) : z * kExpScale);
                     }
                 } else {
