@@ -54,7 +54,7 @@ class Calls:
 
     # model-side operators: tensors by their addresses, everything else as it is
     def _model(self, fn, a, tensors):
-        return fn(*[data_ptr(x) if i in tensors else x for i, x in enumerate(a)])
+        return fn(*[data_ptr(x) if i in tensors and not isinstance(x, int) else x for i, x in enumerate(a)])
 
     def embedding(self, *a):
         return self._model(self._lib.HcclB200Embedding, a, (0, 3, 10))

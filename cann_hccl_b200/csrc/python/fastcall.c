@@ -19,10 +19,14 @@ static combine_fn g_combine;
 static PyObject *s_data_ptr, *s_ctypes, *s_data, *s_numel, *s_size, *s_dtype;
 static PyObject *g_dtypes, *g_get_device, *g_get_stream;  /* {torch / numpy dtype: HcclDataType}, current device, its current raw stream */
 
-/* address of a tensor (data_ptr()) or numpy array (ctypes.data); None is null */
+/* address of a tensor (data_ptr()) or numpy array (ctypes.data), or an integer that is one; None is null */
 static int address(PyObject *x, void **out)
 {
     if (x == Py_None) { *out = NULL; return 0; }
+    if (PyLong_CheckExact(x)) {
+        *out = PyLong_AsVoidPtr(x);
+        return *out == NULL && PyErr_Occurred() ? -1 : 0;
+    }
     PyObject *v = PyObject_CallMethodNoArgs(x, s_data_ptr);
     if (!v) {
         if (!PyErr_ExceptionMatches(PyExc_AttributeError)) return -1;

@@ -17,7 +17,6 @@ Counts travel over the device (all-gather of the per-expert histogram); nothing 
 all-local communicator every tensor argument is a list with one entry per virtual rank.
 """
 import ctypes as C
-from collections import namedtuple
 
 import torch
 
@@ -146,7 +145,61 @@ class MoEExchange:
         self.comm.mem_free(self.h_out)
 
 
-Gate = namedtuple("Gate", "idx gates counts prob_sum routed balance")
+class _Part:
+    """A part of a Gate's memory, made a tensor at its first use (an instance attribute of the same name then takes over)."""
+
+    def __init__(self, place, real):
+        self.place, self.real = place, real  # place: number of the part; real: fp32
+
+    def __set_name__(self, owner, name):
+        self.name = name
+
+    def __get__(self, g, owner=None):
+        if g is None:
+            return self
+        words, i = g._words, self.place
+        if self.real:
+            words = words.view(torch.float32)
+        if i < 2:
+            t = words.as_strided((g._T, g._k), (g._k, 1), g._at[i])
+        elif i < 4:
+            t = words.as_strided((g._E,), (1,), g._at[i])
+        else:
+            t = words.as_strided((), (), g._at[i])
+        g.__dict__[self.name] = t
+        return t
+
+
+class Gate:
+    """What gate() returns: tensors idx, gates, counts, prob_sum, routed, balance (in this order when it is iterated over).  gate() keeps
+    them in one piece of memory and makes a tensor of a part when it is asked for: six allocations cost a decode step more than the
+    kernel does."""
+    _FIELDS = ("idx", "gates", "counts", "prob_sum", "routed", "balance")
+    idx, gates, counts, prob_sum, routed, balance = (_Part(i, n in ("gates", "prob_sum", "balance")) for i, n in enumerate(_FIELDS))
+
+    def __init__(self, idx, gates, counts, prob_sum, routed, balance):
+        self.__dict__.update(zip(self._FIELDS, (idx, gates, counts, prob_sum, routed, balance)), _words=None)
+
+    def __setattr__(self, name, value):
+        raise AttributeError("the parts of a Gate may be written to, not replaced: make a Gate of the tensors")
+
+    @classmethod
+    def _empty(cls, like, T, k, E):
+        g = object.__new__(cls)
+        n, e = (T * k + 3) // 4 * 4, (E + 3) // 4 * 4
+        g.__dict__.update(_T=T, _k=k, _E=E, _at=(0, n, 2 * n, 2 * n + e, 2 * n + 2 * e, 2 * n + 2 * e + 1),
+                          _words=like.new_empty(2 * n + 2 * e + 2, dtype=torch.int32))
+        return g
+
+    def __iter__(self):
+        return (getattr(self, n) for n in self._FIELDS)
+
+    def _addresses(self, *parts):
+        """Of parts by number."""
+        if self._words is None:
+            return [getattr(self, self._FIELDS[i]).data_ptr() for i in parts]
+        base, at = self._words.data_ptr(), self._at
+        return [base + 4 * at[i] for i in parts]
 
 
 _FLOAT = float_codes()
@@ -197,29 +250,34 @@ def gate(logits, topk, mask=None, normalize=True, comm=None):
                                                        g.balance.data_ptr(), _raw_stream()), "HcclB200MoeBalance")
         return gs if isinstance(logits, (list, tuple)) else gs[0]
     T, E, stride, code = _check_gate(logits, topk, mask)
-    new, i32, f32 = logits.new_empty, torch.int32, torch.float32
     with on_device_of(logits):
-        idx, gates = new((T, topk), dtype=i32), new((T, topk), dtype=f32)
-        counts, prob_sum, routed, balance = new(E, dtype=i32), new(E, dtype=f32), new((), dtype=i32), new((), dtype=f32)
+        g = Gate._empty(logits, T, topk, E)
         n = L.lib().HcclB200MoeGateScratchBytes(T, E)
-        scratch = new(n, dtype=torch.uint8) if n > 0 else None
-        rc = L.fast.gate(logits, code, T, E, stride, topk, int(normalize), mask, idx, gates, counts, prob_sum, routed, balance, scratch, _raw_stream())
+        scratch = logits.new_empty(n, dtype=torch.uint8) if n > 0 else None
+        rc = L.fast.gate(logits, code, T, E, stride, topk, int(normalize), mask, *g._addresses(0, 1, 2, 3, 4, 5), scratch, _raw_stream())
         if rc:
             L.check(rc, "HcclB200MoeGate")
-    return Gate(idx, gates, counts, prob_sum, routed, balance)
+    return g
 
 
 def gate_grad(logits, g, d_gates=None, balance=0.0, mask=None, normalize=True, out=None):
     """Gradient of the logits: `d_gates` (fp32 [tokens, topk] or None) is the gates' gradient, the number `balance` that of the balance
     loss.  logits, mask and normalize are those of the gate() call that returned `g`; counts are constants of the loss.  A slot with
     expert -1 passes nothing on, rows that are not routed get zeros."""
-    if g.idx.dim() != 2:
+    if not isinstance(g, Gate):
+        raise TypeError("g must be what gate() returned for these logits")
+    if g._words is not None:
+        shape, experts, device = (g._T, g._k), (g._E,), g._words.device
+    else:
+        ts = (g.idx, g.counts, g.routed)
+        if g.idx.dim() != 2 or g.routed.numel() != 1 or not all(t.dtype == torch.int32 and t.is_contiguous() and t.device == g.idx.device for t in ts):
+            raise ValueError("g needs contiguous int32 tensors idx [tokens, topk], counts [experts] and routed []")
+        shape, experts, device = tuple(g.idx.shape), tuple(g.counts.shape), g.idx.device
+    T, E, stride, code = _check_gate(logits, shape[1], mask)
+    dev, topk = logits.device, shape[1]
+    if shape[0] != T or experts != (E,) or device != dev:
         raise ValueError("g must be what gate() returned for these logits")
-    T, E, stride, code = _check_gate(logits, g.idx.shape[1], mask)
-    dev, topk = logits.device, g.idx.shape[1]
-    if g.idx.shape[0] != T or g.counts.shape != (E,) or g.idx.device != dev or not g.idx.is_contiguous():
-        raise ValueError("g must be what gate() returned for these logits")
-    if d_gates is not None and not (d_gates.device == dev and d_gates.dtype == torch.float32 and d_gates.shape == g.idx.shape and d_gates.is_contiguous()):
+    if d_gates is not None and not (d_gates.device == dev and d_gates.dtype == torch.float32 and d_gates.shape == shape and d_gates.is_contiguous()):
         raise ValueError("d_gates must be a contiguous fp32 tensor [tokens, topk] on the device of the logits")
     with on_device_of(logits):
         if out is None:
@@ -227,7 +285,8 @@ def gate_grad(logits, g, d_gates=None, balance=0.0, mask=None, normalize=True, o
         else:
             check_out(out, (T, E), logits.dtype, dev)
         L.lib()
-        rc = L.fast.gate_grad(logits, code, T, E, stride, topk, int(normalize), mask, g.idx, d_gates, g.counts, g.routed, balance, out, _raw_stream())
+        idx, counts, routed = g._addresses(0, 2, 4)
+        rc = L.fast.gate_grad(logits, code, T, E, stride, topk, int(normalize), mask, idx, d_gates, counts, routed, balance, out, _raw_stream())
         if rc:
             L.check(rc, "HcclB200MoeGateGrad")
     return out

@@ -162,6 +162,32 @@ def test_gradient_against_differences():
         assert abs(float(diff - got)) <= 1e-6 + REL * float((d.abs().sum() + 24) * step.abs().max())
 
 
+def test_parts_of_a_gate():
+    """Parts share memory with what later calls read; a Gate of other tensors (experts dropped by hand) is taken as well."""
+    l = torch.randn(30, 16, device="cuda")
+    g = moe.gate(l, 3)
+    d = torch.randn(30, 3, device="cuda")
+    assert [t.dtype for t in g] == [torch.int32, torch.float32, torch.int32, torch.float32, torch.int32, torch.float32]
+    assert [tuple(t.shape) for t in g] == [(30, 3), (30, 3), (16,), (16,), (), ()] and all(t.is_contiguous() for t in g) and g.idx is g.idx
+    want = moe.gate_grad(l, moe.Gate(*[t.clone() for t in g]), d, 0.3)
+    assert torch.equal(moe.gate_grad(l, g, d, 0.3), want)
+    with pytest.raises(AttributeError):
+        g.idx = g.idx.clone()
+    g.idx[4, 1] = -1                                                  # dropped: it passes nothing on, the other gates share its part
+    dropped = moe.gate_grad(l, g, d)
+    p = torch.softmax(l[4].double(), 0)
+    at = g.idx[4, [0, 2]].long()
+    q = p[at] / p[at].sum()
+    part = q * (d[4, [0, 2]].double() - (q * d[4, [0, 2]].double()).sum())
+    row = torch.zeros(16, device="cuda", dtype=torch.float64).scatter_add(0, at, part)
+    assert bool(((dropped[4].double() - row).abs() <= 8 * REL * d[4].abs().max()).all())
+    for bad in (g.idx[:, :2], g.idx.float(), g.idx[:7]):
+        with pytest.raises(ValueError):
+            moe.gate_grad(l, moe.Gate(bad, *list(g)[1:]))
+    with pytest.raises(TypeError):
+        moe.gate_grad(l, tuple(g))
+
+
 def test_same_bits_again_and_captured():
     l = torch.randn(5000, 256, device="cuda")
     a, b = moe.gate(l, 8), moe.gate(l, 8)
