@@ -463,10 +463,12 @@ struct RowArgs {
     const uint8_t *x, *w;
     uint8_t *xc;
     int64_t tokens, first, vocab, whole, ignore, ld, width, x_stride, w_stride;  // x_stride, w_stride: in bytes
-    int wide, halves, cols, n_tiles, shards, xvec;
+    int wide, halves, cols, shards, xvec, grad;
 };
 
 __device__ __forceinline__ bool counts(const RowArgs &a, int64_t id) { return id != a.ignore && id >= 0 && id < a.whole; }
+
+__device__ __forceinline__ float weight(const RowArgs &a, int64_t t, int64_t id) { return !counts(a, id) ? 0.f : a.weights ? a.weights[t] : 1.f; }
 
 __device__ __forceinline__ float warp_max(float x)
 {
@@ -555,7 +557,7 @@ __global__ void __launch_bounds__(kRowThreads) vocab_loss_rows(const __grid_cons
     }
     a.lse[t] = all + log_z;
     a.target[t] = target;
-    if (a.losses) a.losses[t] = counts(a, id) ? (all - target) + log_z : 0.f;
+    if (a.losses) a.losses[t] = counts(a, id) && !(a.grad && weight(a, t, id) == 0.f) ? (all - target) + log_z : 0.f;
 }
 
 // Joint lse and loss from the shards'.
@@ -588,11 +590,8 @@ __global__ void __launch_bounds__(kSumThreads) vocab_loss_reduce(const __grid_co
     float sum = 0.f;
 #pragma unroll 4
     for (int64_t t = threadIdx.x; t < a.tokens; t += kSumThreads) {
-        float v = 0.f;
-        if (counts(a, target_of(a.y, a.wide, t))) {
-            v = a.weights ? a.weights[t] : 1.f;
-            if (a.losses_in) v = v == 0.f ? 0.f : v * a.losses_in[t];
-        }
+        float v = weight(a, t, target_of(a.y, a.wide, t));
+        if (a.losses_in) v = v == 0.f ? 0.f : v * a.losses_in[t];
         sum += v;
     }
     sum = warp_sum(sum);
@@ -606,7 +605,7 @@ __global__ void __launch_bounds__(kSumThreads) vocab_loss_reduce(const __grid_co
 }
 
 constexpr int kCopyThreads = 256;
-// Rows of x to rows of xc that start on 128-byte boundaries; zeros for tokens that do not count.
+// Rows of x to rows of xc that start on 128-byte boundaries; with gradients zeros for tokens that have no part in them.
 __global__ void __launch_bounds__(kCopyThreads) vocab_loss_x(const __grid_constant__ RowArgs a)
 {
     pdl_trigger();
@@ -614,7 +613,7 @@ __global__ void __launch_bounds__(kCopyThreads) vocab_loss_x(const __grid_consta
     const int v = (int)(i - t * a.xvec);
     pdl_wait();
     if (t >= a.tokens) return;
-    const bool on = counts(a, target_of(a.y, a.wide, t)) && (!a.weights || a.weights[t] != 0.f);
+    const bool on = !a.grad || weight(a, t, target_of(a.y, a.wide, t)) != 0.f;
     ((uint4 *)a.xc)[t * (a.ld / 8) + v] = on ? ((const uint4 *)(a.x + t * a.x_stride))[v] : make_uint4(0, 0, 0, 0);
 }
 
@@ -626,7 +625,7 @@ __global__ void __launch_bounds__(kDThreads) vocab_loss_d(const __grid_constant_
     pdl_wait();
     const int64_t t = blockIdx.y;
     const int64_t id = target_of(a.y, a.wide, t);
-    const float q = !counts(a, id) ? 0.f : a.weights ? a.weights[t] : 1.f;
+    const float q = weight(a, t, id);
     uint4 *row = (uint4 *)(a.e + t * a.ld * 2);
     const uint32_t vecs = (uint32_t)(a.width / 8), cols = (uint32_t)a.cols, mid = (cols / 16 + 1) / 2 * 16;
     const float lse = a.lse[t];
@@ -874,7 +873,7 @@ HcclResult vocab_loss_scores(const VocabLossCall &c, bool grad, float *lse, floa
     P.y = c.targets; P.wide_y = c.wide; P.first = c.first; P.ignore = c.ignore;
     if (l.copy) {
         RowArgs a = row_args(c);
-        a.x = (const uint8_t *)c.x; a.x_stride = c.x_stride * 2; a.xc = s + l.xc; a.ld = l.xld; a.xvec = c.hidden / 8;
+        a.x = (const uint8_t *)c.x; a.x_stride = c.x_stride * 2; a.xc = s + l.xc; a.ld = l.xld; a.xvec = c.hidden / 8; a.grad = grad;
         CHK_RET(launch_pdl((const void *)vocab_loss_x, dim3((unsigned)((c.tokens * a.xvec + kCopyThreads - 1) / kCopyThreads)), kCopyThreads, 0, &a, stream,
                            "vocabulary loss (x)"));
     }
@@ -884,7 +883,7 @@ HcclResult vocab_loss_scores(const VocabLossCall &c, bool grad, float *lse, floa
     RowArgs a = row_args(c);
     a.stats = P.stats; a.halves = 2 * l.n_tiles;
     a.lse = lse; a.target = target; a.losses = losses;
-    a.x = (const uint8_t *)c.x; a.w = (const uint8_t *)c.w; a.x_stride = c.x_stride * 2; a.w_stride = c.w_stride * 2; a.xvec = c.hidden / 8;
+    a.x = (const uint8_t *)c.x; a.w = (const uint8_t *)c.w; a.x_stride = c.x_stride * 2; a.w_stride = c.w_stride * 2; a.xvec = c.hidden / 8; a.grad = grad;
     return launch_pdl((const void *)vocab_loss_rows, dim3((unsigned)c.tokens), kRowThreads, 0, &a, stream, "vocabulary loss (rows)");
 }
 
@@ -916,7 +915,7 @@ HcclResult vocab_loss_grad(const VocabLossCall &c, const float *lse, const float
     CHK_RET(layout_of(c.tokens, c.vocab, c.hidden, true, &l));
     uint8_t *s = (uint8_t *)scratch;
     RowArgs a = row_args(c);
-    a.stats = (const float2 *)(s + l.stats); a.halves = 2 * l.n_tiles; a.cols = l.cols; a.n_tiles = l.n_tiles;
+    a.stats = (const float2 *)(s + l.stats); a.halves = 2 * l.n_tiles; a.cols = l.cols;
     a.e = s; a.ld = l.ld; a.width = l.width; a.lse = (float *)lse; a.target = (float *)target;
     // enough CTAs to fill the GPU a few times, none without work (129 tokens x 160000 by one CTA each: 50 us)
     const int64_t parts = std::min<int64_t>((l.width / 8 + kDVecs - 1) / kDVecs, std::max<int64_t>(1, 4096 / c.tokens));

@@ -162,7 +162,7 @@ extern int64_t HcclB200VocabLossChunk(int64_t vocab, int32_t withGrad);
 extern int64_t HcclB200VocabLossScratchBytes(int64_t tokens, int64_t vocab, int32_t hidden, int32_t withGrad);
 /* lse [tokens] and target [tokens] (the target's logit, -inf where another shard has it) against this shard; losses [tokens] (0 for
  * tokens that do not count) where the shard is the whole vocabulary, else NULL.  withGrad: scratch then holds what
- * HcclB200VocabLossGrad needs. */
+ * HcclB200VocabLossGrad needs, and tokens of weight 0 have a loss of 0 (their rows of x are not looked at). */
 extern HcclResult HcclB200VocabLossScores(const HcclB200VocabLoss *p, int32_t withGrad, float *lse, float *target, float *losses, void *scratch,
                                           aclrtStream stream);
 /* Joint lse and losses from the shards' parts [shards][2][tokens] = (lse, target). */

@@ -210,7 +210,7 @@ def linear_cross_entropy(x, w, targets, weights=None, reduction="mean", ignore_i
     """Softmax cross entropy of the logits x [tokens, hidden] @ w [vocab, hidden].T (bf16, fp32 sums) against `targets` (int32 or int64).
     Tokens whose target is ignore_index or no id of the vocabulary do not count.  `weights`: fp32 [tokens].  reduction: "none" gives
     the unweighted losses [tokens] (0 where a token does not count), "sum" their weighted sum, "mean" that divided by the sum of the
-    weights that count (0 where there is none).  The logits are not stored: memory beyond the arguments is bounded by 128 MB."""
+    weights that count (0 where there is none).  The logits are not stored: beyond the arguments it takes about 130 MB at most (for 256 tokens at least)."""
     _check_loss(x, w, targets, weights, reduction)
     with on_device_of(x):
         return _run_loss([_Shard(x, w, targets, weights, 0, w.shape[0], ignore_index)], None, reduction)[0]
@@ -219,8 +219,8 @@ def linear_cross_entropy(x, w, targets, weights=None, reduction="mean", ignore_i
 def linear_cross_entropy_grad(x, w, targets, weights=None, reduction="mean", ignore_index=-100, scale=1.0, dw=None):
     """(loss, dx, dw): the loss as linear_cross_entropy() gives it ("mean" or "sum") and the gradients of scale * loss.  dx and dw are bf16;
     given an fp32 tensor `dw` [vocab, hidden], the weight's gradient is added to it (several batches, or a weight that the embedding
-    shares) and it is returned.  Beyond the results it takes 2 GiB at most, for the exponentials of a chunk of tokens, and an fp32 sum of
-    dw where the tokens are more than one chunk (16 thousand million logits)."""
+    shares) and it is returned.  Beyond the results it takes about 2 GiB at most, for the exponentials of a chunk of tokens (of 256 tokens at
+    least), and an fp32 sum of dw where the tokens are more than one chunk (a thousand million logits)."""
     _check_loss(x, w, targets, weights, reduction)
     if reduction == "none":
         raise ValueError("gradients need a sum or mean over the tokens (weights scale each token)")

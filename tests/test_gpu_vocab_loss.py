@@ -186,6 +186,19 @@ def test_tokens_that_do_not_count():
     e.check(vocab.linear_cross_entropy_grad(x, w, y.clamp(0, 499), ignore_index=0))
 
 
+@pytest.mark.parametrize("T,hidden", [(7, 72), (300, 1000), (300, 128)])
+def test_tokens_without_weight_have_losses(T, hidden):
+    """reduction "none" gives every token's own loss; weights only matter to the sums."""
+    x, w, y = problem(T, 500, hidden)
+    weights = torch.rand(T, device="cuda")
+    weights[::2] = 0
+    got = vocab.linear_cross_entropy(x, w, y, weights, reduction="none")
+    assert torch.equal(got, vocab.linear_cross_entropy(x, w, y, reduction="none"))
+    e = Exact(x, w, y, weights)
+    e.check_losses(got)
+    assert abs(float(vocab.linear_cross_entropy(x, w, y, weights)) - e.loss) <= e.loss_err
+
+
 def test_sure_and_wild_guesses():
     """Probabilities next to one, logits of thousands, and rows of equal logits."""
     x, w, y = problem(200, 900, 64, lean=0.0)
@@ -294,6 +307,33 @@ def test_captured_and_replayed():
         graph.replay()
         want = vocab.linear_cross_entropy_grad(x, w, y)
         assert all(torch.equal(a, b) for a, b in zip(out, want)) and torch.equal(losses, vocab.linear_cross_entropy(x, w, y, reduction="none"))
+
+
+@pytest.mark.parametrize("call", ["vocab.linear_cross_entropy_grad(x, w, y)", "vocab.linear_cross_entropy(x[:7], w, y[:7])", "vocab.embedding_grad(y, x, 5000)",
+                                  "vocab.embedding_grad(y.repeat(40), x.repeat(40, 1), 5000)", "vocab.embedding(y, w)", "moe.gate_grad(x, moe.gate(x, 3), None, 1.0)"])
+def test_first_call_of_a_program_is_captured(call):
+    """Nothing has been loaded or asked for before the capture."""
+    import os
+    import subprocess
+    import sys
+    prog = """
+import torch
+from cann_hccl_b200.parallel import moe, vocab
+torch.manual_seed(1)
+x, w, y = torch.randn(300, 72, device="cuda").bfloat16(), torch.randn(5000, 72, device="cuda").bfloat16(), torch.randint(0, 5000, (300,), device="cuda")
+side = torch.cuda.Stream()
+graph = torch.cuda.CUDAGraph()
+torch.cuda.synchronize()
+with torch.cuda.graph(graph, stream=side):
+    got = %s
+graph.replay()
+torch.cuda.synchronize()
+want = %s
+for a, b in zip(*[t if isinstance(t, tuple) else (t,) for t in (got, want)]):
+    assert torch.equal(a, b)
+""" % (call, call)
+    r = subprocess.run([sys.executable, "-c", prog], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr
 
 
 def test_two_streams_at_once():
