@@ -7,9 +7,9 @@
 //
 // A warp takes a token, a lane the experts lane, lane + 32, ... : one pass over the logits, as order-preserving integer keys.  The k-th
 // largest of the lanes' maxima is a bound that at least k experts reach and few more do (about ten for top 8 of 256): these go to a
-// list in shared memory, a lane takes one of them and counts the others before it.  More than 32 of them (many equal logits): k rounds
-// of a maximum over the lanes.  (65536 tokens x 256, top 8: rounds in which every lane searches its registers 167 us, rounds that the
-// warp searches together 63 us.)  Sums of probabilities stay in registers, counts in shared memory; each CTA leaves one partial row,
+// list in shared memory, a lane takes one of them and counts the others before it.  More than 32 of them (many equal logits), or NaN: k
+// rounds of a maximum over the lanes.  (65536 tokens x 256, top 8: rounds in which every lane searches its registers 167 us, rounds that the
+// warp searches together 63 us, this 40 us.)  Sums of probabilities stay in registers, counts in shared memory; each CTA leaves one partial row,
 // a second launch adds them in a fixed order (no floating-point atomics).  Up to kOneCta tokens one CTA does it all.
 // Bound: launches and latency for decode batches, instruction issue for large ones.
 #include <cuda_bf16.h>
@@ -53,6 +53,14 @@ __device__ __forceinline__ float exp_of(float x)
     return y;
 }
 
+// Maximum that is NaN where one of the two is.
+__device__ __forceinline__ float max_nan(float x, float y)
+{
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(x), "f"(y));
+    return m;
+}
+
 __device__ __forceinline__ float warp_sum(float x)
 {
 #pragma unroll
@@ -91,6 +99,15 @@ __device__ __forceinline__ float balance_of(float sum, int n, int experts, int t
 template <int V> constexpr bool kInRegs = V <= 32;
 template <int V> constexpr int kGateMost = V <= 32 ? 512 : 128;      // threads of a CTA
 template <int V> constexpr int kGateCtas = V <= 8 ? 2 : 1;           // CTAs of that size on an SM
+template <class T, int V> __device__ __forceinline__ void load_row(const GateArgs &a, int64_t t, int lane, float (&x)[V])
+{
+    const T *row = (const T *)a.logits + t * a.stride;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int e = j * 32 + lane;
+        x[j] = e < a.experts ? ld_f(row + e) : -INFINITY;
+    }
+}
 // Dynamic shared memory: [warps][32 V] keys, [warps][experts] sums, [experts] counts.
 template <class T, int V>
 __global__ void __launch_bounds__(kGateMost<V>, kGateCtas<V>) moe_gate_kernel(const __grid_constant__ GateArgs a)
@@ -98,7 +115,8 @@ __global__ void __launch_bounds__(kGateMost<V>, kGateCtas<V>) moe_gate_kernel(co
     extern __shared__ uint32_t sh[];
     __shared__ int s_n;
     __shared__ float s_b[kOneThreads / 32];
-    __shared__ uint64_t s_list[kGateMost<V> / 32][36];
+    __shared__ alignas(16) uint2 s_list[kGateMost<V> / 32][36];
+    __shared__ alignas(16) uint32_t s_head[kGateMost<V> / 32][32];
     const int E = a.experts, k = a.topk, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5;
     constexpr int S = V * 32;  // keys of a row: zeros behind the experts
     uint32_t *key = sh + warp * S;
@@ -115,36 +133,34 @@ __global__ void __launch_bounds__(kGateMost<V>, kGateCtas<V>) moe_gate_kernel(co
     int mine = 0;  // routed tokens
     float sums[kInRegs<V> ? V : 1] = {};
     for (int64_t t = (int64_t)blockIdx.x * W + warp; t < a.tokens; t += (int64_t)gridDim.x * W) {
-        const T *row = (const T *)a.logits + t * a.stride;
         const bool on = !a.mask || a.mask[t];
-        float x[V];
-        uint32_t best = 0;  // largest key of this lane
+        float x[V], high = -INFINITY;  // experts outside count as -inf
+        load_row<T, V>(a, t, lane, x);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int e = j * 32 + lane;
-            x[j] = e < E ? ld_f(row + e) : -INFINITY;
-        }
-#pragma unroll
-        for (int j = 0; j < V; ++j) best = max(best, key_of(x[j]));  // experts outside count as -inf
+        for (int j = 0; j < V; ++j) high = max_nan(high, x[j]);
+        uint32_t best = key_of(high);  // largest key of this lane
         const uint32_t top = __reduce_max_sync(kAll, best);
         const bool routed = on && top > kInfKey;
         const float m = value_of(top);
         int sel = -1, slot = lane;  // this lane's choice, if it has one, and its place
         uint32_t sel_key = 0;
         if (routed) {
-            // the k-th largest of the lanes' maxima (sorted by a bitonic network)
-            uint32_t bound = best;
+            // the k-th largest of the lanes' maxima: the least one that fewer than k are above
+            uint32_t *heads = s_head[warp];
+            __syncwarp();                       // list and maxima of the token before are not read any more
+            heads[lane] = best;
+            __syncwarp();
+            int above = 0;
 #pragma unroll
-            for (int size = 2; size <= 32; size *= 2)
-#pragma unroll
-                for (int step = size / 2; step; step /= 2) {
-                    const uint32_t other = __shfl_xor_sync(kAll, bound, step);
-                    bound = ((lane & size) == 0) == ((lane & step) == 0) ? max(bound, other) : min(bound, other);
-                }
-            bound = max(__shfl_sync(kAll, bound, k - 1), kInfKey + 1);
+            for (int i = 0; i < 8; ++i) {
+                const uint4 h = ((const uint4 *)heads)[i];
+                above += (h.x > best) + (h.y > best) + (h.z > best) + (h.w > best);
+            }
+            // as a value: comparisons with it see -0 and 0 as one, and no NaN is there where it is used
+            const float least = value_of(max(__reduce_min_sync(kAll, above < k ? best : kAll), kInfKey + 1));
             int own = 0;
 #pragma unroll
-            for (int j = 0; j < V; ++j) own += key_of(x[j]) >= bound;
+            for (int j = 0; j < V; ++j) own += x[j] >= least;
             int at = own;
 #pragma unroll
             for (int o = 1; o < 32; o *= 2) {
@@ -153,15 +169,19 @@ __global__ void __launch_bounds__(kGateMost<V>, kGateCtas<V>) moe_gate_kernel(co
             }
             const int c = __shfl_sync(kAll, at, 31);
             at -= own;
-            if (c <= 32) {
-                uint64_t *list = s_list[warp];  // key, and the expert so that lower ones are larger
-                __syncwarp();                   // the list of the token before is not read any more
-                if (lane < 4) list[c + lane] = 0;
+            if (c <= 32 && top != kAll) {
+                uint2 *raw = s_list[warp];      // logit and expert, then key and the expert so that lower ones are larger
+                raw += at;
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const uint32_t q = key_of(x[j]);
-                    if (q >= bound) list[at++] = (uint64_t)q << 32 | (uint32_t)~(j * 32 + lane);
+                for (int j = 0; j < V; ++j)
+                    if (x[j] >= least) *raw++ = make_uint2(__float_as_uint(x[j]), (uint32_t)(j * 32 + lane));
+                __syncwarp();
+                uint64_t *list = (uint64_t *)s_list[warp];
+                if (lane < c) {
+                    const uint2 r = s_list[warp][lane];
+                    list[lane] = (uint64_t)key_of(__uint_as_float(r.x)) << 32 | (uint32_t)~r.y;
                 }
+                if (lane < 4) list[c + lane] = 0;
                 __syncwarp();
                 if (lane < c) {
                     const uint64_t mine = list[lane];
@@ -338,21 +358,12 @@ __global__ void __launch_bounds__(kGateMost<V>, kGateCtas<V>) moe_gate_grad_kern
         if (sel >= E) sel = -1;
         const float dg = a.d_gates && sel >= 0 ? a.d_gates[t * k + lane] : 0.f;
         float x[V], m = -INFINITY;
-        bool nan = false;
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int e = j * 32 + lane;
-            x[j] = e < E ? ld_f(row + e) : -INFINITY;
-        }
+        load_row<T, V>(a, t, lane, x);
         const float sel_x = sel >= 0 ? ld_f(row + sel) : -INFINITY;
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            m = fmaxf(m, x[j]);
-            nan = nan || x[j] != x[j];
-        }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kAll, m, o));
-        const bool on = (!a.mask || a.mask[t]) && (m > -INFINITY || __any_sync(kAll, nan));
+        for (int j = 0; j < V; ++j) m = max_nan(m, x[j]);
+        m = value_of(__reduce_max_sync(kAll, key_of(m)));  // NaN where one is
+        const bool on = (!a.mask || a.mask[t]) && !(m == -INFINITY);
         if (!on) {
 #pragma unroll
             for (int j = 0; j < V; ++j)
