@@ -119,6 +119,16 @@ def test_masked_experts_and_tokens():
     assert int(g.routed) == 0 and float(g.balance) == 0 and bool((g.gates == 0).all()) and bool((g.counts == 0).all())
 
 
+def test_more_equal_logits_than_a_list_holds():
+    """Rows whose k-th largest logit is shared by many experts, among rows that have no such."""
+    l = torch.randn(300, 200, device="cuda")
+    l[::3] = (l[::3] > 0.5).float()                                   # about sixty experts share the largest
+    l[1::7, 20:] = l[1::7, 20:21]
+    for dtype in TYPES:
+        check(l.to(dtype), 8)
+        check((l * 3).round().to(dtype), 5)
+
+
 def test_infinities_and_nan_stay_in_their_rows():
     l = torch.randn(64, 40, device="cuda")
     l[3, 7], l[9, 0], l[9, 30] = math.nan, math.inf, math.inf
@@ -136,6 +146,8 @@ def test_infinities_and_nan_stay_in_their_rows():
 
 def test_strided_rows_and_no_tokens():
     base = torch.randn(50, 200, device="cuda")
+    for l in (base[:, 4:132], base[:, 5:133], base[:, :100], base.to(torch.bfloat16)[:, 4:104], base.to(torch.float16)[:, 3:103]):
+        assert torch.equal(check(l, 7).idx, moe.gate(l.contiguous(), 7).idx)
     assert torch.equal(check(base[:, 3:67], 6).idx, moe.gate(base[:, 3:67].contiguous(), 6).idx)
     g = moe.gate(base[:0], 6)
     assert g.idx.shape == (0, 6) and float(g.balance) == 0 and int(g.routed) == 0 and bool((g.counts == 0).all())
