@@ -9,9 +9,10 @@
 // largest of the lanes' maxima is a bound that at least k experts reach and few more do (about ten for top 8 of 256): these go to a
 // list in shared memory, a lane takes one of them and counts the others before it.  More than 32 of them (many equal logits), or NaN: k
 // rounds of a maximum over the lanes.  (65536 tokens x 256, top 8: rounds in which every lane searches its registers 167 us, rounds that the
-// warp searches together 63 us, this 40 us.)  Sums of probabilities stay in registers, counts in shared memory; each CTA leaves one partial row,
+// warp searches together 63 us, this 43 us.)  Sums of probabilities stay in registers, counts in shared memory; each CTA leaves one partial row,
 // a second launch adds them in a fixed order (no floating-point atomics).  Up to kOneCta tokens one CTA does it all.
-// Bound: launches and latency for decode batches, instruction issue for large ones.
+// Bound: launches and latency for decode batches (16 tokens x 64: 4.5 us), instruction issue for large ones (0.78 of a warp instruction
+// per cycle; the gradient 35 us, 4.0 TB/s).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
