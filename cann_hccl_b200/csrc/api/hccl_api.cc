@@ -798,7 +798,7 @@ HcclResult HcclB200Embedding(const void *ids, HcclDataType idType, int64_t token
 }
 int64_t HcclB200EmbeddingGradScratchBytes(int64_t tokens, int64_t vocab, int32_t hidden)
 {
-    return tokens < 0 || tokens > INT32_MAX || vocab < 1 || vocab >= INT32_MAX || hidden < 1 ? -1 : embed_grad_scratch_bytes(tokens, vocab, hidden);
+    return tokens < 0 || tokens > kEmbedGradMost || vocab < 1 || vocab >= INT32_MAX || hidden < 1 ? -1 : embed_grad_scratch_bytes(tokens, vocab, hidden);
 }
 HcclResult HcclB200EmbeddingGrad(const void *ids, HcclDataType idType, int64_t tokens, const void *grad, int64_t gradStride, int64_t vocab, int64_t firstId,
                                  int32_t hidden, HcclDataType dataType, float scale, void *out, HcclDataType outType, int32_t accumulate, void *scratch,
@@ -807,6 +807,7 @@ HcclResult HcclB200EmbeddingGrad(const void *ids, HcclDataType idType, int64_t t
     EmbedTable t;
     EmbedIds i;
     CHK_RET(check_embed(ids, idType, tokens, grad, gradStride, vocab, firstId, hidden, dataType, out, "HcclB200EmbeddingGrad", &t, &i));
+    CHK_RET_LOG(tokens > kEmbedGradMost, HCCL_E_PARA, "HcclB200EmbeddingGrad: %lld tokens, at most %lld (add several calls up)", (long long)tokens, (long long)kEmbedGradMost);
     CHK_RET_LOG(outType != (accumulate ? HCCL_DATA_TYPE_FP32 : dataType), HCCL_E_NOT_SUPPORT, "HcclB200EmbeddingGrad: out has the type of grad, or FP32 where it is added to");
     CHK_RET_LOG(!scratch, HCCL_E_PTR, "[EI0003] HcclB200EmbeddingGrad: null pointer");
     CHK_RET(check_aligned({scratch}, 16, "HcclB200EmbeddingGrad"));

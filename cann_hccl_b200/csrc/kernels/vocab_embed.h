@@ -4,6 +4,9 @@
 
 namespace hcclb {
 
+// Tokens of one gradient: every tile of the sort reads the histograms of all of them.
+constexpr int64_t kEmbedGradMost = 1 << 24;
+
 // Rows of a vocabulary (or of one rank's shard of it, which holds the ids first .. first + vocab - 1).
 struct EmbedTable {
     int64_t vocab, first;

@@ -124,7 +124,7 @@ extern HcclResult HcclB200Embedding(const void *ids, HcclDataType idType, int64_
                                     int64_t firstId, int32_t hidden, HcclDataType dataType, float scale, void *out, aclrtStream stream);
 /* Its gradient, out [vocab, hidden] = scale * sum over the tokens of a row of grad [tokens, hidden]: summed in fp32 in the order of
  * the tokens (the same bits every time).  outType dataType: every row of out is written, rows without a token with zeros.
- * outType FP32 with accumulate: the sums are added to out, other rows are left alone. */
+ * outType FP32 with accumulate: the sums are added to out, other rows are left alone.  At most 2^24 tokens. */
 extern int64_t HcclB200EmbeddingGradScratchBytes(int64_t tokens, int64_t vocab, int32_t hidden);
 extern HcclResult HcclB200EmbeddingGrad(const void *ids, HcclDataType idType, int64_t tokens, const void *grad, int64_t gradStride, int64_t vocab,
                                         int64_t firstId, int32_t hidden, HcclDataType dataType, float scale, void *out, HcclDataType outType,

@@ -8,7 +8,8 @@
     vocab_parallel_cross_entropy(comm, x, w, targets) and vocab_parallel_cross_entropy_grad: w sharded over the ranks
 
 Rows of a shard are ids first_id .. first_id + rows - 1; ids outside it (other ranks' rows, padding ids below zero) give zeros and have
-no gradient.  On an all-local communicator w (and what is per rank) is a list with one tensor per virtual rank.
+no gradient.  On an all-local communicator w (and what is per rank) is a list with one tensor per virtual rank.  Gradients are calls of
+their own, as everywhere in this package: results carry no automatic differentiation.
 """
 import ctypes as C
 
@@ -30,7 +31,7 @@ def _check_ids(ids, device):
 
 def _check_rows(t, name):
     """[rows, hidden] whose rows lie in one piece each; returns rows, hidden and the elements between rows."""
-    if not (torch.is_tensor(t) and t.is_cuda and t.dim() == 2 and t.shape[1] > 0):
+    if not (torch.is_tensor(t) and t.is_cuda and t.dim() == 2 and 0 < t.shape[1] < 1 << 31):
         raise ValueError("%s must be a CUDA tensor [rows, hidden]" % name)
     if t.dtype not in _FLOAT:
         raise TypeError("%s must be fp32, fp16 or bf16, got %s" % (name, t.dtype))

@@ -36,6 +36,7 @@ def test_embedding_gradient():
     assert lib.HcclB200EmbeddingGradScratchBytes(-1, 10, 8) == -1 and lib.HcclB200EmbeddingGradScratchBytes(10, 0, 8) == -1
     assert lib.HcclB200EmbeddingGradScratchBytes(10, 10, 0) == -1 and lib.HcclB200EmbeddingGradScratchBytes(0, 10, 8) > 0
     assert embed(False, tokens=0, ids=None, out=None) == L.SUCCESS
+    assert embed(True, tokens=(1 << 24) + 1) == L.E_PARA and lib.HcclB200EmbeddingGradScratchBytes((1 << 24) + 1, 10, 8) == -1
 
 
 def gate(grad=False, logits=AT, dtype=L.FP32, tokens=4, experts=8, stride=8, topk=2, idx=AT, gates=AT, counts=AT, prob=AT, routed=AT, balance=AT, scratch=AT,
