@@ -419,7 +419,7 @@ template <class T, int V> HcclResult run_gate(GateArgs &a, bool grad, void *stre
     const int W = g.threads / 32;
     const size_t smem = grad ? (size_t)(W + 1) * a.experts * 4 : (size_t)W * V * 128 + (size_t)(W + 1) * a.experts * 4;
     const void *fn = grad ? (const void *)moe_gate_grad_kernel<T, V> : (const void *)moe_gate_kernel<T, V>;
-    if (smem > 48 * 1024) {
+    if (smem > 32 * 1024) {  // with what the kernel has of its own, more than 48 KB needs leave
         const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         CHK_RET_LOG(e != cudaSuccess, HCCL_E_RUNTIME, "router set-up failed: %s", cudaGetErrorString(e));
     }

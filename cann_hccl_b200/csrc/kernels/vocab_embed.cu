@@ -135,13 +135,16 @@ __global__ void __launch_bounds__(kLookupThreads) embed_lookup_kernel(const __gr
 // number of tokens that belong before it, counted by comparing with all of them.  More: radix sort from the least significant digit;
 // a warp takes consecutive stretches of 32 pairs, __match_any_sync gives the lanes of one digit, the warp's counters in shared
 // memory the earlier stretches, so equal digits keep their order.
-// (1531 tokens: one CTA of a radix sort 8.1 us, one cluster 13 us, both exchanging through shared memory; 32768 tokens: a cluster 25
-// us, the tiles below 20 us.)
-constexpr int kCountMost = 8192, kCountTokens = 32, kCountThreads = 256;  // tokens that are sorted by counting, tokens of a CTA
+// (1531 tokens by counting 6.0 us; one CTA of a radix sort 8.1 us, one cluster 13 us, both exchanging through shared memory; 32768
+// tokens: a cluster 25 us, the tiles below 20 us.  The whole gradient of rows of 64: 4096 tokens by counting 22 us, 8192 47 us, by
+// tiles 29 us.)
+constexpr int kCountMost = 4096, kCountTokens = 32, kCountThreads = 256;  // tokens that are sorted by counting, tokens of a CTA
 constexpr int kWindow = 1 << 18;                                          // rows whose bits a CTA makes
 constexpr int kDigitBits = 9, kBins = 1 << kDigitBits;
 constexpr int kSortItems = 8;
-constexpr int kTileThreads = 256, kTile = kTileThreads * kSortItems;
+// CTAs of the radix sort: small ones for parallelism, large ones so that the histograms that each of them reads stay few
+constexpr int kSmallTile = 256, kLargeTile = 1024;
+constexpr int64_t kSmallMost = 256 << 10;  // tokens
 
 struct SortArgs {
     const void *ids;                 // first pass
@@ -156,13 +159,12 @@ struct SortArgs {
 };
 
 // Ranks of a warp's pairs within (warp, digit); counts[warp][bin] end up holding the warp's pairs of each digit.
-__device__ __forceinline__ void warp_ranks(const uint32_t (&key)[kSortItems], int items, int shift, uint32_t mask, int32_t *counts, int (&rank)[kSortItems])
+__device__ __forceinline__ void warp_ranks(const uint32_t (&key)[kSortItems], int shift, uint32_t mask, int32_t *counts, int (&rank)[kSortItems])
 {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int32_t *mine = counts + warp * kBins;
 #pragma unroll
     for (int i = 0; i < kSortItems; ++i) {
-        if (i >= items) break;
         const uint32_t d = (key[i] >> shift) & mask;
         const uint32_t peers = __match_any_sync(0xffffffffu, d);
         const int before = mine[d], below = __popc(peers & ((1u << lane) - 1));
@@ -209,7 +211,10 @@ template <int N> __device__ __forceinline__ void bins_prefix(int (&t)[N], int32_
 
 __device__ __forceinline__ void mark_row(const SortArgs &a, uint32_t row)
 {
-    if (a.has && row < (uint32_t)a.vocab) atomicOr(a.has + (row >> 5), 1u << (row & 31));
+    if (!a.has || row >= (uint32_t)a.vocab) return;
+    uint32_t *word = a.has + (row >> 5);
+    const uint32_t bit = 1u << (row & 31);
+    if (!(__ldcg(word) & bit)) atomicOr(word, bit);  // most tokens find their bit set
 }
 
 __device__ __forceinline__ uint32_t key_at(const SortArgs &a, int64_t t)
@@ -262,9 +267,10 @@ __global__ void __launch_bounds__(kCountThreads) embed_sort_count_kernel(const _
     a.out[rank] = make_uint2(mine, (uint32_t)t);
 }
 
+template <int THREADS>
 __device__ __forceinline__ void load_tile(const SortArgs &a, int64_t tile, uint32_t (&key)[kSortItems], uint32_t (&pos)[kSortItems])
 {
-    const int64_t t0 = tile * kTile + (threadIdx.x >> 5) * (32 * kSortItems) + (threadIdx.x & 31);
+    const int64_t t0 = tile * (THREADS * kSortItems) + (threadIdx.x >> 5) * (32 * kSortItems) + (threadIdx.x & 31);
 #pragma unroll
     for (int i = 0; i < kSortItems; ++i) {
         const int64_t t = t0 + i * 32;
@@ -282,58 +288,67 @@ __device__ __forceinline__ void load_tile(const SortArgs &a, int64_t tile, uint3
     }
 }
 
-__global__ void __launch_bounds__(kTileThreads) embed_sort_hist_kernel(const __grid_constant__ SortArgs a)
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) embed_sort_hist_kernel(const __grid_constant__ SortArgs a)
 {
     __shared__ int32_t bins[kBins];
-    for (int i = threadIdx.x; i < kBins; i += kTileThreads) bins[i] = 0;
+    for (int i = threadIdx.x; i < kBins; i += THREADS) bins[i] = 0;
     __syncthreads();
     pdl_trigger();
     pdl_wait();
     if (a.has && !a.in)  // the first pass clears the bits, the last one sets them
-        for (int64_t i = (int64_t)blockIdx.x * kTileThreads + threadIdx.x; i < (a.vocab + 31) / 32; i += (int64_t)gridDim.x * kTileThreads) a.has[i] = 0;
+        for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < (a.vocab + 31) / 32; i += (int64_t)gridDim.x * THREADS) a.has[i] = 0;
     uint32_t key[kSortItems], pos[kSortItems];
-    load_tile(a, blockIdx.x, key, pos);
-    const int64_t t0 = (int64_t)blockIdx.x * kTile + (threadIdx.x >> 5) * (32 * kSortItems) + (threadIdx.x & 31);
+    load_tile<THREADS>(a, blockIdx.x, key, pos);
+    const int64_t t0 = (int64_t)blockIdx.x * (THREADS * kSortItems) + (threadIdx.x >> 5) * (32 * kSortItems) + (threadIdx.x & 31);
 #pragma unroll
     for (int i = 0; i < kSortItems; ++i)
         if (t0 + i * 32 < a.tokens) atomicAdd(&bins[(key[i] >> a.shift) & ((1u << a.digit) - 1)], 1);
     __syncthreads();
-    for (int i = threadIdx.x; i < kBins; i += kTileThreads) a.hist[(int64_t)blockIdx.x * kBins + i] = bins[i];
+    for (int i = threadIdx.x; i < kBins; i += THREADS) a.hist[(int64_t)blockIdx.x * kBins + i] = bins[i];
 }
 
-__global__ void __launch_bounds__(kTileThreads) embed_sort_scatter_kernel(const __grid_constant__ SortArgs a)
+// Dynamic shared memory: [warp][bin] counters, first place of each bin.
+template <int THREADS> constexpr size_t kScatterSmem = (size_t)(THREADS / 32 + 1) * kBins * 4;
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) embed_sort_scatter_kernel(const __grid_constant__ SortArgs a)
 {
-    constexpr int W = kTileThreads / 32, N = kBins / kTileThreads;
-    __shared__ int32_t counts[W * kBins], base[kBins], s_warp[W];
-    for (int i = threadIdx.x; i < W * kBins; i += kTileThreads) counts[i] = 0;
+    constexpr int W = THREADS / 32, N = kBins > THREADS ? kBins / THREADS : 1;  // N bins of a thread
+    extern __shared__ uint4 sh4[];
+    __shared__ int32_t s_warp[W];
+    int32_t *counts = (int32_t *)sh4, *base = counts + W * kBins;
+    for (int i = threadIdx.x; i < W * kBins; i += THREADS) counts[i] = 0;
     __syncthreads();
     pdl_trigger();
     pdl_wait();
     uint32_t key[kSortItems], pos[kSortItems];
-    load_tile(a, blockIdx.x, key, pos);
+    load_tile<THREADS>(a, blockIdx.x, key, pos);
     const uint32_t mask = (1u << a.digit) - 1;
+    const bool mine = (int)threadIdx.x * N < kBins;
     int rank[kSortItems];
-    warp_ranks(key, kSortItems, a.shift, mask, counts, rank);
+    warp_ranks(key, a.shift, mask, counts, rank);
     // pairs of each bin in earlier tiles, and of all smaller bins in all tiles
     int before[N], total[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) before[j] = total[j] = 0;
+    if (mine)
 #pragma unroll 8
-    for (int q = 0; q < a.tiles; ++q)
+        for (int q = 0; q < a.tiles; ++q)
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const int h = a.hist[(int64_t)q * kBins + threadIdx.x * N + j];
+                total[j] += h;
+                before[j] += q < (int)blockIdx.x ? h : 0;
+            }
+    bins_prefix<N>(total, s_warp);  // its barrier puts all warps' counters before warp_prefix
+    if (mine)
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            const int h = a.hist[(int64_t)q * kBins + threadIdx.x * N + j];
-            total[j] += h;
-            before[j] += q < (int)blockIdx.x ? h : 0;
+            base[threadIdx.x * N + j] = total[j] + before[j];
+            warp_prefix<W>(counts, threadIdx.x * N + j);
         }
-    bins_prefix<N>(total, s_warp);  // its barrier puts all warps' counters before warp_prefix
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-        base[threadIdx.x * N + j] = total[j] + before[j];
-        warp_prefix<W>(counts, threadIdx.x * N + j);
-    }
     __syncthreads();
-    const int64_t t0 = (int64_t)blockIdx.x * kTile + (threadIdx.x >> 5) * (32 * kSortItems) + (threadIdx.x & 31);
+    const int64_t t0 = (int64_t)blockIdx.x * (THREADS * kSortItems) + (threadIdx.x >> 5) * (32 * kSortItems) + (threadIdx.x & 31);
 #pragma unroll
     for (int i = 0; i < kSortItems; ++i)
         if (t0 + i * 32 < a.tokens) {  // pairs that pad the tile are last in it: they displace none of the others
@@ -352,7 +367,7 @@ struct SumArgs {
     int64_t tokens, vocab, stride;   // stride: bytes between rows of dy
     const uint32_t *has;             // bits of the rows with a token (null: none has one)
     int64_t tiles;
-    int rows, nvec, nslice, add, zero_rows;     // rows: tokens of a tile
+    int rows, nvec, nslice, add, wide, zero_rows;  // wide: rows of an fp32 out that is added to are whole 32-byte sectors     // rows: tokens of a tile
     float scale;
 };
 constexpr int kSumThreads = 256, kSumBatch = 4, kMostRows = 256;
@@ -363,8 +378,17 @@ template <class T, int B> __device__ __forceinline__ void put_row(const SumArgs 
     const int64_t at = (row * a.nvec + v) * N;
     if (a.add) {
         float *p = (float *)a.out + at;
+        if (N == 8 && a.wide) {  // one 32-byte sector of a lane
+            Bytes<32> v;
+            ld(v, p);
+            float f[8];
+            unpack<float, 32>(v, f);
 #pragma unroll
-        for (int i = 0; i < N; ++i) p[i] += acc[i] * a.scale;
+            for (int i = 0; i < 8; ++i) f[i] = fmaf(acc[i < N ? i : 0], a.scale, f[i]);
+            st(p, pack<float, 32>(f, 1.f));
+        } else
+#pragma unroll
+            for (int i = 0; i < N; ++i) p[i] = fmaf(acc[i], a.scale, p[i]);
     } else
         st((T *)a.out + at, pack<T, B>(acc, a.scale));
 }
@@ -456,12 +480,12 @@ __global__ void __launch_bounds__(kSumThreads) embed_sum_kernel(const __grid_con
         put_row<T, B>(a, cur, v, acc);
 }
 
-// The runs that begin in a tile and go on behind it: their pieces, in order.  N columns of a thread, eight pieces in flight (with one at
+// The runs that begin in a tile and go on behind it: their pieces, in order.  N columns of a thread, sixteen pieces in flight (with one at
 // a time, and 16 columns: 32768 tokens x 4096, the most frequent one 1900 times, 72 us).
 template <class T, int N>
 __global__ void __launch_bounds__(kSumThreads) embed_join_kernel(const __grid_constant__ SumArgs a)
 {
-    constexpr int kBatch = 8;
+    constexpr int kBatch = 16;
     pdl_trigger();
     const int64_t tile = blockIdx.x / a.nslice, t1 = (tile + 1) * a.rows;  // not the last tile
     const int64_t c = ((int64_t)(blockIdx.x - tile * a.nslice) * blockDim.x + threadIdx.x) * N, hidden = a.nvec;
@@ -498,7 +522,7 @@ __global__ void __launch_bounds__(kSumThreads) embed_join_kernel(const __grid_co
     const int64_t at = (int64_t)key * hidden + c;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        if (a.add) ((float *)a.out)[at + i] += acc[i] * a.scale;
+        if (a.add) ((float *)a.out)[at + i] = fmaf(acc[i], a.scale, ((float *)a.out)[at + i]);
         else ((T *)a.out)[at + i] = from_f<T>(acc[i] * a.scale);
     }
 }
@@ -554,7 +578,7 @@ Scratch scratch_of(int64_t tokens, int64_t vocab, int32_t hidden)
     s.pairs = 0;
     s.spare = s.pairs + up(tokens * 8);
     s.hist = s.spare + (tokens > kCountMost ? up(tokens * 8) : 0);
-    s.has = s.hist + (tokens > kCountMost ? up((tokens + kTile - 1) / kTile * kBins * 4) : 0);
+    s.has = s.hist + (tokens > kCountMost ? up(std::max((std::min(tokens, kSmallMost) - 1) / (kSmallTile * kSortItems), (tokens - 1) / (kLargeTile * kSortItems)) * kBins * 4 + kBins * 4) : 0);
     s.pieces = s.has + (tokens ? up((vocab + 31) / 32 * 4) : 0);
     s.bytes = s.pieces + (tiles > 1 ? up(tiles * 2 * hidden * 4) : 0);
     return s;
@@ -582,12 +606,36 @@ template <class T, int B> HcclResult sum(SumArgs &a, int64_t row_bytes, void *st
 template <class T> HcclResult sum_typed(SumArgs &a, int64_t hidden, void *stream)
 {
     const int64_t row = hidden * (int64_t)sizeof(T);
-    switch (vector_bytes(row, (uintptr_t)a.dy | (uintptr_t)a.stride | (a.add ? 0 : (uintptr_t)a.out), sizeof(T), 32)) {
+    a.wide = a.add && hidden % 8 == 0 && ((uintptr_t)a.out & 31) == 0;
+    // where sums are added to an fp32 row a lane has eight columns, a sector of it, at most (with sixteen, one word at a time: 32768 tokens of
+    // 128256 x 4096 954 us)
+    const uintptr_t sector = a.add && sizeof(T) == 2 ? 16 : 0;
+    switch (vector_bytes(row, (uintptr_t)a.dy | (uintptr_t)a.stride | sector | (a.add ? 0 : (uintptr_t)a.out), sizeof(T), 32)) {
         case 32: return sum<T, 32>(a, row, stream);
         case 16: return sum<T, 16>(a, row, stream);
         case 4: return sum<T, 4>(a, row, stream);
         default: return sum<T, sizeof(T)>(a, row, stream);
     }
+}
+
+template <int THREADS> HcclResult sort_tiles(SortArgs &a, uint2 *const (&buf)[2], void *stream, const uint2 **sorted)
+{
+    a.tiles = (int)((a.tokens + THREADS * kSortItems - 1) / (THREADS * kSortItems));
+    const void *scatter = (const void *)embed_sort_scatter_kernel<THREADS>;
+    if (kScatterSmem<THREADS> > 32 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(scatter, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kScatterSmem<THREADS>);
+        CHK_RET_LOG(e != cudaSuccess, HCCL_E_RUNTIME, "embedding gradient set-up failed: %s", cudaGetErrorString(e));
+    }
+    for (int pass = 0; pass < a.passes; ++pass) {
+        a.in = pass ? buf[(pass - 1) & 1] : nullptr;
+        a.out = buf[pass & 1];
+        a.shift = pass * a.digit;
+        a.last = pass == a.passes - 1;
+        CHK_RET(launch_pdl((const void *)embed_sort_hist_kernel<THREADS>, dim3((unsigned)a.tiles), THREADS, 0, &a, stream, "embedding gradient (histogram)"));
+        CHK_RET(launch_pdl(scatter, dim3((unsigned)a.tiles), THREADS, kScatterSmem<THREADS>, &a, stream, "embedding gradient (scatter)"));
+        *sorted = a.out;
+    }
+    return HCCL_SUCCESS;
 }
 
 HcclResult sort_tokens(const EmbedTable &t, const EmbedIds &ids, const Scratch &s, uint8_t *scratch, uint32_t *has, void *stream, const uint2 **sorted)
@@ -606,7 +654,7 @@ HcclResult sort_tokens(const EmbedTable &t, const EmbedIds &ids, const Scratch &
         *sorted = buf[0];
         a.tiles = (int)((ids.tokens + kCountTokens - 1) / kCountTokens);
         const size_t smem = (size_t)(ids.tokens + 3) / 4 * 16 + (has ? kWindow / 8 : 0);
-        if (smem > 48 * 1024) {
+        if (smem > 32 * 1024) {  // with what the kernel has of its own, more than 48 KB needs leave
             const cudaError_t e = cudaFuncSetAttribute((const void *)embed_sort_count_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
             CHK_RET_LOG(e != cudaSuccess, HCCL_E_RUNTIME, "embedding gradient set-up failed: %s", cudaGetErrorString(e));
         }
@@ -614,17 +662,7 @@ HcclResult sort_tokens(const EmbedTable &t, const EmbedIds &ids, const Scratch &
         return launch_pdl((const void *)embed_sort_count_kernel, dim3((unsigned)(a.tiles + windows)), kCountThreads, smem, &a, stream, "embedding gradient (sort)");
     }
     a.hist = (int32_t *)(scratch + s.hist);
-    a.tiles = (int)((ids.tokens + kTile - 1) / kTile);
-    for (int pass = 0; pass < a.passes; ++pass) {
-        a.in = pass ? buf[(pass - 1) & 1] : nullptr;
-        a.out = buf[pass & 1];
-        a.shift = pass * a.digit;
-        a.last = pass == a.passes - 1;
-        CHK_RET(launch_pdl((const void *)embed_sort_hist_kernel, dim3((unsigned)a.tiles), kTileThreads, 0, &a, stream, "embedding gradient (histogram)"));
-        CHK_RET(launch_pdl((const void *)embed_sort_scatter_kernel, dim3((unsigned)a.tiles), kTileThreads, 0, &a, stream, "embedding gradient (scatter)"));
-        *sorted = a.out;
-    }
-    return HCCL_SUCCESS;
+    return ids.tokens <= kSmallMost ? sort_tiles<kSmallTile>(a, buf, stream, sorted) : sort_tiles<kLargeTile>(a, buf, stream, sorted);
 }
 
 }  // namespace

@@ -94,6 +94,16 @@ def test_gate(T, E, k, dtype, normalize):
     check((torch.randn(T, E, device="cuda") * 2).to(dtype), k, None, normalize)
 
 
+def test_every_size_of_a_decode_batch():
+    """Shared memory grows with tokens and experts: every size of it can be launched."""
+    for T in [*range(1, 20), 40, 63, 64, 65, 66, 130]:
+        for E in (60, 129, 257, 300, 400, 511, 700, 1000, 1300, 2000, 2500):
+            l = torch.randn(T, E, device="cuda")
+            g, want = moe.gate(l, 3), gate64(l, 3)
+            assert torch.equal(g.idx, want[0]) and torch.equal(g.counts, want[2]), (T, E)
+            assert moe.gate_grad(l, g, None, 1.0).shape == (T, E)
+
+
 @pytest.mark.parametrize("E,k", [(7, 3), (64, 8), (300, 5)])
 def test_ties_go_to_the_lowest_expert(E, k):
     l = torch.randint(-1, 2, (400, E), device="cuda").float()

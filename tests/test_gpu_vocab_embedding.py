@@ -137,6 +137,15 @@ def test_gradient_of_a_large_batch(T, V, hidden, dtype):
     assert bool((out[(count[:, 0] == 0)] == 0).all())
 
 
+def test_gradient_of_every_number_of_tokens():
+    """Shared memory of the sort grows with the tokens: every size of it can be launched."""
+    for T in [*range(1, 200, 7), *range(3500, 4400, 25), *range(7900, 8300, 33)]:
+        ids, dy = text(T, 77, "zipf"), torch.randn(T, 4, device="cuda")
+        for V in (77, 300000):
+            want, size, count = grad64(ids, dy, V, 1.0)
+            assert close(vocab.embedding_grad(ids, dy, V), want, size, count, torch.float32), T
+
+
 def test_gradient_into_rows_off_a_boundary():
     """A table that starts between vectors, with something before and behind it."""
     for dtype, off in ((torch.bfloat16, 1), (torch.bfloat16, 3), (torch.float32, 1), (torch.float16, 17)):
