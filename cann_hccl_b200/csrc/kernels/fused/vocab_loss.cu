@@ -84,7 +84,7 @@ struct LossShared {
 constexpr size_t kSmemBytes = sizeof(LossShared) + 1024;
 static_assert(kSmemBytes <= 227 * 1024, "one CTA per SM");
 
-// Pairs turn bf16 dW around in the end of the stages' space, 32 rows x 64 columns of a warp at a time, so that a store covers whole 128-byte
+// Pairs turn dW around in the end of the stages' space, 32 rows x 128 bytes of a warp at a time, so that a store covers whole 128-byte
 // lines: a lane's own row in 32-byte stores moves 16 bytes per cycle and SM (1 token, 128256 x 4096: 252 us, 214 this way; as boxes
 // stored by the TMA 335 us).  The exponentials leave in 32-byte stores all the same: beside their 128 values a lane has no
 // registers left for it (1024 tokens, 160000 x 256: 218 against 117 us).
@@ -199,6 +199,35 @@ __device__ __forceinline__ void turn_store(uint8_t *box, const uint4 (&v)[8], in
             const int r = i * 4 + (lane >> 3);
             if (r < rows) *(uint4 *)(to + r * row_bytes + c * 16) = *(const uint4 *)(box + r * 128 + (c ^ (r & 7)) * 16);
         }
+}
+
+// The same for fp32: v: 32 columns of the lane's row; sum, out: the warp's first row and column; rows, cols: that exist.  What is added to
+// is read a whole line at a time too (512 tokens x 128256 x 4096 2.2 ms; with rows added to in 16-byte pieces of a lane 3.3 ms).
+__device__ __forceinline__ void turn_sum(uint8_t *box, const float *v, int lane, int kind, float *sum, __nv_bfloat16 *out, int64_t ld, int rows, int cols)
+{
+    __syncwarp();
+#pragma unroll
+    for (int c = 0; c < 8; ++c) *(float4 *)(box + lane * 128 + (c ^ (lane & 7)) * 16) = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+    __syncwarp();
+    const int c = lane & 7;
+    if (c * 4 >= cols) return;
+    float4 g[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int r = i * 4 + (lane >> 3);
+        g[i] = kind != VL_F32 && r < rows ? __ldcs((const float4 *)(sum + r * ld + c * 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int r = i * 4 + (lane >> 3);
+        if (r >= rows) continue;
+        const float4 x = *(const float4 *)(box + r * 128 + (c ^ (r & 7)) * 16);
+        const float4 y = make_float4(g[i].x + x.x, g[i].y + x.y, g[i].z + x.z, g[i].w + x.w);
+        if (kind == VL_ADD_BF16)
+            *(uint2 *)(out + r * ld + c * 4) = make_uint2(pack_bf16(__float_as_uint(y.x), __float_as_uint(y.y)), pack_bf16(__float_as_uint(y.z), __float_as_uint(y.w)));
+        else
+            __stcs((float4 *)(sum + r * ld + c * 4), y);
+    }
 }
 
 template <int MODE, bool kPair>
@@ -414,6 +443,15 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_loss_gemm(const __grid_cons
                         if (last && c + 64 == kHalf) release(buf);
 #pragma unroll
                         for (int i = 0; i < 64; ++i) v[i] *= scale;
+                        if constexpr (kTurn<MODE, kPair>)
+                            if (P.kind != VL_BF16) {
+#pragma unroll
+                                for (int i = 0; i < 64; i += 32)
+                                    if (c + i < left)
+                                        turn_sum(box, v + i, lane, P.kind, sum + at - (int64_t)lane * P.N + c + i, P.out + at - (int64_t)lane * P.N + c + i, P.N,
+                                                 P.M - (row - lane), left - c - i);
+                                continue;
+                            }
                         if (P.kind == VL_ADD || P.kind == VL_ADD_BF16)
 #pragma unroll
                             for (int i = 0; i < 64; i += 4)
@@ -813,7 +851,7 @@ HcclResult launch_gemm(int mode, bool pair, LossGemm &P, void *stream)
     P.units = pair ? d.pairs : d.sms;
     P.a_bytes = (uint32_t)a_rows(mode, P.M, P.cols) * BK * 2;
     P.stage_bytes = P.a_bytes + (uint32_t)(P.cols / ctas) * BK * 2;
-    const bool turned = pair && mode == DW && (P.kind == VL_BF16 || P.kind == VL_ADD_BF16);
+    const bool turned = pair && mode == DW;
     P.stages = (int)std::min<uint32_t>(kMaxStages, (kStageSpace - (turned ? kTurnSpace : 0)) / P.stage_bytes);
     P.idesc = instr_desc((uint32_t)(ctas * BM), (uint32_t)P.cols) | (mode == DW ? 1u << 15 : 0u) | (mode != SCORES ? 1u << 16 : 0u);
     // a panel's columns of B stay in L2 (40 MB of it) while the rows stream past

@@ -214,7 +214,9 @@ __device__ __forceinline__ void mark_row(const SortArgs &a, uint32_t row)
     if (!a.has || row >= (uint32_t)a.vocab) return;
     uint32_t *word = a.has + (row >> 5);
     const uint32_t bit = 1u << (row & 31);
-    if (!(__ldcg(word) & bit)) atomicOr(word, bit);  // most tokens find their bit set
+    // where tokens are more than rows most find their bit set (2^20 tokens of 1000 rows: 370 us for their atomics alone); elsewhere the
+    // look costs more than it saves (32768 tokens of 128256 rows: 3 us)
+    if (a.tokens < a.vocab || !(__ldcg(word) & bit)) atomicOr(word, bit);
 }
 
 __device__ __forceinline__ uint32_t key_at(const SortArgs &a, int64_t t)
@@ -480,12 +482,28 @@ __global__ void __launch_bounds__(kSumThreads) embed_sum_kernel(const __grid_con
         put_row<T, B>(a, cur, v, acc);
 }
 
+// Up to M pieces, one after the other but loaded together.
+template <int N, int M> __device__ __forceinline__ void add_pieces(const float *src, int64_t hidden, int n, float (&acc)[N])
+{
+    float h[M][N];
+#pragma unroll
+    for (int j = 0; j < M; ++j)
+        if (j < n) {
+            if (N == 4) *(float4 *)h[j] = *(const float4 *)(src + j * 2 * hidden);
+            else h[j][0] = src[j * 2 * hidden];
+        }
+#pragma unroll
+    for (int j = 0; j < M; ++j)
+        if (j < n)
+#pragma unroll
+            for (int i = 0; i < N; ++i) acc[i] += h[j][i];
+}
+
 // The runs that begin in a tile and go on behind it: their pieces, in order.  N columns of a thread, sixteen pieces in flight (with one at
 // a time, and 16 columns: 32768 tokens x 4096, the most frequent one 1900 times, 72 us).
 template <class T, int N>
 __global__ void __launch_bounds__(kSumThreads) embed_join_kernel(const __grid_constant__ SumArgs a)
 {
-    constexpr int kBatch = 16;
     pdl_trigger();
     const int64_t tile = blockIdx.x / a.nslice, t1 = (tile + 1) * a.rows;  // not the last tile
     const int64_t c = ((int64_t)(blockIdx.x - tile * a.nslice) * blockDim.x + threadIdx.x) * N, hidden = a.nvec;
@@ -503,22 +521,9 @@ __global__ void __launch_bounds__(kSumThreads) embed_join_kernel(const __grid_co
     const float *p = a.pieces + (tile * 2 + 1) * hidden + c;
 #pragma unroll
     for (int i = 0; i < N; ++i) acc[i] = p[i];
-    for (int64_t q0 = tile + 1; q0 <= last; q0 += kBatch) {
-        float h[kBatch][N];
-#pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-            const float *src = a.pieces + (q0 + j) * 2 * hidden + c;
-            if (q0 + j <= last) {
-                if (N == 4) *(float4 *)h[j] = *(const float4 *)src;
-                else h[j][0] = src[0];
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < kBatch; ++j)
-            if (q0 + j <= last)
-#pragma unroll
-                for (int i = 0; i < N; ++i) acc[i] += h[j][i];
-    }
+    int64_t q0 = tile + 1;
+    for (; q0 + 15 <= last; q0 += 16) add_pieces<N, 16>(a.pieces + q0 * 2 * hidden + c, hidden, 16, acc);
+    for (; q0 <= last; q0 += 4) add_pieces<N, 4>(a.pieces + q0 * 2 * hidden + c, hidden, (int)min((int64_t)4, last - q0 + 1), acc);
     const int64_t at = (int64_t)key * hidden + c;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
