@@ -189,6 +189,7 @@ def lib():
         "HcclB200VocabLossTotal": [P(VocabLoss), vp, vp],
         "HcclB200VocabLossSum": [P(VocabLoss), vp, vp, vp, vp],
         "HcclB200VocabLossGrad": [P(VocabLoss), vp, vp, vp, C.c_float, vp, vp, vp, i32, vp, vp],
+        "HcclB200VocabLossStep": [P(VocabLoss), i32, C.c_float, vp, vp, vp, vp, i32, vp, vp],
         "HcclB200MoeGate": [vp, C.c_int, C.c_int64, i32, C.c_int64, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp],
         "HcclB200MoeBalance": [vp, vp, vp, i32, i32, vp, vp],
         "HcclB200MoeGateGrad": [vp, C.c_int, C.c_int64, i32, C.c_int64, i32, i32, vp, vp, vp, vp, vp, C.c_float, vp, vp],
@@ -243,7 +244,8 @@ def lib():
     L.HcclB200MoeGateScratchBytes.argtypes = [C.c_int64, i32]
     L.HcclB200VocabLossChunk.argtypes = [C.c_int64, i32]
     L.HcclB200VocabLossScratchBytes.argtypes = [C.c_int64, C.c_int64, i32, i32]
-    L.HcclB200VocabLossChunk.restype = L.HcclB200VocabLossScratchBytes.restype = C.c_int64
+    L.HcclB200VocabLossStepBytes.argtypes = [C.c_int64, C.c_int64, i32]
+    L.HcclB200VocabLossChunk.restype = L.HcclB200VocabLossScratchBytes.restype = L.HcclB200VocabLossStepBytes.restype = C.c_int64
     L.HcclB200EmbeddingGradScratchBytes.restype = L.HcclB200MoeGateScratchBytes.restype = C.c_int64
     L.HcclGetErrorString.argtypes = [C.c_int]
     L.HcclGetErrorString.restype = C.c_char_p

@@ -926,18 +926,36 @@ HcclResult HcclB200VocabLossSum(const HcclB200VocabLoss *p, const float *losses,
     CHK_RET(check_aligned({losses, total}, 4, "HcclB200VocabLossSum"));
     return vocab_loss_sum(c, losses, total, loss, stream);
 }
+static HcclResult check_dw(const VocabLossCall &c, const void *dx, const void *dw, const void *dwSum, int32_t dwKind, const void *scratch, const char *api)
+{
+    CHK_RET_LOG(dwKind < VL_BF16 || dwKind > VL_ADD_BF16, HCCL_E_PARA, "%s: unknown kind %d of dw", api, dwKind);
+    CHK_RET_LOG((c.tokens && !dx) || (!dw && (dwKind == VL_BF16 || dwKind == VL_ADD_BF16)) || (!dwSum && dwKind != VL_BF16), HCCL_E_PTR, "[EI0003] %s: null pointer", api);
+    CHK_RET(check_aligned({dx, dw, dwSum}, 16, api));
+    CHK_RET(check_aligned({scratch}, 256, api));
+    CHK_RET_LOG(!c.tokens, HCCL_E_PARA, "%s: no tokens", api);
+    return HCCL_SUCCESS;
+}
+int64_t HcclB200VocabLossStepBytes(int64_t tokens, int64_t vocab, int32_t hidden)
+{
+    return tokens < 1 || tokens > kVocabStepMost || vocab < 1 || vocab >= INT32_MAX - 256 || hidden < 8 || hidden % 8 ? -1 : vocab_loss_step_bytes(tokens, vocab, hidden);
+}
+HcclResult HcclB200VocabLossStep(const HcclB200VocabLoss *p, int32_t mean, float scale, float *loss, void *dx, void *dw, float *dwSum, int32_t dwKind, void *scratch,
+                                 aclrtStream stream)
+{
+    VocabLossCall c;
+    CHK_RET(check_vocab_loss(p, false, {loss, scratch}, "HcclB200VocabLossStep", &c));
+    CHK_RET(check_dw(c, dx, dw, dwSum, dwKind, scratch, "HcclB200VocabLossStep"));
+    CHK_RET_LOG(c.tokens > kVocabStepMost || c.vocab != c.whole, HCCL_E_PARA, "HcclB200VocabLossStep: %lld tokens (at most %lld) against %lld of %lld ids", (long long)c.tokens,
+                (long long)kVocabStepMost, (long long)c.vocab, (long long)c.whole);
+    return vocab_loss_step(c, mean != 0, scale, loss, dx, dw, dwSum, dwKind, scratch, stream);
+}
 HcclResult HcclB200VocabLossGrad(const HcclB200VocabLoss *p, const float *lse, const float *target, const float *total, float scale, void *dx, void *dw,
                                  float *dwSum, int32_t dwKind, void *scratch, aclrtStream stream)
 {
     VocabLossCall c;
     CHK_RET(check_vocab_loss(p, false, {lse, target, scratch}, "HcclB200VocabLossGrad", &c));
-    CHK_RET_LOG(dwKind < VL_BF16 || dwKind > VL_ADD_BF16, HCCL_E_PARA, "HcclB200VocabLossGrad: unknown kind %d of dw", dwKind);
-    CHK_RET_LOG((c.tokens && !dx) || (!dw && (dwKind == VL_BF16 || dwKind == VL_ADD_BF16)) || (!dwSum && dwKind != VL_BF16), HCCL_E_PTR,
-                "[EI0003] HcclB200VocabLossGrad: null pointer");
-    CHK_RET(check_aligned({dx, dw, dwSum}, 16, "HcclB200VocabLossGrad"));
     CHK_RET(check_aligned({total}, 4, "HcclB200VocabLossGrad"));
-    CHK_RET(check_aligned({scratch}, 256, "HcclB200VocabLossGrad"));
-    CHK_RET_LOG(!c.tokens, HCCL_E_PARA, "HcclB200VocabLossGrad: no tokens");
+    CHK_RET(check_dw(c, dx, dw, dwSum, dwKind, scratch, "HcclB200VocabLossGrad"));
     return vocab_loss_grad(c, lse, target, total, scale, dx, dw, dwSum, dwKind, scratch, stream);
 }
 static HcclResult check_act(int32_t act, const char *api)

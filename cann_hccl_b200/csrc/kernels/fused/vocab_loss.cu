@@ -499,6 +499,7 @@ struct RowArgs {
     const void *y;
     const float *weights, *losses_in, *total;
     float *lse, *target, *losses, *out;
+    uint32_t *arrived;               // whole step: CTAs that have a token's loss; the last one adds the losses to `out` (null: none does)
     uint8_t *e;                      // [row][ld] 2 bytes each
     const uint8_t *x, *w;
     uint8_t *xc;
@@ -525,22 +526,42 @@ __device__ __forceinline__ float warp_sum(float x)
 
 constexpr int kRowThreads = 128, kRowRegs = 8;
 
-// One CTA per token.
-__global__ void __launch_bounds__(kRowThreads) vocab_loss_rows(const __grid_constant__ RowArgs a)
+// Sum of v over the CTA's threads in one order; the result in thread 0 (in its warp).
+template <int THREADS> __device__ __forceinline__ float block_sum(float v, float *s_w)
 {
-    __shared__ float s_m[kRowThreads / 32], s_z[kRowThreads / 32], s_d[kRowThreads / 32];
-    pdl_trigger();
-    pdl_wait();
-    const int64_t t = blockIdx.x;
+    v = warp_sum(v);
+    if ((threadIdx.x & 31) == 0) s_w[threadIdx.x >> 5] = v;
+    __syncthreads();
+    return threadIdx.x < 32 ? warp_sum(threadIdx.x < THREADS / 32 ? s_w[threadIdx.x] : 0.f) : 0.f;
+}
+// A thread's share of the sum of the weights (losses null) or of weights * losses.
+template <int THREADS> __device__ __forceinline__ float weights_sum(const RowArgs &a, const float *losses)
+{
+    float sum = 0.f;
+#pragma unroll 4
+    for (int64_t t = threadIdx.x; t < a.tokens; t += THREADS) {
+        const float q = weight(a, t, target_of(a.y, a.wide, t));
+        sum += !losses ? q : q == 0.f ? 0.f : q * __ldcg(losses + t);
+    }
+    return sum;
+}
+
+struct RowState { float top, log_z, target; };  // lse = top + log_z
+template <int THREADS> struct RowShared { float m[THREADS / 32], z[THREADS / 32], d[THREADS / 32]; };
+
+// A token's sums over its half tiles, by the whole CTA.
+template <int THREADS> __device__ __forceinline__ RowState row_state(const RowArgs &a, int64_t t, int64_t id, RowShared<THREADS> &s)
+{
+    constexpr int W = THREADS / 32;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t id = target_of(a.y, a.wide, t);
     const uint64_t at = (uint64_t)id - (uint64_t)a.first;
     const bool here = counts(a, id) && at < (uint64_t)a.vocab;
-    float dot = 0.f;  // the target's logit
+    float dot = 0.f, given = 0.f;  // the target's logit, as it is and as the tensor cores have it
     if (here) {
+        given = a.target[t];
         const uint4 *x = (const uint4 *)(a.x + t * a.x_stride), *w = (const uint4 *)(a.w + (int64_t)at * a.w_stride);
 #pragma unroll 4
-        for (int v = threadIdx.x; v < a.xvec; v += kRowThreads) {
+        for (int v = threadIdx.x; v < a.xvec; v += THREADS) {
             const uint4 p = x[v], q = w[v];
             const uint32_t pw[4] = {p.x, p.y, p.z, p.w}, qw[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
@@ -550,16 +571,16 @@ __global__ void __launch_bounds__(kRowThreads) vocab_loss_rows(const __grid_cons
             }
         }
         dot = warp_sum(dot);
-        if (lane == 0) s_d[warp] = dot;
+        if (lane == 0) s.d[warp] = dot;
     }
     const float2 *p = a.stats + t * a.halves;
     float m = -INFINITY, z = 0.f;
-    for (int i0 = 0; i0 < a.halves; i0 += kRowThreads * kRowRegs) {
+    for (int i0 = 0; i0 < a.halves; i0 += THREADS * kRowRegs) {
         float2 v[kRowRegs];
         float top = m;
 #pragma unroll
         for (int k = 0; k < kRowRegs; ++k) {
-            const int i = i0 + k * kRowThreads + threadIdx.x;
+            const int i = i0 + k * THREADS + threadIdx.x;
             v[k] = i < a.halves ? p[i] : make_float2(-INFINITY, 0.f);
             top = fmaxf(top, v[k].x);
         }
@@ -570,34 +591,67 @@ __global__ void __launch_bounds__(kRowThreads) vocab_loss_rows(const __grid_cons
         m = top;
     }
     const float wm = warp_max(m);
-    if (lane == 0) s_m[warp] = wm;
+    if (lane == 0) s.m[warp] = wm;
     __syncthreads();
-    float all = s_m[0];
+    RowState r;
+    r.top = s.m[0];
 #pragma unroll
-    for (int w = 1; w < kRowThreads / 32; ++w) all = fmaxf(all, s_m[w]);
-    const float ref = all == -INFINITY ? 0.f : all;
+    for (int w = 1; w < W; ++w) r.top = fmaxf(r.top, s.m[w]);
+    const float ref = r.top == -INFINITY ? 0.f : r.top;
     z = warp_sum(z * __expf(m - ref));
-    if (lane == 0) s_z[warp] = z;
-    __syncthreads();
-    if (threadIdx.x) return;
-    z = s_z[0];
+    if (lane == 0) s.z[warp] = z;
+    __syncthreads();  // also: every thread has read the target's logit that the caller replaces
+    z = s.z[0];
 #pragma unroll
-    for (int w = 1; w < kRowThreads / 32; ++w) z += s_z[w];
-    float log_z = logf(z), target = -INFINITY;
+    for (int w = 1; w < W; ++w) z += s.z[w];
+    r.log_z = logf(z);
+    r.target = -INFINITY;
     if (here) {
-        target = a.target[t];
-        dot = s_d[0];
+        dot = s.d[0];
 #pragma unroll
-        for (int w = 1; w < kRowThreads / 32; ++w) dot += s_d[w];
-        const float off = dot - target;  // far off only where logits have no digits behind the point: both stay as they are then
+        for (int w = 1; w < W; ++w) dot += s.d[w];
+        const float off = dot - given;  // far off only where logits have no digits behind the point: both stay as they are then
+        r.target = given;
         if (fabsf(off) < 0.5f) {
-            log_z += log1pf(__expf((target - all) - log_z) * expm1f(off));
-            target = dot;
+            r.log_z += log1pf(__expf((given - r.top) - r.log_z) * expm1f(off));
+            r.target = dot;
         }
     }
-    a.lse[t] = all + log_z;
-    a.target[t] = target;
-    if (a.losses) a.losses[t] = counts(a, id) && !(a.grad && weight(a, t, id) == 0.f) ? (all - target) + log_z : 0.f;
+    return r;
+}
+
+// What a token's CTA leaves; in a whole step the CTA that is last adds the losses, in the order of the tokens.
+template <int THREADS> __device__ __forceinline__ void row_end(const RowArgs &a, int64_t t, int64_t id, const RowState &r, float *s_w)
+{
+    __shared__ int s_last;
+    if (threadIdx.x == 0) {
+        a.lse[t] = r.top + r.log_z;
+        a.target[t] = r.target;
+        if (a.losses) a.losses[t] = counts(a, id) && !(a.grad && weight(a, t, id) == 0.f) ? (r.top - r.target) + r.log_z : 0.f;
+        if (a.arrived) {
+            __threadfence();
+            s_last = atomicAdd(a.arrived, 1u) == a.tokens - 1;
+            __threadfence();
+        }
+    }
+    if (!a.arrived) return;
+    __syncthreads();
+    if (!s_last) return;
+    float sum = block_sum<THREADS>(weights_sum<THREADS>(a, a.losses), s_w);
+    if (threadIdx.x) return;
+    if (a.total) sum = *a.total != 0.f ? sum / *a.total : 0.f;
+    *a.out = sum;
+}
+
+// One CTA per token.
+__global__ void __launch_bounds__(kRowThreads) vocab_loss_rows(const __grid_constant__ RowArgs a)
+{
+    __shared__ RowShared<kRowThreads> s;
+    pdl_trigger();
+    pdl_wait();
+    const int64_t t = blockIdx.x, id = target_of(a.y, a.wide, t);
+    const RowState r = row_state<kRowThreads>(a, t, id, s);
+    row_end<kRowThreads>(a, t, id, r, s.m);
 }
 
 // Joint lse and loss from the shards'.
@@ -627,18 +681,7 @@ __global__ void __launch_bounds__(kSumThreads) vocab_loss_reduce(const __grid_co
     __shared__ float s_w[kSumThreads / 32];
     pdl_trigger();
     pdl_wait();
-    float sum = 0.f;
-#pragma unroll 4
-    for (int64_t t = threadIdx.x; t < a.tokens; t += kSumThreads) {
-        float v = weight(a, t, target_of(a.y, a.wide, t));
-        if (a.losses_in) v = v == 0.f ? 0.f : v * a.losses_in[t];
-        sum += v;
-    }
-    sum = warp_sum(sum);
-    if ((threadIdx.x & 31) == 0) s_w[threadIdx.x >> 5] = sum;
-    __syncthreads();
-    if (threadIdx.x >= 32) return;
-    sum = warp_sum(s_w[threadIdx.x]);
+    float sum = block_sum<kSumThreads>(weights_sum<kSumThreads>(a, a.losses_in), s_w);
     if (threadIdx.x) return;
     if (a.total) sum = *a.total != 0.f ? sum / *a.total : 0.f;
     *a.out = sum;
@@ -648,31 +691,35 @@ constexpr int kCopyThreads = 256;
 // Rows of x to rows of xc that start on 128-byte boundaries; with gradients zeros for tokens that have no part in them.
 __global__ void __launch_bounds__(kCopyThreads) vocab_loss_x(const __grid_constant__ RowArgs a)
 {
+    __shared__ float s_w[kCopyThreads / 32];
     pdl_trigger();
     const int64_t i = (int64_t)blockIdx.x * kCopyThreads + threadIdx.x, t = i / a.xvec;
     const int v = (int)(i - t * a.xvec);
     pdl_wait();
+    if (a.arrived && blockIdx.x == gridDim.x - 1) {  // a whole step: the CTA behind the copies has the sum of the weights
+        const float sum = block_sum<kCopyThreads>(weights_sum<kCopyThreads>(a, nullptr), s_w);
+        if (threadIdx.x == 0) {
+            *a.arrived = 0;
+            if (a.out) *a.out = sum;
+        }
+        return;
+    }
     if (t >= a.tokens) return;
     const bool on = !a.grad || weight(a, t, target_of(a.y, a.wide, t)) != 0.f;
     ((uint4 *)a.xc)[t * (a.ld / 8) + v] = on ? ((const uint4 *)(a.x + t * a.x_stride))[v] : make_uint4(0, 0, 0, 0);
 }
 
 constexpr int kDThreads = 256, kDBatch = 4, kDVecs = kDThreads * kDBatch;
-// Exponentials -> d, in place.  grid (stretches of a row, tokens): kDVecs vectors of 8 columns at a time, in turn.
-__global__ void __launch_bounds__(kDThreads) vocab_loss_d(const __grid_constant__ RowArgs a)
+// Exponentials -> d, in place: kDVecs vectors of 8 columns at a time, from the part-th on, every parts-th.
+__device__ __forceinline__ void row_to_d(const RowArgs &a, int64_t t, int64_t id, float lse, float target, uint32_t part, uint32_t parts)
 {
-    pdl_trigger();
-    pdl_wait();
-    const int64_t t = blockIdx.y;
-    const int64_t id = target_of(a.y, a.wide, t);
     const float q = weight(a, t, id);
     uint4 *row = (uint4 *)(a.e + t * a.ld * 2);
     const uint32_t vecs = (uint32_t)(a.width / 8), cols = (uint32_t)a.cols, mid = (cols / 16 + 1) / 2 * 16;
-    const float lse = a.lse[t];
     const int64_t y = id - a.first;  // may lie in another shard
-    const float dy = q * expm1f(a.target[t] - lse);
+    const float dy = q * expm1f(target - lse);
     const float2 *stats = a.stats + t * a.halves;
-    for (uint32_t v0 = blockIdx.x * kDVecs + threadIdx.x; v0 < vecs; v0 += gridDim.x * kDVecs) {
+    for (uint32_t v0 = part * kDVecs + threadIdx.x; v0 < vecs; v0 += parts * kDVecs) {
         uint4 v[kDBatch];
         float f[kDBatch];
         if (q != 0.f)
@@ -708,6 +755,27 @@ __global__ void __launch_bounds__(kDThreads) vocab_loss_d(const __grid_constant_
             row[i] = o;
         }
     }
+}
+
+// grid (parts of a row, tokens)
+__global__ void __launch_bounds__(kDThreads) vocab_loss_d(const __grid_constant__ RowArgs a)
+{
+    pdl_trigger();
+    pdl_wait();
+    const int64_t t = blockIdx.y;
+    row_to_d(a, t, target_of(a.y, a.wide, t), a.lse[t], a.target[t], blockIdx.x, gridDim.x);
+}
+
+// rows and d of a token by one CTA
+__global__ void __launch_bounds__(kDThreads) vocab_loss_rows_d(const __grid_constant__ RowArgs a)
+{
+    __shared__ RowShared<kDThreads> s;
+    pdl_trigger();
+    pdl_wait();
+    const int64_t t = blockIdx.x, id = target_of(a.y, a.wide, t);
+    const RowState r = row_state<kDThreads>(a, t, id, s);
+    row_to_d(a, t, id, r.top + r.log_z, r.target, 0, 1);
+    row_end<kDThreads>(a, t, id, r, s.m);
 }
 
 struct ShareArgs { const float *shares; __nv_bfloat16 *out; int64_t n; int split; };
@@ -885,11 +953,11 @@ int64_t vocab_loss_scratch_bytes(int64_t tokens, int64_t vocab, int32_t hidden, 
     return layout_of(tokens, vocab, hidden, grad, &l) == HCCL_SUCCESS ? std::max<int64_t>(1024, l.bytes) : -1;
 }
 
-HcclResult vocab_loss_scores(const VocabLossCall &c, bool grad, float *lse, float *target, float *losses, void *scratch, void *stream)
+namespace {
+
+// The copy of x (with the sum of the weights of a whole step) and the scores; leaves what the rows need in *a.
+HcclResult scores(const VocabLossCall &c, const Layout &l, bool grad, float *target, uint8_t *s, void *stream, RowArgs *a)
 {
-    Layout l;
-    CHK_RET(layout_of(c.tokens, c.vocab, c.hidden, grad, &l));
-    uint8_t *s = (uint8_t *)scratch;
     LossGemm P;
     memset(&P, 0, sizeof(P));
     P.M = (int)c.tokens; P.N = (int)c.vocab; P.cols = l.cols; P.split = 1;
@@ -897,19 +965,75 @@ HcclResult vocab_loss_scores(const VocabLossCall &c, bool grad, float *lse, floa
     P.stats = (float2 *)(s + l.stats); P.target = target;
     P.e = grad ? (__half *)s : nullptr; P.ld = l.ld; P.width = l.width;
     P.y = c.targets; P.wide_y = c.wide; P.first = c.first; P.ignore = c.ignore;
+    a->x = (const uint8_t *)c.x; a->x_stride = c.x_stride * 2; a->xvec = c.hidden / 8; a->grad = grad;
     if (l.copy) {
-        RowArgs a = row_args(c);
-        a.x = (const uint8_t *)c.x; a.x_stride = c.x_stride * 2; a.xc = s + l.xc; a.ld = l.xld; a.xvec = c.hidden / 8; a.grad = grad;
-        CHK_RET(launch_pdl((const void *)vocab_loss_x, dim3((unsigned)((c.tokens * a.xvec + kCopyThreads - 1) / kCopyThreads)), kCopyThreads, 0, &a, stream,
-                           "vocabulary loss (x)"));
+        RowArgs q = *a;
+        q.xc = s + l.xc; q.ld = l.xld;
+        const int64_t ctas = (c.tokens * q.xvec + kCopyThreads - 1) / kCopyThreads + (a->arrived ? 1 : 0);
+        CHK_RET(launch_pdl((const void *)vocab_loss_x, dim3((unsigned)ctas), kCopyThreads, 0, &q, stream, "vocabulary loss (x)"));
     }
     CHK_RET(encode_2d(&P.tmA, l.copy ? s + l.xc : c.x, c.tokens, c.hidden, a_rows(SCORES, (int)c.tokens, l.cols), l.copy ? l.xld : c.x_stride));
     CHK_RET(encode_2d(&P.tmB, c.w, c.vocab, c.hidden, l.cols / (l.pair ? 2 : 1), c.w_stride));
     CHK_RET(launch_gemm(SCORES, l.pair, P, stream));
+    a->stats = P.stats; a->halves = 2 * l.n_tiles; a->cols = l.cols;
+    a->w = (const uint8_t *)c.w; a->w_stride = c.w_stride * 2;
+    a->e = s; a->ld = l.ld; a->width = l.width;
+    return HCCL_SUCCESS;
+}
+
+HcclResult rows_to_d(const VocabLossCall &c, const Layout &l, const RowArgs &a, void *stream)
+{
+    // enough CTAs to fill the GPU a few times, none without work (129 tokens x 160000 by one CTA each: 50 us)
+    const int64_t parts = std::min<int64_t>((l.width / 8 + kDVecs - 1) / kDVecs, std::max<int64_t>(1, 4096 / c.tokens));
+    // tokens along y, 65535 of them at most in a launch
+    for (int64_t t0 = 0; t0 < c.tokens; t0 += 65535) {
+        RowArgs q = a;
+        const int64_t n = std::min<int64_t>(65535, c.tokens - t0);
+        q.y = (const uint8_t *)a.y + t0 * (a.wide ? 8 : 4);
+        q.weights = a.weights ? a.weights + t0 : nullptr;
+        q.e += t0 * a.ld * 2; q.lse += t0; q.target += t0; q.stats += t0 * a.halves;
+        CHK_RET(launch_pdl((const void *)vocab_loss_d, dim3((unsigned)parts, (unsigned)n), kDThreads, 0, &q, stream, "vocabulary loss (d)"));
+    }
+    return HCCL_SUCCESS;
+}
+
+HcclResult products(const VocabLossCall &c, const Layout &l, const float *total, float scale, void *dx, void *dw, float *dw_sum, int out, uint8_t *s, void *stream)
+{
+    LossGemm P;
+    memset(&P, 0, sizeof(P));
+    P.M = (int)c.tokens; P.N = c.hidden; P.cols = kMaxCols;
+    P.total = total; P.scale = scale;
+    P.k_iters = (int)((c.vocab + BK - 1) / BK);
+    P.split = l.split;
+    P.kind = l.split > 1 ? VL_F32 : VL_BF16;
+    P.out = (__nv_bfloat16 *)dx; P.sum = (float *)(s + l.shares);
+    CHK_RET(encode_2d(&P.tmA, s, c.tokens, l.width, a_rows(DX, (int)c.tokens, kMaxCols), l.ld));
+    CHK_RET(encode_2d(&P.tmB, c.w, c.vocab, c.hidden, BK, c.w_stride));
+    CHK_RET(launch_gemm(DX, l.pair, P, stream));
+    if (l.split > 1) {
+        ShareArgs q = {P.sum, P.out, c.tokens * c.hidden, l.split};
+        CHK_RET(launch_pdl((const void *)vocab_loss_shares, dim3((unsigned)((q.n / 8 + 31) / 32)), 32 * kShareSlices, 0, &q, stream, "vocabulary loss (dx)"));
+    }
+
+    memset(&P, 0, sizeof(P));
+    P.M = (int)c.vocab; P.N = c.hidden; P.cols = kMaxCols; P.split = 1;
+    P.total = total; P.scale = scale;
+    P.k_iters = (int)((c.tokens + BK - 1) / BK);
+    P.kind = out; P.out = (__nv_bfloat16 *)dw; P.sum = dw_sum;
+    CHK_RET(encode_2d(&P.tmA, s, c.tokens, l.width, BK, l.ld));
+    CHK_RET(encode_2d(&P.tmB, s + l.xc, c.tokens, c.hidden, BK, l.xld));
+    return launch_gemm(DW, c.vocab > BM, P, stream);
+}
+
+}  // namespace
+
+HcclResult vocab_loss_scores(const VocabLossCall &c, bool grad, float *lse, float *target, float *losses, void *scratch, void *stream)
+{
+    Layout l;
+    CHK_RET(layout_of(c.tokens, c.vocab, c.hidden, grad, &l));
     RowArgs a = row_args(c);
-    a.stats = P.stats; a.halves = 2 * l.n_tiles;
+    CHK_RET(scores(c, l, grad, target, (uint8_t *)scratch, stream, &a));
     a.lse = lse; a.target = target; a.losses = losses;
-    a.x = (const uint8_t *)c.x; a.w = (const uint8_t *)c.w; a.x_stride = c.x_stride * 2; a.w_stride = c.w_stride * 2; a.xvec = c.hidden / 8; a.grad = grad;
     return launch_pdl((const void *)vocab_loss_rows, dim3((unsigned)c.tokens), kRowThreads, 0, &a, stream, "vocabulary loss (rows)");
 }
 
@@ -943,42 +1067,36 @@ HcclResult vocab_loss_grad(const VocabLossCall &c, const float *lse, const float
     RowArgs a = row_args(c);
     a.stats = (const float2 *)(s + l.stats); a.halves = 2 * l.n_tiles; a.cols = l.cols;
     a.e = s; a.ld = l.ld; a.width = l.width; a.lse = (float *)lse; a.target = (float *)target;
-    // enough CTAs to fill the GPU a few times, none without work (129 tokens x 160000 by one CTA each: 50 us)
-    const int64_t parts = std::min<int64_t>((l.width / 8 + kDVecs - 1) / kDVecs, std::max<int64_t>(1, 4096 / c.tokens));
-    // tokens along y, 65535 of them at most in a launch
-    for (int64_t t0 = 0; t0 < c.tokens; t0 += 65535) {
-        RowArgs q = a;
-        const int64_t n = std::min<int64_t>(65535, c.tokens - t0);
-        q.y = (const uint8_t *)a.y + t0 * (a.wide ? 8 : 4);
-        q.weights = a.weights ? a.weights + t0 : nullptr;
-        q.e += t0 * a.ld * 2; q.lse += t0; q.target += t0; q.stats += t0 * a.halves;
-        CHK_RET(launch_pdl((const void *)vocab_loss_d, dim3((unsigned)parts, (unsigned)n), kDThreads, 0, &q, stream, "vocabulary loss (d)"));
-    }
+    CHK_RET(rows_to_d(c, l, a, stream));
+    return products(c, l, total, scale, dx, dw, dw_sum, out, s, stream);
+}
 
-    LossGemm P;
-    memset(&P, 0, sizeof(P));
-    P.M = (int)c.tokens; P.N = c.hidden; P.cols = kMaxCols;
-    P.total = total; P.scale = scale;
-    P.k_iters = (int)((c.vocab + BK - 1) / BK);
-    P.split = l.split;
-    P.kind = l.split > 1 ? VL_F32 : VL_BF16;
-    P.out = (__nv_bfloat16 *)dx; P.sum = (float *)(s + l.shares);
-    CHK_RET(encode_2d(&P.tmA, s, c.tokens, l.width, a_rows(DX, (int)c.tokens, kMaxCols), l.ld));
-    CHK_RET(encode_2d(&P.tmB, c.w, c.vocab, c.hidden, BK, c.w_stride));
-    CHK_RET(launch_gemm(DX, l.pair, P, stream));
-    if (l.split > 1) {
-        ShareArgs q = {P.sum, P.out, c.tokens * c.hidden, l.split};
-        CHK_RET(launch_pdl((const void *)vocab_loss_shares, dim3((unsigned)((q.n / 8 + 31) / 32)), 32 * kShareSlices, 0, &q, stream, "vocabulary loss (dx)"));
-    }
+// Behind the scratch of its parts: lse, target logit and loss of every token, the sum of the weights, the tokens that have arrived.
+int64_t vocab_loss_step_bytes(int64_t tokens, int64_t vocab, int32_t hidden)
+{
+    const int64_t n = vocab_loss_scratch_bytes(tokens, vocab, hidden, true);
+    return n < 0 ? -1 : (n + 255) / 256 * 256 + (3 * tokens + 2) * 4;
+}
 
-    memset(&P, 0, sizeof(P));
-    P.M = (int)c.vocab; P.N = c.hidden; P.cols = kMaxCols; P.split = 1;
-    P.total = total; P.scale = scale;
-    P.k_iters = (int)((c.tokens + BK - 1) / BK);
-    P.kind = out; P.out = (__nv_bfloat16 *)dw; P.sum = dw_sum;
-    CHK_RET(encode_2d(&P.tmA, s, c.tokens, l.width, BK, l.ld));
-    CHK_RET(encode_2d(&P.tmB, s + l.xc, c.tokens, c.hidden, BK, l.xld));
-    return launch_gemm(DW, c.vocab > BM, P, stream);
+HcclResult vocab_loss_step(const VocabLossCall &c, bool mean, float scale, float *loss, void *dx, void *dw, float *dw_sum, int out, void *scratch, void *stream)
+{
+    Layout l;
+    CHK_RET(layout_of(c.tokens, c.vocab, c.hidden, true, &l));
+    uint8_t *s = (uint8_t *)scratch;
+    float *words = (float *)(s + (std::max<int64_t>(1024, l.bytes) + 255) / 256 * 256), *total = words + 3 * c.tokens;
+    RowArgs a = row_args(c);
+    a.lse = words; a.target = words + c.tokens; a.losses = words + 2 * c.tokens;
+    a.arrived = (uint32_t *)total + 1; a.out = mean ? total : nullptr;
+    CHK_RET(scores(c, l, true, a.target, s, stream, &a));
+    a.out = loss; a.total = mean ? total : nullptr;
+    // one launch for rows and d where a CTA per token fills the GPU, or has little to do
+    if (c.tokens >= 1024 || l.width <= 8 * kDVecs)
+        CHK_RET(launch_pdl((const void *)vocab_loss_rows_d, dim3((unsigned)c.tokens), kDThreads, 0, &a, stream, "vocabulary loss (rows, d)"));
+    else {
+        CHK_RET(launch_pdl((const void *)vocab_loss_rows, dim3((unsigned)c.tokens), kRowThreads, 0, &a, stream, "vocabulary loss (rows)"));
+        CHK_RET(rows_to_d(c, l, a, stream));
+    }
+    return products(c, l, a.total, scale, dx, dw, dw_sum, out, s, stream);
 }
 
 }  // namespace hcclb

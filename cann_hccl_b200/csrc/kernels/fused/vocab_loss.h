@@ -33,4 +33,9 @@ enum VocabLossOut : int { VL_BF16 = 0, VL_F32 = 1, VL_ADD = 2, VL_ADD_BF16 = 3 }
 HcclResult vocab_loss_grad(const VocabLossCall &c, const float *lse, const float *target, const float *total, float scale, void *dx, void *dw, float *dw_sum,
                            int out, void *scratch, void *stream);
 
+// Loss and gradients of at most kVocabStepMost tokens against the whole vocabulary, in five to seven launches.
+constexpr int64_t kVocabStepMost = 65536;
+int64_t vocab_loss_step_bytes(int64_t tokens, int64_t vocab, int32_t hidden);
+HcclResult vocab_loss_step(const VocabLossCall &c, bool mean, float scale, float *loss, void *dx, void *dw, float *dw_sum, int out, void *scratch, void *stream);
+
 }  // namespace hcclb

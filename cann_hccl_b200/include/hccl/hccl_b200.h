@@ -176,6 +176,11 @@ extern HcclResult HcclB200VocabLossSum(const HcclB200VocabLoss *p, const float *
  * to dw as bf16 (dwSum is left as it was).  lse: joint; scratch: as HcclB200VocabLossScores left it for the same p, with withGrad. */
 extern HcclResult HcclB200VocabLossGrad(const HcclB200VocabLoss *p, const float *lse, const float *target, const float *total, float scale, void *dx,
                                         void *dw, float *dwSum, int32_t dwKind, void *scratch, aclrtStream stream);
+/* All of it in one call, for 1 to 65536 tokens (HcclB200VocabLossChunk() of them at most) against the whole vocabulary: *loss = sum(weights *
+ * losses), mean: divided by the sum of the weights that count; dx and dw as HcclB200VocabLossGrad leaves them. */
+extern int64_t HcclB200VocabLossStepBytes(int64_t tokens, int64_t vocab, int32_t hidden);
+extern HcclResult HcclB200VocabLossStep(const HcclB200VocabLoss *p, int32_t mean, float scale, float *loss, void *dx, void *dw, float *dwSum,
+                                        int32_t dwKind, void *scratch, aclrtStream stream);
 /* In-kernel timestamps of the newest executor launch (needs HCCL_KERNEL_TRACE=1 at communicator creation):
  * out[0] = kernel start (globaltimer ns), then per step {after wait, after data movement, after signal}. */
 extern HcclResult HcclB200GetKernelTrace(HcclComm comm, uint32_t localRank, uint64_t *out, size_t capWords, int32_t *nsteps);

@@ -207,6 +207,24 @@ def _run_loss(shards, comm, reduction, scale=1.0, outs=None, grad=False):
     return list(zip(losses, dxs, dws)) if grad else losses
 
 
+_STEP_MOST = 65536
+
+
+def _step(s, reduction, scale, dw):
+    """Loss and gradients of a lone shard whose tokens are one chunk: one call of the library."""
+    n = L.lib().HcclB200VocabLossStepBytes(s.T, s.V, s.H)
+    if n < 0:
+        raise RuntimeError("no scratch size for %d tokens, %d rows of %d" % (s.T, s.V, s.H))
+    mem, loss, dx = s.new(n, torch.uint8), s.new(()), s.new((s.T, s.H), torch.bfloat16)
+    out = s.new((s.V, s.H), torch.bfloat16) if dw is None else dw
+    at = out.data_ptr()
+    rc = L.lib().HcclB200VocabLossStep(s.part(0, s.T), int(reduction == "mean"), scale, loss.data_ptr(), dx.data_ptr(), at, at if dw is not None else None,
+                                       _BF16_OUT if dw is None else _ADD, mem.data_ptr(), _raw_stream())
+    if rc:
+        L.check(rc, "HcclB200VocabLossStep")
+    return loss, dx, out
+
+
 def linear_cross_entropy(x, w, targets, weights=None, reduction="mean", ignore_index=-100):
     """Softmax cross entropy of the logits x [tokens, hidden] @ w [vocab, hidden].T (bf16, fp32 sums) against `targets` (int32 or int64).
     Tokens whose target is ignore_index or no id of the vocabulary do not count.  `weights`: fp32 [tokens].  reduction: "none" gives
@@ -228,7 +246,10 @@ def linear_cross_entropy_grad(x, w, targets, weights=None, reduction="mean", ign
     if dw is not None:
         check_out(dw, w.shape, torch.float32, w.device)
     with on_device_of(x):
-        return _run_loss([_Shard(x, w, targets, weights, 0, w.shape[0], ignore_index)], None, reduction, scale, [dw], True)[0]
+        s = _Shard(x, w, targets, weights, 0, w.shape[0], ignore_index)
+        if 0 < s.T <= min(_STEP_MOST, L.lib().HcclB200VocabLossChunk(s.V, 1)):
+            return _step(s, reduction, scale, dw)
+        return _run_loss([s], None, reduction, scale, [dw], True)[0]
 
 
 def _sharded(comm, x, w, targets, weights, reduction, ignore_index):

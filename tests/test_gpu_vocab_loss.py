@@ -129,6 +129,26 @@ def test_gradients_at_the_end_of_the_vocabulary(V):
         Exact(x, w, y).check(vocab.linear_cross_entropy_grad(x, w, y))
 
 
+@pytest.mark.parametrize("T,V,hidden", [(40, 20001, 64), (1100, 9000, 64), (300, 500, 72), (1023, 9001, 40), (1024, 9001, 40)])
+def test_one_call_and_its_parts(T, V, hidden, monkeypatch):
+    """The whole step in one call, with rows and d in one launch and in two, gives what its parts give."""
+    x, w, y = problem(T, V, hidden)
+    weights = torch.rand(T, device="cuda")
+    weights[::3] = 0
+    for q, reduction in ((weights, "mean"), (None, "mean"), (weights, "sum")):
+        whole = vocab.linear_cross_entropy_grad(x, w, y, q, reduction)
+        monkeypatch.setattr(vocab, "_STEP_MOST", 0)
+        parts = vocab.linear_cross_entropy_grad(x, w, y, q, reduction)
+        monkeypatch.undo()
+        e = Exact(x, w, y, q, reduction)
+        e.check(whole)
+        e.check(parts)
+        # the same sums in another order
+        assert abs(float(whole[0]) - float(parts[0])) <= 2.0 ** -20 * abs(float(parts[0])) + 1e-30
+        for a, b in zip(whole[1:], parts[1:]):
+            assert float((a.float() - b.float()).norm()) <= 2.0 ** -8 * float(b.float().norm())
+
+
 def test_gradients_of_norm():
     """The errors are those of two roundings to bf16, not their bounds: 2-norm within one half step of the gradients'."""
     x, w, y = problem(700, 3000, 512)

@@ -78,6 +78,7 @@ def loss(entry="Scores", args=None, **bad):
     return {"Scores": lambda: lib.HcclB200VocabLossScores(p, 1, a["lse"], a["target"], a["losses"], a["scratch"], None),
             "Combine": lambda: lib.HcclB200VocabLossCombine(p, a["parts"], a["shards"], a["lse"], a["losses"], None),
             "Total": lambda: lib.HcclB200VocabLossTotal(p, a["total"], None),
+            "Step": lambda: lib.HcclB200VocabLossStep(p, 1, 1.0, a["loss"], a["dx"], a["dw"], a["sum"], a["kind"], a["scratch"], None),
             "Sum": lambda: lib.HcclB200VocabLossSum(p, a["losses"], a["total"], a["loss"], None),
             "Grad": lambda: lib.HcclB200VocabLossGrad(p, a["lse"], a["target"], a["total"], 1.0, a["dx"], a["dw"], a["sum"], a["kind"], a["scratch"], None)}[entry]()
 
@@ -85,7 +86,7 @@ def loss(entry="Scores", args=None, **bad):
 AT0 = (C.addressof(MEM) + 255) // 256 * 256
 
 
-@pytest.mark.parametrize("entry", ["Scores", "Grad"])
+@pytest.mark.parametrize("entry", ["Scores", "Grad", "Step"])
 @pytest.mark.parametrize("bad,want", [({"x": None}, "PTR"), ({"w": None}, "PTR"), ({"targets": None}, "PTR"), ({"targetType": L.FP32}, "NOT_SUPPORT"),
                                       ({"hidden": 12}, "PARA"), ({"hidden": 0}, "PARA"), ({"hidden": 16}, "PARA"), ({"xStride": 12}, "PARA"), ({"wStride": 0}, "PARA"),
                                       ({"vocab": 0}, "PARA"), ({"vocab": 17}, "PARA"), ({"firstId": 1}, "PARA"), ({"firstId": -1}, "PARA"), ({"wholeVocab": 15}, "PARA"),
@@ -98,14 +99,16 @@ def test_vocab_loss(entry, bad, want):
 def test_vocab_loss_outputs():
     assert loss("Scores", vocab=8) == L.E_PARA                              # a shard has no losses of its own
     for entry, names in (("Scores", ("lse", "target", "scratch")), ("Combine", ("parts", "lse", "losses")), ("Total", ("total",)), ("Sum", ("losses", "loss")),
-                         ("Grad", ("lse", "target", "dx", "dw", "scratch"))):
+                         ("Grad", ("lse", "target", "dx", "dw", "scratch")), ("Step", ("loss", "dx", "dw", "scratch"))):
         for n in names:
             assert loss(entry, {n: None}) == L.E_PTR and loss(entry, {n: AT0 + 2}) == L.E_PARA, (entry, n)
     assert loss("Grad", {"scratch": AT0 + 128}) == L.E_PARA and loss("Combine", {"shards": 0}) == L.E_PARA and loss("Grad", tokens=0) == L.E_PARA
     assert loss("Grad", {"kind": 4}) == L.E_PARA and loss("Grad", {"kind": -1}) == L.E_PARA
-    for kind in (1, 2, 3):
-        assert loss("Grad", {"kind": kind, "sum": None}) == L.E_PTR
-    assert loss("Grad", {"kind": 3, "dw": None}) == L.E_PTR
+    assert loss("Step", tokens=65537) == L.E_PARA and loss("Step", vocab=8) == L.E_PARA and loss("Step", tokens=0) == L.E_PARA
+    for entry in ("Grad", "Step"):
+        for kind in (1, 2, 3):
+            assert loss(entry, {"kind": kind, "sum": None}) == L.E_PTR
+        assert loss(entry, {"kind": 3, "dw": None}) == L.E_PTR and loss(entry, {"kind": 4}) == L.E_PARA and loss(entry, {"scratch": AT0 + 128}) == L.E_PARA
     assert loss("Scores", tokens=0, x=None, targets=None) == L.SUCCESS and loss("Combine", tokens=0, targets=None) == L.SUCCESS
     lib = L.lib()
     assert lib.HcclB200VocabLossScores(None, 0, AT, AT, None, AT0, None) == L.E_PTR
@@ -113,6 +116,7 @@ def test_vocab_loss_outputs():
     for vocab in (1, 1000, 128256, 1 << 24):
         for grad in (0, 1):
             assert lib.HcclB200VocabLossChunk(vocab, grad) >= 256 and lib.HcclB200VocabLossChunk(vocab, grad) % 256 == 0
+    assert lib.HcclB200VocabLossStepBytes(0, 16, 8) == -1 and lib.HcclB200VocabLossStepBytes(65537, 16, 8) == -1 and lib.HcclB200VocabLossStepBytes(4, 16, 12) == -1
     assert lib.HcclB200VocabLossScratchBytes(4, 16, 12, 1) == -1 and lib.HcclB200VocabLossScratchBytes((1 << 20) + 1, 16, 8, 1) == -1
 
 
