@@ -369,7 +369,7 @@ struct SumArgs {
     int64_t tokens, vocab, stride;   // stride: bytes between rows of dy
     const uint32_t *has;             // bits of the rows with a token (null: none has one)
     int64_t tiles;
-    int rows, nvec, nslice, add, wide, zero_rows;  // wide: rows of an fp32 out that is added to are whole 32-byte sectors     // rows: tokens of a tile
+    int rows, nvec, nslice, add, wide, zero_rows;  // rows: tokens of a tile; wide: rows of an fp32 out that is added to are whole sectors
     float scale;
 };
 constexpr int kSumThreads = 256, kSumBatch = 4, kMostRows = 256;

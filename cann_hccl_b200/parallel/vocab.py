@@ -229,7 +229,9 @@ def linear_cross_entropy(x, w, targets, weights=None, reduction="mean", ignore_i
     """Softmax cross entropy of the logits x [tokens, hidden] @ w [vocab, hidden].T (bf16, fp32 sums) against `targets` (int32 or int64).
     Tokens whose target is ignore_index or no id of the vocabulary do not count.  `weights`: fp32 [tokens].  reduction: "none" gives
     the unweighted losses [tokens] (0 where a token does not count), "sum" their weighted sum, "mean" that divided by the sum of the
-    weights that count (0 where there is none).  The logits are not stored: beyond the arguments it takes about 130 MB at most (for 256 tokens at least)."""
+    weights that count (0 where there is none).  The logits are not stored: beyond the arguments it takes about 130 MB at most (for 256 tokens at least).
+    The tensor cores' fp32 sums lean towards zero: losses come out low by a few 1e-6 of themselves at hidden 4096 (means of 256 tokens:
+    6e-7 at a loss of 10, 7e-6 at 0.1), growing with hidden."""
     _check_loss(x, w, targets, weights, reduction)
     with on_device_of(x):
         return _run_loss([_Shard(x, w, targets, weights, 0, w.shape[0], ignore_index)], None, reduction)[0]
