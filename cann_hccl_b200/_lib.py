@@ -92,7 +92,7 @@ class MoeLayer(C.Structure):
 
 class VocabLoss(C.Structure):
     _fields_ = [("x", C.c_void_p), ("w", C.c_void_p), ("xStride", C.c_int64), ("wStride", C.c_int64), ("targets", C.c_void_p), ("weights", C.c_void_p)] + \
-               [(n, C.c_int64) for n in ("tokens", "vocab", "firstId", "wholeVocab", "ignoreId")] + [("hidden", C.c_int32), ("targetType", C.c_int32)]
+               [(n, C.c_int64) for n in ("tokens", "vocab", "firstId", "wholeVocab", "ignoreId")] + [("hidden", C.c_int32), ("targetType", C.c_int32), ("scratchBytes", C.c_int64)]
 
 
 _lib = None
@@ -244,7 +244,9 @@ def lib():
     L.HcclB200MoeGateScratchBytes.argtypes = [C.c_int64, i32]
     L.HcclB200VocabLossChunk.argtypes = [C.c_int64, i32]
     L.HcclB200VocabLossScratchBytes.argtypes = [C.c_int64, C.c_int64, i32, i32]
+    L.HcclB200VocabLossScratchBytesOn.argtypes = [i32, i32, C.c_int64, C.c_int64, i32, i32]
     L.HcclB200VocabLossStepBytes.argtypes = [C.c_int64, C.c_int64, i32]
+    L.HcclB200VocabLossScratchBytesOn.restype = C.c_int64
     L.HcclB200VocabLossChunk.restype = L.HcclB200VocabLossScratchBytes.restype = L.HcclB200VocabLossStepBytes.restype = C.c_int64
     L.HcclB200EmbeddingGradScratchBytes.restype = L.HcclB200MoeGateScratchBytes.restype = C.c_int64
     L.HcclGetErrorString.argtypes = [C.c_int]

@@ -879,6 +879,7 @@ static HcclResult check_vocab_loss(const HcclB200VocabLoss *p, bool targets, std
         CHK_RET_LOG(p->tokens > (1 << 20), HCCL_E_PARA, "%s: %lld tokens are more than a chunk", api, (long long)p->tokens);
         CHK_RET_LOG(p->xStride < p->hidden || p->wStride < p->hidden || p->xStride % 8 || p->wStride % 8, HCCL_E_PARA, "%s: strides %lld, %lld of rows of %d", api,
                     (long long)p->xStride, (long long)p->wStride, p->hidden);
+        CHK_RET_LOG(p->scratchBytes < 0, HCCL_E_PARA, "%s: scratch of %lld bytes", api, (long long)p->scratchBytes);
         null = null || !p->w || (p->tokens > 0 && !p->x);
     }
     CHK_RET_LOG(null, HCCL_E_PTR, "[EI0003] %s: null pointer", api);
@@ -887,14 +888,21 @@ static HcclResult check_vocab_loss(const HcclB200VocabLoss *p, bool targets, std
     CHK_RET(check_aligned({p->weights}, 4, api));
     CHK_RET(check_aligned(words, 4, api));
     *c = VocabLossCall{p->x, p->w, p->xStride, p->wStride, p->targets, p->targetType == HCCL_DATA_TYPE_INT64, p->weights, p->tokens, p->vocab, p->firstId,
-                       p->wholeVocab, p->ignoreId, p->hidden};
+                       p->wholeVocab, p->ignoreId, p->hidden, p->scratchBytes};
     return HCCL_SUCCESS;
 }
 int64_t HcclB200VocabLossChunk(int64_t vocab, int32_t withGrad) { return vocab < 1 || vocab >= INT32_MAX - 256 ? -1 : vocab_loss_chunk(vocab, withGrad != 0); }
+static bool loss_size(int64_t tokens, int64_t vocab, int32_t hidden)
+{
+    return tokens >= 0 && tokens <= (1 << 20) && vocab >= 1 && vocab < INT32_MAX - 256 && hidden >= 8 && hidden % 8 == 0;
+}
 int64_t HcclB200VocabLossScratchBytes(int64_t tokens, int64_t vocab, int32_t hidden, int32_t withGrad)
 {
-    return tokens < 0 || tokens > (1 << 20) || vocab < 1 || vocab >= INT32_MAX - 256 || hidden < 8 || hidden % 8 ? -1
-           : vocab_loss_scratch_bytes(tokens, vocab, hidden, withGrad != 0);
+    return loss_size(tokens, vocab, hidden) ? vocab_loss_scratch_bytes(tokens, vocab, hidden, withGrad != 0) : -1;
+}
+int64_t HcclB200VocabLossScratchBytesOn(int32_t sms, int32_t pairs, int64_t tokens, int64_t vocab, int32_t hidden, int32_t withGrad)
+{
+    return loss_size(tokens, vocab, hidden) && sms > 0 && pairs > 0 ? vocab_loss_scratch_bytes_on(sms, pairs, tokens, vocab, hidden, withGrad != 0) : -1;
 }
 HcclResult HcclB200VocabLossScores(const HcclB200VocabLoss *p, int32_t withGrad, float *lse, float *target, float *losses, void *scratch, aclrtStream stream)
 {

@@ -887,10 +887,9 @@ int shares_of(int64_t tokens, int64_t vocab, int32_t hidden, const LossDevice &d
     return std::max(1, best);
 }
 
-HcclResult layout_of(int64_t tokens, int64_t vocab, int32_t hidden, bool grad, Layout *l)
+// Fewer tokens may need more scratch: their dx is cut into more shares, and their tiles may be narrower.
+void layout_on(const LossDevice &d, int64_t tokens, int64_t vocab, int32_t hidden, bool grad, Layout *l)
 {
-    LossDevice d;
-    CHK_RET(loss_device(&d));
     auto up = [](int64_t n) { return (n + 1023) / 1024 * 1024; };
     l->pair = tokens > BM;
     l->cols = score_cols((tokens + (l->pair ? 255 : 127)) / (l->pair ? 256 : 128), vocab, l->pair, l->pair ? d.pairs : d.sms);
@@ -905,7 +904,22 @@ HcclResult layout_of(int64_t tokens, int64_t vocab, int32_t hidden, bool grad, L
     // one, which bounds the product (1531 x 50257 x 1000: scores 150 us, DW 127): more than one row of tiles is worth the copy.
     l->copy = grad || (hidden % 64 != 0 && l->pair);
     l->shares = l->xc + (l->copy ? up(tokens * l->xld * 2) : 0);
-    l->bytes = l->shares + (l->split > 1 ? up((int64_t)l->split * tokens * hidden * 4) : 0);
+    l->bytes = std::max<int64_t>(1024, l->shares + (l->split > 1 ? up((int64_t)l->split * tokens * hidden * 4) : 0));
+}
+
+HcclResult layout_of(int64_t tokens, int64_t vocab, int32_t hidden, bool grad, Layout *l)
+{
+    LossDevice d;
+    CHK_RET(loss_device(&d));
+    layout_on(d, tokens, vocab, hidden, grad, l);
+    return HCCL_SUCCESS;
+}
+
+// The caller's scratch has the bytes that the call is about to use.
+HcclResult check_scratch(const VocabLossCall &c, int64_t bytes)
+{
+    CHK_RET_LOG(c.scratch_bytes && c.scratch_bytes < bytes, HCCL_E_PARA, "vocabulary loss: scratch of %lld bytes, %lld tokens need %lld", (long long)c.scratch_bytes,
+                (long long)c.tokens, (long long)bytes);
     return HCCL_SUCCESS;
 }
 
@@ -954,7 +968,16 @@ int64_t vocab_loss_chunk(int64_t vocab, bool grad)
 int64_t vocab_loss_scratch_bytes(int64_t tokens, int64_t vocab, int32_t hidden, bool grad)
 {
     Layout l;
-    return layout_of(tokens, vocab, hidden, grad, &l) == HCCL_SUCCESS ? std::max<int64_t>(1024, l.bytes) : -1;
+    return layout_of(tokens, vocab, hidden, grad, &l) == HCCL_SUCCESS ? l.bytes : -1;
+}
+
+int64_t vocab_loss_scratch_bytes_on(int sms, int pairs, int64_t tokens, int64_t vocab, int32_t hidden, bool grad)
+{
+    LossDevice d;
+    d.sms = sms; d.pairs = pairs;
+    Layout l;
+    layout_on(d, tokens, vocab, hidden, grad, &l);
+    return l.bytes;
 }
 
 namespace {
@@ -1035,6 +1058,7 @@ HcclResult vocab_loss_scores(const VocabLossCall &c, bool grad, float *lse, floa
 {
     Layout l;
     CHK_RET(layout_of(c.tokens, c.vocab, c.hidden, grad, &l));
+    CHK_RET(check_scratch(c, l.bytes));
     RowArgs a = row_args(c);
     CHK_RET(scores(c, l, grad, target, (uint8_t *)scratch, stream, &a));
     a.lse = lse; a.target = target; a.losses = losses;
@@ -1067,6 +1091,7 @@ HcclResult vocab_loss_grad(const VocabLossCall &c, const float *lse, const float
 {
     Layout l;
     CHK_RET(layout_of(c.tokens, c.vocab, c.hidden, true, &l));
+    CHK_RET(check_scratch(c, l.bytes));
     uint8_t *s = (uint8_t *)scratch;
     RowArgs a = row_args(c);
     a.stats = (const float2 *)(s + l.stats); a.halves = 2 * l.n_tiles; a.cols = l.cols;
@@ -1076,18 +1101,21 @@ HcclResult vocab_loss_grad(const VocabLossCall &c, const float *lse, const float
 }
 
 // Behind the scratch of its parts: lse, target logit and loss of every token, the sum of the weights, the tokens that have arrived.
+static int64_t step_bytes(int64_t parts, int64_t tokens) { return (parts + 255) / 256 * 256 + (3 * tokens + 2) * 4; }
+
 int64_t vocab_loss_step_bytes(int64_t tokens, int64_t vocab, int32_t hidden)
 {
     const int64_t n = vocab_loss_scratch_bytes(tokens, vocab, hidden, true);
-    return n < 0 ? -1 : (n + 255) / 256 * 256 + (3 * tokens + 2) * 4;
+    return n < 0 ? -1 : step_bytes(n, tokens);
 }
 
 HcclResult vocab_loss_step(const VocabLossCall &c, bool mean, float scale, float *loss, void *dx, void *dw, float *dw_sum, int out, void *scratch, void *stream)
 {
     Layout l;
     CHK_RET(layout_of(c.tokens, c.vocab, c.hidden, true, &l));
+    CHK_RET(check_scratch(c, step_bytes(l.bytes, c.tokens)));
     uint8_t *s = (uint8_t *)scratch;
-    float *words = (float *)(s + (std::max<int64_t>(1024, l.bytes) + 255) / 256 * 256), *total = words + 3 * c.tokens;
+    float *words = (float *)(s + (l.bytes + 255) / 256 * 256), *total = words + 3 * c.tokens;
     RowArgs a = row_args(c);
     a.lse = words; a.target = words + c.tokens; a.losses = words + 2 * c.tokens;
     a.arrived = (uint32_t *)total + 1; a.out = mean ? total : nullptr;

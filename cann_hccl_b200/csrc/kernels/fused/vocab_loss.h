@@ -13,10 +13,14 @@ struct VocabLossCall {
     const float *weights;            // of the tokens; null: ones
     int64_t tokens, vocab, first, whole, ignore;  // first id of the shard, ids of all shards, target of tokens that do not count
     int32_t hidden;
+    int64_t scratch_bytes;           // at the call's scratch; 0: not stated
 };
 // Tokens whose exponentials fit the scratch of a call with gradients, or whose sums fit that of one without.
 int64_t vocab_loss_chunk(int64_t vocab, bool grad);
+// Scratch of a call of exactly `tokens`; a call of fewer may need more.
 int64_t vocab_loss_scratch_bytes(int64_t tokens, int64_t vocab, int32_t hidden, bool grad);
+// The same where a device has `sms` multiprocessors and runs `pairs` clusters of two CTAs at once.
+int64_t vocab_loss_scratch_bytes_on(int sms, int pairs, int64_t tokens, int64_t vocab, int32_t hidden, bool grad);
 // lse and target logit (-inf where another shard has it) of every token against this shard; losses (may be null) for a lone shard.
 // grad: the exponentials stay in scratch for vocab_loss_grad.
 HcclResult vocab_loss_scores(const VocabLossCall &c, bool grad, float *lse, float *target, float *losses, void *scratch, void *stream);

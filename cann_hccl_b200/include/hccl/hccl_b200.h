@@ -157,9 +157,14 @@ typedef struct HcclB200VocabLossDef {
     const float *weights;                    /* of the tokens; NULL: ones */
     int64_t tokens, vocab, firstId, wholeVocab, ignoreId;
     int32_t hidden, targetType;
+    int64_t scratchBytes;                    /* at the scratch of Scores, Grad and Step, which refuse too few; 0: not stated, not looked at */
 } HcclB200VocabLoss;
 extern int64_t HcclB200VocabLossChunk(int64_t vocab, int32_t withGrad);
+/* Scratch of a call of exactly `tokens`.  Fewer tokens may need MORE (their dx is cut into more shares): scratch that serves several calls
+ * is the largest of theirs.  ...On: the same for a device of `sms` multiprocessors that runs `pairs` clusters of two CTAs at once, without
+ * asking the current one. */
 extern int64_t HcclB200VocabLossScratchBytes(int64_t tokens, int64_t vocab, int32_t hidden, int32_t withGrad);
+extern int64_t HcclB200VocabLossScratchBytesOn(int32_t sms, int32_t pairs, int64_t tokens, int64_t vocab, int32_t hidden, int32_t withGrad);
 /* lse [tokens] and target [tokens] (the target's logit, -inf where another shard has it) against this shard; losses [tokens] (0 for
  * tokens that do not count) where the shard is the whole vocabulary, else NULL.  withGrad: scratch then holds what
  * HcclB200VocabLossGrad needs, and tokens of weight 0 have a loss of 0 (their rows of x are not looked at). */

@@ -148,6 +148,10 @@ class _Shard:
             c.weights = self._q + a * 4
         return C.byref(c)
 
+    def scratch(self, n):
+        """Bytes of the scratch that the calls of part() are given."""
+        self._call.scratchBytes = n
+
     def new(self, shape, dtype=torch.float32):
         return self.x.new_empty(shape, dtype=dtype)
 
@@ -158,13 +162,15 @@ def _run_loss(shards, comm, reduction, scale=1.0, outs=None, grad=False):
     T, alone, none = s0.T, comm is None or comm.nranks == 1, reduction == "none"
     chunk = min(max(T, 1), min(lib.HcclB200VocabLossChunk(s.V, int(grad)) for s in shards))
     losses = [s.new(T) for s in shards]
+    sizes = {min(chunk, T), T % chunk}  # tokens of the chunks: a short last one may need more scratch than a whole one
     # fp32 words of each shard behind its scratch: lse and target logit of a chunk, the joint lse, the sum of the weights
     mem, words = [], []
     for s in shards:
-        n = lib.HcclB200VocabLossScratchBytes(chunk if T else 0, s.V, s.H, int(grad))
-        if n < 0:
+        needs = [lib.HcclB200VocabLossScratchBytes(n, s.V, s.H, int(grad)) for n in sizes]
+        if min(needs) < 0:
             raise RuntimeError("no scratch size for %d tokens, %d rows of %d" % (chunk, s.V, s.H))
-        n = (n + 255) // 256 * 256
+        n = (max(needs) + 255) // 256 * 256
+        s.scratch(n)
         m = s.new(n + (3 * chunk + 1) * 4, torch.uint8)
         mem.append(m)
         words.append(m.data_ptr() + n)
@@ -215,6 +221,7 @@ def _step(s, reduction, scale, dw):
     n = L.lib().HcclB200VocabLossStepBytes(s.T, s.V, s.H)
     if n < 0:
         raise RuntimeError("no scratch size for %d tokens, %d rows of %d" % (s.T, s.V, s.H))
+    s.scratch(n)
     mem, loss, dx = s.new(n, torch.uint8), s.new(()), s.new((s.T, s.H), torch.bfloat16)
     out = s.new((s.V, s.H), torch.bfloat16) if dw is None else dw
     at = out.data_ptr()
