@@ -52,9 +52,9 @@ class Calls:
         rows = C.cast(C.c_void_p(rows), C.POINTER(C.c_void_p)) if rows else None
         return self._lib.HcclB200MoeCombineLocal(comm, _layer(layer), rows, *at, stream)
 
-    # model-side operators: tensors by their addresses, everything else as it is
-    def _model(self, fn, a, tensors):
-        return fn(*[data_ptr(x) if i in tensors and not isinstance(x, int) else x for i, x in enumerate(a)])
+    # model-side operators: tensors and, of the router's results, parts by their addresses, everything else as it is
+    def _model(self, fn, a, tensors, parts=()):
+        return fn(*[data_ptr(x) if i in tensors or i in parts and not isinstance(x, int) else x for i, x in enumerate(a)])
 
     def embedding(self, *a):
         return self._model(self._lib.HcclB200Embedding, a, (0, 3, 10))
@@ -63,7 +63,7 @@ class Calls:
         return self._model(self._lib.HcclB200EmbeddingGrad, a, (0, 3, 10, 13))
 
     def gate(self, *a):
-        return self._model(self._lib.HcclB200MoeGate, a, (0, *range(7, 15)))
+        return self._model(self._lib.HcclB200MoeGate, a, (0, 7, 14), range(8, 14))
 
     def gate_grad(self, *a):
-        return self._model(self._lib.HcclB200MoeGateGrad, a, (0, 7, 8, 9, 10, 11, 13))
+        return self._model(self._lib.HcclB200MoeGateGrad, a, (0, 7, 9, 13), (8, 10, 11))

@@ -19,14 +19,10 @@ static combine_fn g_combine;
 static PyObject *s_data_ptr, *s_ctypes, *s_data, *s_numel, *s_size, *s_dtype;
 static PyObject *g_dtypes, *g_get_device, *g_get_stream;  /* {torch / numpy dtype: HcclDataType}, current device, its current raw stream */
 
-/* address of a tensor (data_ptr()) or numpy array (ctypes.data), or an integer that is one; None is null */
+/* address of a tensor (data_ptr()) or numpy array (ctypes.data); None is null, anything else, an integer too, is refused */
 static int address(PyObject *x, void **out)
 {
     if (x == Py_None) { *out = NULL; return 0; }
-    if (PyLong_CheckExact(x)) {
-        *out = PyLong_AsVoidPtr(x);
-        return *out == NULL && PyErr_Occurred() ? -1 : 0;
-    }
     PyObject *v = PyObject_CallMethodNoArgs(x, s_data_ptr);
     if (!v) {
         if (!PyErr_ExceptionMatches(PyExc_AttributeError)) return -1;
@@ -254,6 +250,15 @@ static PyObject *moe_combine(PyObject *self, PyObject *const *a, Py_ssize_t n)
 }
 
 /* ---- model-side operators.  Integers and floats are taken as they come, tensors by their addresses (None: null) ---- */
+
+/* a part of a router's results: a tensor, or the address where the Python layer has put it without making one */
+static int part_address(PyObject *x, void **out)
+{
+    if (!PyLong_CheckExact(x)) return address(x, out);
+    *out = PyLong_AsVoidPtr(x);
+    return *out == NULL && PyErr_Occurred() ? -1 : 0;
+}
+
 typedef HcclResult (*embedding_fn)(const void *, HcclDataType, int64_t, const void *, int64_t, int64_t, int64_t, int32_t, HcclDataType, float, void *, aclrtStream);
 typedef HcclResult (*embedding_grad_fn)(const void *, HcclDataType, int64_t, const void *, int64_t, int64_t, int64_t, int32_t, HcclDataType, float, void *, HcclDataType,
                                         int32_t, void *, aclrtStream);
@@ -322,8 +327,8 @@ static PyObject *gate(PyObject *self, PyObject *const *a, Py_ssize_t n)
     const int64_t tokens = PyLong_AsLongLong(a[2]), stride = PyLong_AsLongLong(a[4]);
     const int32_t experts = (int32_t)PyLong_AsLong(a[3]), topk = (int32_t)PyLong_AsLong(a[5]), normalize = (int32_t)PyLong_AsLong(a[6]);
     if (PyErr_Occurred()) return NULL;
-    for (int i = 0; i < 9; ++i)
-        if (address(a[from[i]], &at[i])) return NULL;
+    for (int i = 0; i < 9; ++i)  /* idx, gates, counts, prob_sum, routed, balance are parts */
+        if ((i >= 2 && i <= 7 ? part_address : address)(a[from[i]], &at[i])) return NULL;
     HcclResult rc;
     Py_BEGIN_ALLOW_THREADS
     rc = g_gate(at[0], (HcclDataType)t, tokens, experts, stride, topk, normalize, at[1], at[2], at[3], at[4], at[5], at[6], at[7], at[8], (aclrtStream)stream);
@@ -342,8 +347,8 @@ static PyObject *gate_grad(PyObject *self, PyObject *const *a, Py_ssize_t n)
     const int32_t experts = (int32_t)PyLong_AsLong(a[3]), topk = (int32_t)PyLong_AsLong(a[5]), normalize = (int32_t)PyLong_AsLong(a[6]);
     const float coef = (float)PyFloat_AsDouble(a[12]);
     if (PyErr_Occurred()) return NULL;
-    for (int i = 0; i < 7; ++i)
-        if (address(a[from[i]], &at[i])) return NULL;
+    for (int i = 0; i < 7; ++i)  /* idx, counts, routed are parts */
+        if ((i == 2 || i == 4 || i == 5 ? part_address : address)(a[from[i]], &at[i])) return NULL;
     HcclResult rc;
     Py_BEGIN_ALLOW_THREADS
     rc = g_gate_grad(at[0], (HcclDataType)t, tokens, experts, stride, topk, normalize, at[1], at[2], at[3], at[4], at[5], coef, at[6], (aclrtStream)stream);
