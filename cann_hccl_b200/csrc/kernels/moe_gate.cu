@@ -22,6 +22,7 @@
 #include "common/log.h"
 #include "kernels/moe_gate.h"
 #include "kernels/pdl.cuh"
+#include "kernels/smem_grant.h"
 
 namespace hcclb {
 
@@ -413,16 +414,17 @@ GateGrid gate_grid(int64_t tokens, int experts, bool grad)
     return {threads, (int)std::min<int64_t>(grad ? 148 * 4 : kMaxBlocks, (tokens + warps - 1) / warps)};
 }
 
+// Dynamic shared memory of a CTA: a row of the experts for each warp and one more, `keys` words of a warp.
+constexpr size_t gate_smem(int threads, int experts, int keys) { return ((size_t)(threads / 32) * (keys + experts) + experts) * 4; }
+template <int V> constexpr int kGradMost = kGateMost<V> < kGradThreads ? kGateMost<V> : kGradThreads;
+static_assert(gate_smem(kGateMost<128>, 4096, 4096) <= 220 * 1024 && gate_smem(kGateMost<32>, 1024, 1024) <= 220 * 1024, "beside what the kernel has of its own");
+
 template <class T, int V> HcclResult run_gate(GateArgs &a, bool grad, void *stream)
 {
     const GateGrid g = gate_grid(a.tokens, a.experts, grad);
-    const int W = g.threads / 32;
-    const size_t smem = grad ? (size_t)(W + 1) * a.experts * 4 : (size_t)W * V * 128 + (size_t)(W + 1) * a.experts * 4;
+    const size_t smem = gate_smem(g.threads, a.experts, grad ? 0 : V * 32);
     const void *fn = grad ? (const void *)moe_gate_grad_kernel<T, V> : (const void *)moe_gate_kernel<T, V>;
-    if (smem > 32 * 1024) {  // with what the kernel has of its own, more than 48 KB needs leave
-        const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        CHK_RET_LOG(e != cudaSuccess, HCCL_E_RUNTIME, "router set-up failed: %s", cudaGetErrorString(e));
-    }
+    if (smem > 32 * 1024) CHK_RET(grant_smem(fn, grad ? gate_smem(kGradMost<V>, V * 32, 0) : gate_smem(kGateMost<V>, V * 32, V * 32), "router"));
     return launch_pdl(fn, dim3((unsigned)g.ctas), (unsigned)g.threads, smem, &a, stream, grad ? "router gradient" : "router");
 }
 

@@ -18,6 +18,7 @@
 #include "common/base.h"
 #include "common/log.h"
 #include "kernels/pdl.cuh"
+#include "kernels/smem_grant.h"
 #include "kernels/vocab_embed.h"
 
 namespace hcclb {
@@ -627,10 +628,7 @@ template <int THREADS> HcclResult sort_tiles(SortArgs &a, uint2 *const (&buf)[2]
 {
     a.tiles = (int)((a.tokens + THREADS * kSortItems - 1) / (THREADS * kSortItems));
     const void *scatter = (const void *)embed_sort_scatter_kernel<THREADS>;
-    if (kScatterSmem<THREADS> > 32 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(scatter, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kScatterSmem<THREADS>);
-        CHK_RET_LOG(e != cudaSuccess, HCCL_E_RUNTIME, "embedding gradient set-up failed: %s", cudaGetErrorString(e));
-    }
+    if (kScatterSmem<THREADS> > 32 * 1024) CHK_RET(grant_smem(scatter, kScatterSmem<THREADS>, "embedding gradient"));
     for (int pass = 0; pass < a.passes; ++pass) {
         a.in = pass ? buf[(pass - 1) & 1] : nullptr;
         a.out = buf[pass & 1];
@@ -659,10 +657,7 @@ HcclResult sort_tokens(const EmbedTable &t, const EmbedIds &ids, const Scratch &
         *sorted = buf[0];
         a.tiles = (int)((ids.tokens + kCountTokens - 1) / kCountTokens);
         const size_t smem = (size_t)(ids.tokens + 3) / 4 * 16 + (has ? kWindow / 8 : 0);
-        if (smem > 32 * 1024) {  // with what the kernel has of its own, more than 48 KB needs leave
-            const cudaError_t e = cudaFuncSetAttribute((const void *)embed_sort_count_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-            CHK_RET_LOG(e != cudaSuccess, HCCL_E_RUNTIME, "embedding gradient set-up failed: %s", cudaGetErrorString(e));
-        }
+        if (smem > 32 * 1024) CHK_RET(grant_smem((const void *)embed_sort_count_kernel, kCountMost * 4 + kWindow / 8, "embedding gradient"));
         const int64_t windows = has ? (t.vocab + kWindow - 1) / kWindow : 0;
         return launch_pdl((const void *)embed_sort_count_kernel, dim3((unsigned)(a.tiles + windows)), kCountThreads, smem, &a, stream, "embedding gradient (sort)");
     }
