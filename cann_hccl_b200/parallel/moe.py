@@ -11,7 +11,7 @@ The router in front of it, with the balance loss and the gradients of both:
     g = gate(logits, topk, mask=None)                                    # Gate(idx, gates, counts, prob_sum, routed, balance)
     recv, expert_offsets, recv_rows = ex.dispatch(x, g.idx)              # slots without an expert (-1) are skipped
     ...
-    d_logits = gate_grad(logits, g, d_gates, balance=coefficient)
+    d_logits = gate_grad(logits, g, d_gates, balance=coefficient)        # of the routed tokens: g has the mask
 
 Counts travel over the device (all-gather of the per-expert histogram); nothing synchronises with the host.  On an
 all-local communicator every tensor argument is a list with one entry per virtual rank.
@@ -170,25 +170,32 @@ class _Part:
         return t
 
 
+def _writes(t):
+    """Number of writes that torch has counted on a tensor."""
+    return None if t.is_inference() else t._version
+
+
 class Gate:
     """What gate() returns: tensors idx, gates, counts, prob_sum, routed, balance (in this order when it is iterated over).  gate() keeps
     them in one piece of memory and makes a tensor of a part when it is asked for: six allocations cost a decode step more than the
-    kernel does."""
+    kernel does.  Besides these it has the call's `mask` (the tensor itself, no copy) and `normalize`, which gate_grad() goes by."""
     _FIELDS = ("idx", "gates", "counts", "prob_sum", "routed", "balance")
     idx, gates, counts, prob_sum, routed, balance = (_Part(i, n in ("gates", "prob_sum", "balance")) for i, n in enumerate(_FIELDS))
 
-    def __init__(self, idx, gates, counts, prob_sum, routed, balance):
-        self.__dict__.update(zip(self._FIELDS, (idx, gates, counts, prob_sum, routed, balance)), _words=None)
+    def __init__(self, idx, gates, counts, prob_sum, routed, balance, mask=None, normalize=True):
+        self.__dict__.update(zip(self._FIELDS, (idx, gates, counts, prob_sum, routed, balance)), _words=None, mask=mask, normalize=normalize,
+                             _written=None if mask is None else _writes(mask))
 
     def __setattr__(self, name, value):
         raise AttributeError("the parts of a Gate may be written to, not replaced: make a Gate of the tensors")
 
     @classmethod
-    def _empty(cls, like, T, k, E):
+    def _empty(cls, like, T, k, E, mask, normalize):
         g = object.__new__(cls)
         n, e = (T * k + 3) // 4 * 4, (E + 3) // 4 * 4
         g.__dict__.update(_T=T, _k=k, _E=E, _at=(0, n, 2 * n, 2 * n + e, 2 * n + 2 * e, 2 * n + 2 * e + 1),
-                          _words=like.new_empty(2 * n + 2 * e + 2, dtype=torch.int32))
+                          _words=like.new_empty(2 * n + 2 * e + 2, dtype=torch.int32), mask=mask, normalize=normalize,
+                          _written=None if mask is None else _writes(mask))
         return g
 
     def __iter__(self):
@@ -232,8 +239,8 @@ def gate(logits, topk, mask=None, normalize=True, comm=None):
     counts    int32 [experts], prob_sum fp32 [experts], routed int32 []: pairs, sums of probabilities and number of the routed tokens
     balance   fp32 []: experts / (topk * routed^2) * sum(counts * prob_sum), 1 for an even load
 
-    The sums have a fixed order: the same inputs give the same bits.  With `comm` the three sums, and so the loss, are those of all
-    ranks' tokens (on an all-local communicator logits and mask are lists with one tensor per rank, and a list of Gates returns)."""
+    The Gate has mask and normalize as well, for gate_grad().  The sums have a fixed order: the same inputs give the same bits.  With
+    `comm` the three sums, and so the loss, are those of all ranks' tokens (on an all-local communicator logits and mask are lists with one tensor per rank, and a list of Gates returns)."""
     if comm is not None:
         ls = list(logits) if isinstance(logits, (list, tuple)) else [logits]
         ms = list(mask) if isinstance(mask, (list, tuple)) else [mask] * len(ls)
@@ -251,7 +258,7 @@ def gate(logits, topk, mask=None, normalize=True, comm=None):
         return gs if isinstance(logits, (list, tuple)) else gs[0]
     T, E, stride, code = _check_gate(logits, topk, mask)
     with on_device_of(logits):
-        g = Gate._empty(logits, T, topk, E)
+        g = Gate._empty(logits, T, topk, E, mask, normalize)
         n = L.lib().HcclB200MoeGateScratchBytes(T, E)
         scratch = logits.new_empty(n, dtype=torch.uint8) if n > 0 else None
         rc = L.fast.gate(logits, code, T, E, stride, topk, int(normalize), mask, *g._addresses(0, 1, 2, 3, 4, 5), scratch, _raw_stream())
@@ -260,12 +267,19 @@ def gate(logits, topk, mask=None, normalize=True, comm=None):
     return g
 
 
-def gate_grad(logits, g, d_gates=None, balance=0.0, mask=None, normalize=True, out=None):
+def gate_grad(logits, g, d_gates=None, balance=0.0, mask=None, normalize=None, out=None):
     """Gradient of the logits: `d_gates` (fp32 [tokens, topk] or None) is the gates' gradient, the number `balance` that of the balance
-    loss.  logits, mask and normalize are those of the gate() call that returned `g`; counts are constants of the loss.  A slot with
-    expert -1 passes nothing on, rows that are not routed get zeros."""
+    loss.  logits are those of the gate() call that returned `g`, and so are mask and normalize where they are not given; counts are constants
+    of the loss.  A slot with expert -1 passes nothing on, rows that are not routed get zeros.  A mask that torch has seen written to since
+    gate() is refused: give the one that gate() had."""
     if not isinstance(g, Gate):
         raise TypeError("g must be what gate() returned for these logits")
+    if mask is None and g.mask is not None:
+        mask = g.mask
+        if _writes(mask) != g._written:
+            raise RuntimeError("the mask has been written to since gate()")
+    if normalize is None:
+        normalize = g.normalize
     if g._words is not None:
         shape, experts, device = (g._T, g._k), (g._E,), g._words.device
     else:

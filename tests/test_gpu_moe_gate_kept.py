@@ -1,0 +1,72 @@
+"""What a Gate keeps of the call that made it: gate_grad() without mask and normalize is the gradient of that call."""
+import pytest
+
+torch = pytest.importorskip("torch")
+from cann_hccl_b200.parallel import moe  # noqa: E402
+from test_gpu_moe_gate import REL, gate64, grad64  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    torch.manual_seed(8)
+
+
+@pytest.mark.parametrize("normalize", [True, False])
+@pytest.mark.parametrize("T,E,k", [(40, 16, 3), (2371, 60, 4), (5000, 256, 8)])
+def test_gradient_of_a_masked_batch(T, E, k, normalize):
+    l, mask = torch.randn(T, E, device="cuda"), torch.rand(T, device="cuda") < 0.7
+    d = torch.randn(T, k, device="cuda")
+    g = moe.gate(l, k, mask, normalize)
+    want = gate64(l, k, mask, normalize)
+    for kind in (mask, mask.to(torch.uint8)):
+        g = moe.gate(l, k, kind, normalize)
+        got = moe.gate_grad(l, g, d, balance=0.9)
+        assert bool((got[~mask] == 0).all())
+        assert torch.equal(got, moe.gate_grad(l, g, d, 0.9, mask, normalize))
+        d64 = grad64(l, want, k, d, 0.9, normalize)
+        size = (want[6] * want[2].double()[None, :] * (0.9 * E / (k * want[4] ** 2))).amax() * 2 + d.abs().double().amax() * 2
+        assert float((got.double() - d64).abs().max()) <= 8 * REL * float(size)
+
+
+def test_gradient_without_normalised_gates():
+    l, d = torch.randn(50, 24, device="cuda"), torch.randn(50, 5, device="cuda")
+    g = moe.gate(l, 5, normalize=False)
+    assert torch.equal(moe.gate_grad(l, g, d), moe.gate_grad(l, g, d, normalize=False))
+    assert not torch.equal(moe.gate_grad(l, g, d), moe.gate_grad(l, g, d, normalize=True))
+    # a Gate of other tensors: as it is told, normalised where nothing is said
+    assert torch.equal(moe.gate_grad(l, moe.Gate(*g, normalize=False), d), moe.gate_grad(l, g, d))
+    assert torch.equal(moe.gate_grad(l, moe.Gate(*g), d), moe.gate_grad(l, g, d, normalize=True))
+
+
+def test_mask_that_was_written_to():
+    """The Gate has the mask itself, not a copy: one that was written to since is refused, unless the caller gives one."""
+    l, mask = torch.randn(64, 16, device="cuda"), torch.rand(64, device="cuda") < 0.5
+    g, keep = moe.gate(l, 2, mask), mask.clone()
+    want = moe.gate_grad(l, g, g.gates, 1.0)
+    mask.logical_not_()
+    with pytest.raises(RuntimeError, match="mask"):
+        moe.gate_grad(l, g, g.gates, 1.0)
+    assert torch.equal(moe.gate_grad(l, g, g.gates, 1.0, mask=keep), want)
+    assert torch.equal(moe.gate_grad(l, moe.Gate(*g, mask=keep), g.gates, 1.0), want)
+    with torch.inference_mode():                                    # tensors that do not count their writes
+        m = keep.clone()
+        assert torch.equal(moe.gate_grad(l, moe.gate(l, 2, m), g.gates, 1.0), want)
+
+
+def test_captured_with_a_mask():
+    l, mask = torch.randn(500, 64, device="cuda"), torch.rand(500, device="cuda") < 0.5
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        g = moe.gate(l, 4, mask)
+        dl = moe.gate_grad(l, g, g.gates, 0.5)
+    for _ in range(3):
+        l.normal_()
+        mask.copy_(torch.rand(500, device="cuda") < 0.5)
+        graph.replay()
+        want = moe.gate(l, 4, mask)
+        assert torch.equal(dl, moe.gate_grad(l, want, want.gates, 0.5)) and bool((dl[~mask] == 0).all())
