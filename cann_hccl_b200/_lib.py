@@ -92,7 +92,7 @@ class MoeLayer(C.Structure):
 
 class VocabLoss(C.Structure):
     _fields_ = [("x", C.c_void_p), ("w", C.c_void_p), ("xStride", C.c_int64), ("wStride", C.c_int64), ("targets", C.c_void_p), ("weights", C.c_void_p)] + \
-               [(n, C.c_int64) for n in ("tokens", "vocab", "firstId", "wholeVocab", "ignoreId")] + [("hidden", C.c_int32), ("targetType", C.c_int32), ("scratchBytes", C.c_int64)]
+               [(n, C.c_int64) for n in ("tokens", "vocab", "firstId", "wholeVocab", "ignoreId")] + [("hidden", C.c_int32), ("targetType", C.c_int32), ("scratchBytes", C.c_int64), ("losses", C.c_void_p)]
 
 
 _lib = None

@@ -888,7 +888,7 @@ static HcclResult check_vocab_loss(const HcclB200VocabLoss *p, bool targets, std
     CHK_RET(check_aligned({p->weights}, 4, api));
     CHK_RET(check_aligned(words, 4, api));
     *c = VocabLossCall{p->x, p->w, p->xStride, p->wStride, p->targets, p->targetType == HCCL_DATA_TYPE_INT64, p->weights, p->tokens, p->vocab, p->firstId,
-                       p->wholeVocab, p->ignoreId, p->hidden, p->scratchBytes};
+                       p->wholeVocab, p->ignoreId, p->hidden, p->scratchBytes, p->losses};
     return HCCL_SUCCESS;
 }
 int64_t HcclB200VocabLossChunk(int64_t vocab, int32_t withGrad) { return vocab < 1 || vocab >= INT32_MAX - 256 ? -1 : vocab_loss_chunk(vocab, withGrad != 0); }
@@ -962,7 +962,7 @@ HcclResult HcclB200VocabLossGrad(const HcclB200VocabLoss *p, const float *lse, c
 {
     VocabLossCall c;
     CHK_RET(check_vocab_loss(p, false, {lse, target, scratch}, "HcclB200VocabLossGrad", &c));
-    CHK_RET(check_aligned({total}, 4, "HcclB200VocabLossGrad"));
+    CHK_RET(check_aligned({total, p->losses}, 4, "HcclB200VocabLossGrad"));
     CHK_RET(check_dw(c, dx, dw, dwSum, dwKind, scratch, "HcclB200VocabLossGrad"));
     return vocab_loss_grad(c, lse, target, total, scale, dx, dw, dwSum, dwKind, scratch, stream);
 }

@@ -17,8 +17,9 @@
 //          to zero by about 1e-9 H of themselves (measured: 2.6e-7, 1.05e-6, 4.1e-6, 8.4e-6 for H = 256, 1024, 4096, 8192), so losses
 //          lean low (means at H = 4096 by 6e-7 of themselves around 10, 7e-6 around 0.1), and a mean does not average it out.  Nothing is added to make up for it: what
 //          is cut off depends on the order in which a sum grows, which the result does not show.
-// d        exponentials to d in place (bf16), rescaled by exp(m - lse); the target's column is q expm1(s_y - lse), which keeps its
-//          digits for sure guesses.  Tokens that do not count become rows of zeros.
+// d        exponentials to d in place (bf16), rescaled by exp(m - lse); the target's column is q expm1(-loss), and the loss is formed of the
+//          largest logit, the target's and log of the sum beside it, never of lse: rounded to fp32 that would be off by half a step of
+//          a logit, more than a sure guess has (1e-6 at logits of 20).  Tokens that do not count become rows of zeros.
 //          In a whole step with gradients rows and d are one launch, a CTA for each token.
 // dx, dW   tcgen05 products that read W, d and x as they lie: an operand whose depth is not its contiguous side goes to the tensor
 //          cores MN-major (boxes of 64 elements x 64 deep).  dx with few tiles is cut along the vocabulary into fp32 shares that a
@@ -714,14 +715,14 @@ __global__ void __launch_bounds__(kCopyThreads) vocab_loss_x(const __grid_consta
 }
 
 constexpr int kDThreads = 256, kDBatch = 4, kDVecs = kDThreads * kDBatch;
-// Exponentials -> d, in place: kDVecs vectors of 8 columns at a time, from the part-th on, every parts-th.
-__device__ __forceinline__ void row_to_d(const RowArgs &a, int64_t t, int64_t id, float lse, float target, uint32_t part, uint32_t parts)
+// Exponentials -> d, in place: kDVecs vectors of 8 columns at a time, from the part-th on, every parts-th.  behind: target's logit - lse.
+__device__ __forceinline__ void row_to_d(const RowArgs &a, int64_t t, int64_t id, float lse, float behind, uint32_t part, uint32_t parts)
 {
     const float q = weight(a, t, id);
     uint4 *row = (uint4 *)(a.e + t * a.ld * 2);
     const uint32_t vecs = (uint32_t)(a.width / 8), cols = (uint32_t)a.cols, mid = (cols / 16 + 1) / 2 * 16;
     const int64_t y = id - a.first;  // may lie in another shard
-    const float dy = q * expm1f(target - lse);
+    const float dy = q * expm1f(behind);
     const float2 *stats = a.stats + t * a.halves;
     for (uint32_t v0 = part * kDVecs + threadIdx.x; v0 < vecs; v0 += parts * kDVecs) {
         uint4 v[kDBatch];
@@ -741,7 +742,7 @@ __device__ __forceinline__ void row_to_d(const RowArgs &a, int64_t t, int64_t id
             if (i >= vecs) break;
             uint4 o = make_uint4(0, 0, 0, 0);
             if (q != 0.f) {
-                const float fac = __expf(f[k] - lse) * q * kExpScale;
+                const float fac = __expf(f[k] - lse) * q * kExpScale;  // lse's rounding is relative here, 2^-24 |lse|: nothing beside bf16's step
                 float d[8];
                 const __half2 *h = (const __half2 *)&v[k];
 #pragma unroll
@@ -767,7 +768,7 @@ __global__ void __launch_bounds__(kDThreads) vocab_loss_d(const __grid_constant_
     pdl_trigger();
     pdl_wait();
     const int64_t t = blockIdx.y;
-    row_to_d(a, t, target_of(a.y, a.wide, t), a.lse[t], a.target[t], blockIdx.x, gridDim.x);
+    row_to_d(a, t, target_of(a.y, a.wide, t), a.lse[t], a.losses_in ? -a.losses_in[t] : a.target[t] - a.lse[t], blockIdx.x, gridDim.x);
 }
 
 // rows and d of a token by one CTA
@@ -778,7 +779,7 @@ __global__ void __launch_bounds__(kDThreads) vocab_loss_rows_d(const __grid_cons
     pdl_wait();
     const int64_t t = blockIdx.x, id = target_of(a.y, a.wide, t);
     const RowState r = row_state<kDThreads>(a, t, id, s);
-    row_to_d(a, t, id, r.top + r.log_z, r.target, 0, 1);
+    row_to_d(a, t, id, r.top + r.log_z, (r.target - r.top) - r.log_z, 0, 1);
     row_end<kDThreads>(a, t, id, r, s.m);
 }
 
@@ -1018,6 +1019,7 @@ HcclResult rows_to_d(const VocabLossCall &c, const Layout &l, const RowArgs &a, 
         const int64_t n = std::min<int64_t>(65535, c.tokens - t0);
         q.y = (const uint8_t *)a.y + t0 * (a.wide ? 8 : 4);
         q.weights = a.weights ? a.weights + t0 : nullptr;
+        q.losses_in = a.losses_in ? a.losses_in + t0 : nullptr;
         q.e += t0 * a.ld * 2; q.lse += t0; q.target += t0; q.stats += t0 * a.halves;
         CHK_RET(launch_pdl((const void *)vocab_loss_d, dim3((unsigned)parts, (unsigned)n), kDThreads, 0, &q, stream, "vocabulary loss (d)"));
     }
@@ -1095,7 +1097,7 @@ HcclResult vocab_loss_grad(const VocabLossCall &c, const float *lse, const float
     uint8_t *s = (uint8_t *)scratch;
     RowArgs a = row_args(c);
     a.stats = (const float2 *)(s + l.stats); a.halves = 2 * l.n_tiles; a.cols = l.cols;
-    a.e = s; a.ld = l.ld; a.width = l.width; a.lse = (float *)lse; a.target = (float *)target;
+    a.e = s; a.ld = l.ld; a.width = l.width; a.lse = (float *)lse; a.target = (float *)target; a.losses_in = c.losses;
     CHK_RET(rows_to_d(c, l, a, stream));
     return products(c, l, total, scale, dx, dw, dw_sum, out, s, stream);
 }
@@ -1126,6 +1128,7 @@ HcclResult vocab_loss_step(const VocabLossCall &c, bool mean, float scale, float
         CHK_RET(launch_pdl((const void *)vocab_loss_rows_d, dim3((unsigned)c.tokens), kDThreads, 0, &a, stream, "vocabulary loss (rows, d)"));
     else {
         CHK_RET(launch_pdl((const void *)vocab_loss_rows, dim3((unsigned)c.tokens), kRowThreads, 0, &a, stream, "vocabulary loss (rows)"));
+        a.losses_in = a.losses;
         CHK_RET(rows_to_d(c, l, a, stream));
     }
     return products(c, l, a.total, scale, dx, dw, dw_sum, out, s, stream);

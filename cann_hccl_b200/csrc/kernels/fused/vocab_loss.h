@@ -14,6 +14,7 @@ struct VocabLossCall {
     int64_t tokens, vocab, first, whole, ignore;  // first id of the shard, ids of all shards, target of tokens that do not count
     int32_t hidden;
     int64_t scratch_bytes;           // at the call's scratch; 0: not stated
+    const float *losses;             // of the tokens, for the gradients; null: target - lse in their place
 };
 // Tokens whose exponentials fit the scratch of a call with gradients, or whose sums fit that of one without.
 int64_t vocab_loss_chunk(int64_t vocab, bool grad);
@@ -32,7 +33,7 @@ HcclResult vocab_loss_total(const VocabLossCall &c, float *total, void *stream);
 HcclResult vocab_loss_sum(const VocabLossCall &c, const float *losses, const float *total, float *loss, void *stream);
 // What becomes of dw: written in bf16; written or added to in fp32; added to an fp32 sum and written in bf16.
 enum VocabLossOut : int { VL_BF16 = 0, VL_F32 = 1, VL_ADD = 2, VL_ADD_BF16 = 3 };
-// Gradients of scale * loss after vocab_loss_scores with grad: dx bf16 [tokens, hidden] (of this shard alone), dw by `out`: in dw_sum
+// Gradients of scale * loss after vocab_loss_scores with grad (and with the losses that it or vocab_loss_combine left): dx bf16 [tokens, hidden] (of this shard alone), dw by `out`: in dw_sum
 // where it is fp32, in dw where it is bf16.
 HcclResult vocab_loss_grad(const VocabLossCall &c, const float *lse, const float *target, const float *total, float scale, void *dx, void *dw, float *dw_sum,
                            int out, void *scratch, void *stream);

@@ -158,6 +158,8 @@ typedef struct HcclB200VocabLossDef {
     int64_t tokens, vocab, firstId, wholeVocab, ignoreId;
     int32_t hidden, targetType;
     int64_t scratchBytes;                    /* at the scratch of Scores, Grad and Step, which refuse too few; 0: not stated, not looked at */
+    const float *losses;                     /* Grad: the joint losses [tokens] as Scores or Combine left them, for the targets' column of guesses
+                                              * that are all but sure; NULL: lse - target, which loses a step of a logit */
 } HcclB200VocabLoss;
 extern int64_t HcclB200VocabLossChunk(int64_t vocab, int32_t withGrad);
 /* Scratch of a call of exactly `tokens`.  Fewer tokens may need MORE (their dx is cut into more shares): scratch that serves several calls

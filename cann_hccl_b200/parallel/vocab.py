@@ -140,9 +140,10 @@ class _Shard:
         self._call = L.VocabLoss(self._x, w.data_ptr(), self._xs, ws, self._y, self._q, self.T, self.V, first, whole, ignore,
                                  self.H, _IDS[targets.dtype])
 
-    def part(self, a, b):
-        """The call for tokens a to b (the structure is the shard's: valid until the next one)."""
+    def part(self, a, b, losses=None):
+        """The call for tokens a to b (the structure is the shard's: valid until the next one); losses: address of theirs."""
         c = self._call
+        c.losses = losses
         c.x, c.targets, c.tokens = self._x + a * self._xs * 2, self._y + a * self._ysize, b - a
         if self._q is not None:
             c.weights = self._q + a * 4
@@ -195,9 +196,9 @@ def _run_loss(shards, comm, reduction, scale=1.0, outs=None, grad=False):
             for s, e, p, loss in zip(shards, every, words, losses):
                 check(lib.HcclB200VocabLossCombine(s.part(a, b), e.data_ptr(), comm.nranks, p + 8 * chunk, loss.data_ptr() + a * 4, st), "HcclB200VocabLossCombine")
         if grad:
-            for i, (s, m, p) in enumerate(zip(shards, mem, words)):
+            for i, (s, m, p, loss) in enumerate(zip(shards, mem, words, losses)):
                 kind = _ADD if outs[i] is not None else _BF16_OUT if not several else _F32_OUT if a == 0 else _ADD if b < T else _ADD_BF16
-                check(lib.HcclB200VocabLossGrad(s.part(a, b), p if alone else p + 8 * chunk, p + n * 4, totals[i], scale, dxs[i].data_ptr() + a * s.H * 2,
+                check(lib.HcclB200VocabLossGrad(s.part(a, b, loss.data_ptr() + a * 4), p if alone else p + 8 * chunk, p + n * 4, totals[i], scale, dxs[i].data_ptr() + a * s.H * 2,
                                                 dws[i].data_ptr(), None if sums[i] is None else sums[i].data_ptr(), kind, m.data_ptr(), st), "HcclB200VocabLossGrad")
     if grad and not T:
         for o, d in zip(outs, dws):

@@ -108,3 +108,13 @@ def test_sizes_that_are_none():
     on = REAL.HcclB200VocabLossScratchBytesOn
     assert on(0, 74, 4, 16, 8, 1) == on(148, 0, 4, 16, 8, 1) == on(148, 74, -1, 16, 8, 1) == on(148, 74, 4, 16, 12, 1) == on(148, 74, 4, 0, 8, 1) == -1
     assert on(148, 74, 0, 16, 8, 1) > 0
+
+
+def test_refused_before_anything_is_asked_for():
+    mem = C.create_string_buffer(2048)
+    at = (C.addressof(mem) + 255) // 256 * 256
+    call = lambda **k: C.byref(L.VocabLoss(**{**dict(x=at, w=at, xStride=8, wStride=8, targets=at, tokens=4, vocab=16, wholeVocab=16, ignoreId=-100, hidden=8, targetType=L.INT64), **k}))
+    assert REAL.HcclB200VocabLossScores(call(scratchBytes=-1), 1, at, at, at, at, None) == L.E_PARA
+    assert REAL.HcclB200VocabLossStep(call(scratchBytes=-1), 1, 1.0, at, at, at, None, 0, at, None) == L.E_PARA
+    assert REAL.HcclB200VocabLossGrad(call(scratchBytes=-1), at, at, at, 1.0, at, at, None, 0, at, None) == L.E_PARA
+    assert REAL.HcclB200VocabLossGrad(call(losses=at + 2), at, at, at, 1.0, at, at, None, 0, at, None) == L.E_PARA
