@@ -12,6 +12,7 @@ no gradient.  On an all-local communicator w (and what is per rank) is a list wi
 their own, as everywhere in this package: results carry no automatic differentiation.
 """
 import ctypes as C
+import struct
 
 import torch
 
@@ -96,10 +97,27 @@ def first_ids(comm, vocab_rows):
     return [r * vocab_rows for r in (range(comm.nranks) if comm.nlocal > 1 else [comm.rank])]
 
 
+def _check_shards(comm, ws):
+    """Refuses shards of several sizes: first ids follow from one.  Ranks of other processes are asked over the control plane, at the first
+    call with a size (on every rank, since all of them have the same calls)."""
+    rows = [t.shape[0] for t in ws]
+    # a communicator without a control plane cannot be asked
+    if comm.nlocal < comm.nranks and hasattr(comm, "exchange"):
+        known = comm.__dict__.setdefault("_shard_rows", set())
+        if rows[0] in known:
+            return
+        rows = [struct.unpack("<q", b)[0] for b in comm.exchange("vocab-rows", struct.pack("<q", rows[0]))]
+        if len(set(rows)) == 1:
+            known.add(rows[0])
+    if len(set(rows)) > 1:
+        raise ValueError("all ranks need shards of one size, they have %s rows: pad the vocabulary" % rows)
+
+
 def vocab_parallel_embedding(comm, ids, w, scale=1.0):
-    """Every rank holds vocab / p rows of the table (rank r the ids from r * rows on) and the same ids: the lookups are summed over the
-    ranks (all but one are zero, so nothing is rounded twice).  Its gradient is embedding_grad() with the shard's first_id."""
+    """Every rank holds vocab / p rows of the table (rank r the ids from r * rows on, the same number on all ranks) and the same ids: the
+    lookups are summed over the ranks (all but one are zero, so nothing is rounded twice).  Its gradient is embedding_grad() with the shard's first_id."""
     ids_l, ws = _per_rank(comm, ids, w)
+    _check_shards(comm, ws)
     outs = [embedding(i, t, scale, first) for i, t, first in zip(ids_l, ws, first_ids(comm, ws[0].shape[0]))]
     if comm.nranks > 1 and outs[0].numel():
         comm.all_reduce(outs, outs)
@@ -268,13 +286,14 @@ def _sharded(comm, x, w, targets, weights, reduction, ignore_index):
         _check_loss(*a, reduction)
     if len({t.shape for t in xs}) > 1 or len({t.shape for t in ws}) > 1:
         raise ValueError("all ranks need the same tokens and shards of one size")
+    _check_shards(comm, ws)
     whole = ws[0].shape[0] * comm.nranks
     return [_Shard(*a, f, whole, ignore_index) for a, f in zip(zip(xs, ws, ys, qs), first_ids(comm, ws[0].shape[0]))]
 
 
 def vocab_parallel_cross_entropy(comm, x, w, targets, weights=None, reduction="mean", ignore_index=-100):
-    """linear_cross_entropy() where every rank holds vocab / p rows of w (rank r the ids from r * rows on), and the same x, targets and
-    weights.  The ranks exchange two numbers for each token."""
+    """linear_cross_entropy() where every rank holds vocab / p rows of w (rank r the ids from r * rows on, the same number on all ranks), and
+    the same x, targets and weights.  The ranks exchange two numbers for each token."""
     shards = _sharded(comm, x, w, targets, weights, reduction, ignore_index)
     with on_device_of(shards[0].x):
         out = _run_loss(shards, comm, reduction)
