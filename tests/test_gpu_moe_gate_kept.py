@@ -70,3 +70,27 @@ def test_captured_with_a_mask():
         graph.replay()
         want = moe.gate(l, 4, mask)
         assert torch.equal(dl, moe.gate_grad(l, want, want.gates, 0.5)) and bool((dl[~mask] == 0).all())
+
+
+@pytest.mark.parametrize("normalize", [True, False])
+@pytest.mark.parametrize("E", [16, 200])
+def test_gate_by_hand_that_names_an_expert_twice(E, normalize):
+    """Each slot passes its part on, whichever expert it names."""
+    l, d = torch.randn(300, E, device="cuda"), torch.randn(300, 4, device="cuda")
+    g = moe.gate(l, 4, normalize=normalize)
+    idx = g.idx.clone()
+    idx[::2, 1] = idx[::2, 0]
+    idx[::4, 3] = idx[::4, 0]
+    idx[1::4, 3] = idx[1::4, 2]
+    p = torch.softmax(l.double(), 1)
+    gates = p.gather(1, idx.long())
+    if normalize:
+        gates = gates / gates.sum(1, keepdim=True)
+    counts = torch.bincount(idx.flatten(), minlength=E).int()
+    hand = moe.Gate(idx, gates.float(), counts, p.sum(0).float(), g.routed, g.balance, normalize=normalize)
+    want = grad64(l, (idx, gates, counts, None, 300, None, p), 4, d, 0.6, normalize)
+    got = moe.gate_grad(l, hand, d, 0.6).double()
+    # sums of at most nine terms of this size, each off by REL
+    size = d.abs().double().amax() * 2 + 0.6 * E / (4 * 300 ** 2) * float(counts.max()) * 2
+    assert float((got - want).abs().max()) <= 9 * REL * float(size)
+    assert torch.equal(got, moe.gate_grad(l, hand, d, 0.6).double())
