@@ -961,7 +961,8 @@ RowArgs row_args(const VocabLossCall &c)
 
 int64_t vocab_loss_chunk(int64_t vocab, bool grad)
 {
-    // two thousand million bytes of exponentials, or 128 MB of sums of half tiles (16 bytes for 256 columns, or for 128 at worst)
+    // two thousand million bytes of exponentials, or 128 MB of sums of half tiles (16 bytes for 256 columns, or for 128 at worst); the copy of x
+    // (as large as the chunk's x) and shares of dx (up to 0.9 GB, of fewer tokens) come on top
     const int64_t ld = (vocab + 63) / 64 * 64, rows = grad ? (int64_t)(1ll << 31) / (ld * 2) : (int64_t)(128ll << 20) / (ld / 128 * 16 + 16);
     return std::min<int64_t>(1 << 20, std::max<int64_t>(256, rows / 256 * 256));
 }

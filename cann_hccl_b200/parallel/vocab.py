@@ -255,7 +255,9 @@ def linear_cross_entropy(x, w, targets, weights=None, reduction="mean", ignore_i
     """Softmax cross entropy of the logits x [tokens, hidden] @ w [vocab, hidden].T (bf16, fp32 sums) against `targets` (int32 or int64).
     Tokens whose target is ignore_index or no id of the vocabulary do not count.  `weights`: fp32 [tokens].  reduction: "none" gives
     the unweighted losses [tokens] (0 where a token does not count), "sum" their weighted sum, "mean" that divided by the sum of the
-    weights that count (0 where there is none).  The logits are not stored: beyond the arguments it takes about 130 MB at most (for 256 tokens at least).
+    weights that count (0 where there is none).  The logits are not stored: beyond arguments and results it takes about 130 MB at
+    most (for 256 tokens at least) and, for more than 128 tokens whose hidden size is no multiple of 64, a copy of x (of a chunk of tokens,
+    at most 2^20).
     The tensor cores' fp32 sums lean towards zero: losses come out low by a few 1e-6 of themselves at hidden 4096 (means of 256 tokens:
     6e-7 at a loss of 10, 7e-6 at 0.1), growing with hidden."""
     _check_loss(x, w, targets, weights, reduction)
@@ -266,8 +268,9 @@ def linear_cross_entropy(x, w, targets, weights=None, reduction="mean", ignore_i
 def linear_cross_entropy_grad(x, w, targets, weights=None, reduction="mean", ignore_index=-100, scale=1.0, dw=None):
     """(loss, dx, dw): the loss as linear_cross_entropy() gives it ("mean" or "sum") and the gradients of scale * loss.  dx and dw are bf16;
     given an fp32 tensor `dw` [vocab, hidden], the weight's gradient is added to it (several batches, or a weight that the embedding
-    shares) and it is returned.  Beyond the results it takes about 2 GiB at most, for the exponentials of a chunk of tokens (of 256 tokens at
-    least), and an fp32 sum of dw where the tokens are more than one chunk (a thousand million logits)."""
+    shares) and it is returned.  Beyond the results it takes, for a chunk of tokens (a thousand million logits, 256 to 2^20 tokens), a copy of
+    the chunk's x and about 3 GB at most up to hidden 16384 (exponentials, row sums, fp32 shares of dx); and an fp32 sum of dw where the
+    tokens are more than one chunk."""
     _check_loss(x, w, targets, weights, reduction)
     if reduction == "none":
         raise ValueError("gradients need a sum or mean over the tokens (weights scale each token)")

@@ -118,3 +118,19 @@ def test_refused_before_anything_is_asked_for():
     assert REAL.HcclB200VocabLossStep(call(scratchBytes=-1), 1, 1.0, at, at, at, None, 0, at, None) == L.E_PARA
     assert REAL.HcclB200VocabLossGrad(call(scratchBytes=-1), at, at, at, 1.0, at, at, None, 0, at, None) == L.E_PARA
     assert REAL.HcclB200VocabLossGrad(call(losses=at + 2), at, at, at, 1.0, at, at, None, 0, at, None) == L.E_PARA
+
+
+@pytest.mark.parametrize("grad", [0, 1])
+@pytest.mark.parametrize("V", [256, 1000, 8000, 32000, 50257, 128256, 151936, 200064, 1 << 18, 1 << 19])
+def test_scratch_stays_within_what_is_stated(V, grad):
+    """Beside the copy of x (none without gradients where its rows start on 128-byte lines, or there is one row of tiles): 130 MB, or
+    3 GB with the exponentials and shares of the gradients."""
+    chunk = REAL.HcclB200VocabLossChunk(V, grad)
+    for H in (64, 1000, 4096, 4104, 8192, 16384):
+        for T in {1, 128, 129, 300, 700, 1500, 3000, 6000, *range(chunk - chunk // 4, chunk, max(1, chunk // 50)), chunk - 1, chunk}:
+            if T > chunk:
+                continue
+            copy = T * ((H + 63) // 64 * 128) if grad or (T > 128 and H % 64) else 0
+            for pairs in (70, 74):
+                got = REAL.HcclB200VocabLossScratchBytesOn(148, pairs, T, V, H, grad) - copy
+                assert got <= (3 * 10 ** 9 if grad else 130 * 10 ** 6), (H, T)
