@@ -829,7 +829,7 @@ static HcclResult check_gate(const void *logits, HcclDataType type, int64_t toke
     CHK_RET(check_aligned({logits}, dtype_size(type), api));
     CHK_RET(check_aligned(words, 4, api));
     CHK_RET(check_aligned(per_token, dtype_size(type), api));
-    *s = GateShape{tokens, nExperts, topk, type, stride, normalize != 0};
+    *s = GateShape{tokens, nExperts, topk, type, stride, normalize != 0, false};
     return HCCL_SUCCESS;
 }
 int64_t HcclB200MoeGateScratchBytes(int64_t tokens, int32_t nExperts)
@@ -859,6 +859,8 @@ HcclResult HcclB200MoeGateGrad(const void *logits, HcclDataType dataType, int64_
 {
     GateShape s;
     CHK_RET(check_gate(logits, dataType, tokens, nExperts, stride, topk, normalize, {counts, routed}, {idx, dLogits}, "HcclB200MoeGateGrad", &s));
+    s.normalize = (normalize & ~HCCL_B200_GATE_REPEATED) != 0;
+    s.again = (normalize & HCCL_B200_GATE_REPEATED) != 0;
     CHK_RET(check_aligned({idx, dGates}, 4, "HcclB200MoeGateGrad"));
     return moe_gate_grad(s, logits, idx, dGates, counts, routed, mask, dBalance, dLogits, stream);
 }

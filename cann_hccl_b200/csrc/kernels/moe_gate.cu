@@ -88,7 +88,7 @@ struct GateArgs {
     const float *d_gates;
     void *d_logits;
     int64_t tokens, stride;
-    int experts, topk, normalize;
+    int experts, topk, normalize, again;
     float coef;
 };
 
@@ -339,10 +339,11 @@ __global__ void __launch_bounds__(kEndThreads) moe_gate_end_kernel(const __grid_
     *a.balance = balance_of(a.arrived ? all : sum, n, E, a.topk);
 }
 
-// gate() names an expert once; where a caller's slots name one again, the first of them stands for all: how many they are, and the sum of
-// their gradients, in the order of the slots.  peers: lanes with this lane's expert.
-__device__ __forceinline__ void merge_slots(uint32_t peers, int lane, int k, int *sel, float *dg, float *times)
+// kAgain: slots of a token may name an expert again, as gate() never does.  The first of them stands for all then: how many they are, and
+// the sum of their gradients, in the order of the slots.  (A variant of its own: the look for such slots alone costs the others 6 to 15 %.)
+__device__ __forceinline__ void merge_slots(int lane, int k, int *sel, float *dg, float *times)
 {
+    const uint32_t peers = __match_any_sync(kAll, *sel);
     float sum = 0.f;
     for (int j = 0; j < k; ++j) {
         const float v = __shfl_sync(kAll, *dg, j);
@@ -354,86 +355,69 @@ __device__ __forceinline__ void merge_slots(uint32_t peers, int lane, int k, int
     *sel = first ? *sel : -1;
 }
 
-template <class T, int V> __device__ __noinline__ void grad_merged(const GateArgs &a, int64_t t, int lane, const float *s_u, float *extra);
-
-// Gradient of token t by a warp; extra: a row of zeros, left so.  kMerge: slots may name an expert again (a variant of its own: such a branch
-// in the way of the others costs them 15 %).
-template <class T, int V, bool kMerge>
-__device__ __forceinline__ void grad_row(const GateArgs &a, int64_t t, int lane, const float *s_u, float *extra)
-{
-    const int E = a.experts, k = a.topk;
-    const T *row = (const T *)a.logits + t * a.stride;
-    T *out = (T *)a.d_logits + t * E;
-    int sel = lane < k ? a.idx[t * k + lane] : -1;
-    if (sel >= E) sel = -1;
-    float dg = a.d_gates && sel >= 0 ? a.d_gates[t * k + lane] : 0.f, times = 1.f;
-    float x[V], m = -INFINITY;
-    load_row<T, V>(a, t, lane, x);
-    const uint32_t peers = __match_any_sync(kAll, sel);
-    if (kMerge) merge_slots(peers, lane, k, &sel, &dg, &times);
-    const bool again = !kMerge && __any_sync(kAll, sel >= 0 && (peers & (peers - 1)));
-    const float sel_x = sel >= 0 ? ld_f(row + sel) : -INFINITY;
-#pragma unroll
-    for (int j = 0; j < V; ++j) m = max_nan(m, x[j]);
-    m = value_of(__reduce_max_sync(kAll, key_of(m)));  // NaN where one is
-    const bool on = (!a.mask || a.mask[t]) && !(m == -INFINITY);
-    if (!on || again) {
-        if (on) grad_merged<T, V>(a, t, lane, s_u, extra);
-        else
-#pragma unroll
-            for (int j = 0; j < V; ++j)
-                if (j * 32 + lane < E) st_f(out + j * 32 + lane, 0.f);
-        return;
-    }
-    float z = 0.f;
-#pragma unroll
-    for (int j = 0; j < V; ++j) { x[j] = exp_of(x[j] - m); z += x[j]; }
-    z = warp_sum(z);
-    const float inv = __fdividef(1.f, z);
-    float g = exp_of(sel_x - m);   // 0 where the slot is empty
-    const float whole = a.normalize ? warp_sum(kMerge ? g * times : g) : z;
-    g = g > 0.f ? __fdividef(g, whole) : g;
-    const float gd = warp_sum(g * dg);
-    if (sel >= 0) extra[sel] = a.normalize ? g * (dg - (kMerge ? times * gd : gd)) : g * dg;
-    float dot = 0.f;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const int e = j * 32 + lane;
-        x[j] *= inv;
-        if (e < E) dot += x[j] * s_u[e];
-    }
-    dot = warp_sum(dot);  // its shuffles also put `extra` before the reads below
-    __syncwarp();
-    if (!a.normalize) dot += gd;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const int e = j * 32 + lane;
-        if (e < E) st_f(out + e, fmaf(x[j], s_u[e] - dot, extra[e]));
-    }
-    __syncwarp();
-    if (sel >= 0) extra[sel] = 0.f;
-    __syncwarp();
-}
-template <class T, int V> __device__ __noinline__ void grad_merged(const GateArgs &a, int64_t t, int lane, const float *s_u, float *extra)
-{
-    grad_row<T, V, true>(a, t, lane, s_u, extra);
-}
-
 // Dynamic shared memory: [experts] u, [warps][experts] what the gates add at the chosen experts.
-template <class T, int V>
+template <class T, int V, bool kAgain>
 __global__ void __launch_bounds__(kGateMost<V>, kGateCtas<V>) moe_gate_grad_kernel(const __grid_constant__ GateArgs a)
 {
     extern __shared__ uint32_t sh[];
-    const int E = a.experts, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5;
+    const int E = a.experts, k = a.topk, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5;
     float *s_u = (float *)sh, *extra = s_u + E + warp * E;
     for (int i = lane; i < E; i += 32) extra[i] = 0.f;
     pdl_trigger();
     pdl_wait();
     const int n = *a.routed;
-    const float per = n ? a.coef * ((float)E / (float)a.topk) / (float)n / (float)n : 0.f;
+    const float per = n ? a.coef * ((float)E / (float)k) / (float)n / (float)n : 0.f;
     for (int e = threadIdx.x; e < E; e += blockDim.x) s_u[e] = per * (float)a.counts[e];
     __syncthreads();
-    for (int64_t t = (int64_t)blockIdx.x * W + warp; t < a.tokens; t += (int64_t)gridDim.x * W) grad_row<T, V, false>(a, t, lane, s_u, extra);
+    for (int64_t t = (int64_t)blockIdx.x * W + warp; t < a.tokens; t += (int64_t)gridDim.x * W) {
+        const T *row = (const T *)a.logits + t * a.stride;
+        T *out = (T *)a.d_logits + t * E;
+        int sel = lane < k ? a.idx[t * k + lane] : -1;
+        if (sel >= E) sel = -1;
+        float dg = a.d_gates && sel >= 0 ? a.d_gates[t * k + lane] : 0.f, times = 1.f;
+        float x[V], m = -INFINITY;
+        load_row<T, V>(a, t, lane, x);
+        if (kAgain) merge_slots(lane, k, &sel, &dg, &times);
+        const float sel_x = sel >= 0 ? ld_f(row + sel) : -INFINITY;
+#pragma unroll
+        for (int j = 0; j < V; ++j) m = max_nan(m, x[j]);
+        m = value_of(__reduce_max_sync(kAll, key_of(m)));  // NaN where one is
+        const bool on = (!a.mask || a.mask[t]) && !(m == -INFINITY);
+        if (!on) {
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (j * 32 + lane < E) st_f(out + j * 32 + lane, 0.f);
+            continue;
+        }
+        float z = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) { x[j] = exp_of(x[j] - m); z += x[j]; }
+        z = warp_sum(z);
+        const float inv = __fdividef(1.f, z);
+        float g = exp_of(sel_x - m);   // 0 where the slot is empty
+        const float whole = a.normalize ? warp_sum(kAgain ? g * times : g) : z;
+        g = g > 0.f ? __fdividef(g, whole) : g;
+        const float gd = warp_sum(g * dg);
+        if (sel >= 0) extra[sel] = a.normalize ? g * (dg - (kAgain ? times * gd : gd)) : g * dg;
+        float dot = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int e = j * 32 + lane;
+            x[j] *= inv;
+            if (e < E) dot += x[j] * s_u[e];
+        }
+        dot = warp_sum(dot);  // its shuffles also put `extra` before the reads below
+        __syncwarp();
+        if (!a.normalize) dot += gd;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int e = j * 32 + lane;
+            if (e < E) st_f(out + e, fmaf(x[j], s_u[e] - dot, extra[e]));
+        }
+        __syncwarp();
+        if (sel >= 0) extra[sel] = 0.f;
+        __syncwarp();
+    }
 }
 
 // Threads and CTAs of a call.
@@ -456,7 +440,7 @@ template <class T, int V> HcclResult run_gate(GateArgs &a, bool grad, void *stre
 {
     const GateGrid g = gate_grid(a.tokens, a.experts, grad);
     const size_t smem = gate_smem(g.threads, a.experts, grad ? 0 : V * 32);
-    const void *fn = grad ? (const void *)moe_gate_grad_kernel<T, V> : (const void *)moe_gate_kernel<T, V>;
+    const void *fn = !grad ? (const void *)moe_gate_kernel<T, V> : a.again ? (const void *)moe_gate_grad_kernel<T, V, true> : (const void *)moe_gate_grad_kernel<T, V, false>;
     if (smem > 32 * 1024) CHK_RET(grant_smem(fn, grad ? gate_smem(kGradMost<V>, V * 32, 0) : gate_smem(kGateMost<V>, V * 32, V * 32), "router"));
     return launch_pdl(fn, dim3((unsigned)g.ctas), (unsigned)g.threads, smem, &a, stream, grad ? "router gradient" : "router");
 }
@@ -475,7 +459,7 @@ template <class T> HcclResult gate_typed(GateArgs &a, bool grad, void *stream)
 
 HcclResult gate_any(const GateShape &s, GateArgs &a, bool grad, void *stream)
 {
-    a.tokens = s.tokens; a.stride = s.stride; a.experts = s.experts; a.topk = s.topk; a.normalize = s.normalize;
+    a.tokens = s.tokens; a.stride = s.stride; a.experts = s.experts; a.topk = s.topk; a.normalize = s.normalize; a.again = s.again;
     switch (s.type) {
         case HCCL_DATA_TYPE_FP32: return gate_typed<float>(a, grad, stream);
         case HCCL_DATA_TYPE_FP16: return gate_typed<__half>(a, grad, stream);

@@ -12,6 +12,7 @@ struct GateShape {
     HcclDataType type;       // of the logits: FP32, FP16, BFP16
     int64_t stride;          // elements between rows of the logits
     bool normalize;          // gates of a token sum to one
+    bool again;              // gradient: slots of a token may name an expert more than once
 };
 int64_t moe_gate_scratch_bytes(int64_t tokens, int32_t experts);
 HcclResult moe_gate(const GateShape &s, const void *logits, const uint8_t *mask, int32_t *idx, float *gates, int32_t *counts, float *prob_sum,

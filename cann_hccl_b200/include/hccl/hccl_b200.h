@@ -142,7 +142,9 @@ extern HcclResult HcclB200MoeGate(const void *logits, HcclDataType dataType, int
 extern HcclResult HcclB200MoeBalance(const int32_t *counts, const float *probSum, const int32_t *routed, int32_t nExperts, int32_t topk,
                                      float *balance, aclrtStream stream);
 /* dLogits [tokens, nExperts] (of the logits' type) from the gates' gradient (null: none) and the balance loss's, which is the number
- * dBalance; counts and routed as the loss had them (counts are constants of it). */
+ * dBalance; counts and routed as the loss had them (counts are constants of it).  A token's slots name an expert once, as HcclB200MoeGate
+ * leaves them; where some may name one again, HCCL_B200_GATE_REPEATED goes with normalize: all of them pass their part on then. */
+#define HCCL_B200_GATE_REPEATED 256
 extern HcclResult HcclB200MoeGateGrad(const void *logits, HcclDataType dataType, int64_t tokens, int32_t nExperts, int64_t stride, int32_t topk,
                                       int32_t normalize, const uint8_t *mask, const int32_t *idx, const float *dGates, const int32_t *counts,
                                       const int32_t *routed, float dBalance, void *dLogits, aclrtStream stream);

@@ -198,6 +198,10 @@ class Gate:
                           _written=None if mask is None else _writes(mask))
         return g
 
+    def _touched(self):
+        """Whether someone may have written to the parts: they are the caller's own, or torch has seen a write."""
+        return self._words is None or _writes(self._words) != 0
+
     def __iter__(self):
         return (getattr(self, n) for n in self._FIELDS)
 
@@ -210,6 +214,7 @@ class Gate:
 
 
 _FLOAT = float_codes()
+_REPEATED = 256  # of HcclB200MoeGateGrad's normalize
 
 
 def _check_gate(logits, topk, mask):
@@ -300,7 +305,8 @@ def gate_grad(logits, g, d_gates=None, balance=0.0, mask=None, normalize=None, o
             check_out(out, (T, E), logits.dtype, dev)
         L.lib()
         idx, counts, routed = g._addresses(0, 2, 4)
-        rc = L.fast.gate_grad(logits, code, T, E, stride, topk, int(normalize), mask, idx, d_gates, counts, routed, balance, out, _raw_stream())
+        # slots that were written to may name an expert again
+        rc = L.fast.gate_grad(logits, code, T, E, stride, topk, int(bool(normalize)) | (_REPEATED if g._touched() else 0), mask, idx, d_gates, counts, routed, balance, out, _raw_stream())
         if rc:
             L.check(rc, "HcclB200MoeGateGrad")
     return out

@@ -94,3 +94,16 @@ def test_gate_by_hand_that_names_an_expert_twice(E, normalize):
     size = d.abs().double().amax() * 2 + 0.6 * E / (4 * 300 ** 2) * float(counts.max()) * 2
     assert float((got - want).abs().max()) <= 9 * REL * float(size)
     assert torch.equal(got, moe.gate_grad(l, hand, d, 0.6).double())
+
+
+def test_slots_written_to_by_hand():
+    """The same of a Gate of gate() whose experts were changed in place."""
+    l, d = torch.randn(300, 40, device="cuda"), torch.randn(300, 4, device="cuda")
+    g = moe.gate(l, 4)
+    plain = moe.gate_grad(l, g, d, 0.6)
+    assert torch.equal(plain, moe.gate_grad(l, moe.Gate(*g), d, 0.6))                # two variants, the same bits where experts differ
+    g.idx[::3, 2] = g.idx[::3, 0]
+    got = moe.gate_grad(l, g, d, 0.6)
+    assert torch.equal(got, moe.gate_grad(l, moe.Gate(*[t.clone() for t in g]), d, 0.6))
+    keep = torch.arange(300, device="cuda") % 3 != 0
+    assert torch.equal(got[keep], plain[keep]) and not torch.equal(got, plain)
