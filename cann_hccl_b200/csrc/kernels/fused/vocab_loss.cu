@@ -1,7 +1,9 @@
 // Linear layer and softmax cross entropy over the vocabulary, with gradients, without keeping the logits:
 //   s = x W^T;  lse_t = log sum_v exp s_tv;  loss_t = lse_t - s_t,y;  d_tv = q_t (exp(s_tv - lse_t) - [v = y]);  dx = a d W;  dW = a d^T x
 // (q: weight of the token; a: scale, divided by the sum of the weights for a mean; applied to the fp32 sums, so that the d of a target
-// far from sure is -q and not -q a: an ordinary weight of one is not rounded at all)
+// far from sure is -q and not -q a: an ordinary weight of one is not rounded at all.  Other weights are, with d, by half a step of bf16: dx and dW
+// are 2.4e-3 off in their 2-norm then, 1.9e-3 without.  d without q, with q in dx's epilogue and in the x that dW reads, would spare dx that
+// rounding and round dW's operands twice)
 //
 // x        with gradients (or where rows do not start on 128-byte lines) the tokens' rows are copied, those of tokens that do not count as
 //          zeros: 0 x inf is not 0.
@@ -27,8 +29,9 @@
 //
 // One persistent CTA per SM: warp 0 TMA producer (128-byte swizzle, never multicast), warp 1 MMA issuer into one of two TMEM
 // accumulators, warps 2-9 epilogue of the other.  More than 128 rows: clusters of two CTAs on 256 rows (cta_group::2).
-// Bound: tensor cores under the power cap (8192 x 128256 x 4096: scores 5.5, dx 5.4, dW 5.5 ms, 1.57 PFLOP/s alone; d 0.65 ms, 6.5 TB/s;
-// 19.4 ms together), HBM for few tokens (7 x 32000 x 4096: 47 us).
+// Bound: tensor cores under the power cap (8192 x 128256 x 4096: scores 5.5, dx 5.4, dW 5.5 ms, 1.57 PFLOP/s alone; rows and d 0.69 ms, 6.5
+// TB/s; a step 19.4 to 23 ms by box and by what ran before), HBM for few tokens (7 x 32000 x 4096: 47 us) and, with gradients, for small
+// hidden sizes, since each logit moves ten bytes (1024 x 160000 x 256: scores 118, rows and d 123, dx 74, dW 73 us).
 // A wait that runs out makes what it was for NaN.
 #include <cuda.h>
 #include <cuda_bf16.h>
