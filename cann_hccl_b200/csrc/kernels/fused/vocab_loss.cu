@@ -16,9 +16,10 @@
 // rows     lse and loss of a token from its half tiles.  The target's logit is summed once more in fp32 FMAs of short chains and put in the
 //          place of the tensor cores' one in lse too: their running sum cuts digits off instead of rounding, and a loss near zero is
 //          the difference of two logits that would carry that.  The other logits keep the cut: sums that grow evenly come out nearer
-//          to zero by about 1e-9 H of themselves (measured: 2.6e-7, 1.05e-6, 4.1e-6, 8.4e-6 for H = 256, 1024, 4096, 8192), so losses
-//          lean low (means at H = 4096 by 6e-7 of themselves around 10, 7e-6 around 0.1), and a mean does not average it out.  Nothing is added to make up for it: what
-//          is cut off depends on the order in which a sum grows, which the result does not show.
+//          to zero by about 1e-9 of themselves for each element of the depth (2.6e-7, 1.05e-6, 4.1e-6 for 256, 1024, 4096), with one sign, so
+//          that a mean does not average it out.  So the depth is taken in parts of 1024 to 2047 elements (512 to 1023 where a single CTA
+//          has the rows), whose sums the epilogue adds in fp32: means of losses at H = 4096 are 1.3e-7 low around 10, 2.7e-6 around
+//          0.1 (5.8e-7 and 7.3e-6 in one part).
 // d        exponentials to d in place (bf16), rescaled by exp(m - lse); the target's column is q expm1(-loss), and the loss is formed of the
 //          largest logit, the target's and log of the sum beside it, never of lse: rounded to fp32 that would be off by half a step of
 //          a logit, more than a sure guess has (1e-6 at logits of 20).  Tokens that do not count become rows of zeros.
@@ -55,6 +56,9 @@ enum Mode : int { SCORES = 0, DX = 1, DW = 2 };
 constexpr int kThreads = 320, kEpiWarps = 8;
 constexpr uint32_t kABytes = BM * BK * 2, kStageSpace = 7 * 32768;  // seven stages of a pair
 constexpr uint32_t kTmemCols = 512;
+// k_iters of a part of the scores' depth, the least.  Parts as short as these cost 0.7 % at most; of pairs, half as long ones cost the step up
+// to 7 % (1024 x 128256 x 2048), since the epilogue has half of the time for its own work while the next parts are multiplied.
+template <bool kPair> constexpr int kPartLeast = kPair ? 16 : 8;
 constexpr int kMaxStages = 8, kMaxCols = BN;
 constexpr uint32_t kChunkBytes = BK * 128;         // MN-major: 64 elements x 64 deep
 constexpr float kExpBits = 15.f, kExpScale = 1.f / 32768.f, kLog2e = 1.4426950408889634f;
@@ -64,6 +68,7 @@ struct alignas(64) LossGemm {
     int M, N;                        // rows and columns of the result
     int cols, um_tiles, n_tiles, panel;
     int k_iters, split;              // split: shares along the depth (DX)
+    int part;                        // k_iters of a part of the depth (scores in parts)
     int units, stages;
     uint32_t stage_bytes, a_bytes, idesc;  // of a stage, of A in it
     // scores
@@ -145,6 +150,13 @@ __device__ __forceinline__ float exp2_approx(float x)
     return y;
 }
 __device__ __forceinline__ int64_t target_of(const void *y, int wide, int64_t t) { return wide ? ((const int64_t *)y)[t] : (int64_t)((const int32_t *)y)[t]; }
+
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const float *v)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(taddr), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]), "f"(v[10]),
+                   "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]) : "memory");
+}
 
 // Half a tile's columns of a row stay in registers: the accumulator is free again before any of them is worked on.
 constexpr int kHalf = kMaxCols / 2;
@@ -238,9 +250,11 @@ __device__ __forceinline__ void turn_sum(uint8_t *box, const float *v, int lane,
     }
 }
 
-template <int MODE, bool kPair>
+// kParts (scores): the accumulators take turns with the parts of a tile's depth, whose sums the epilogue adds.
+template <int MODE, bool kPair, bool kParts>
 __global__ void __launch_bounds__(kThreads, 1) vocab_loss_gemm(const __grid_constant__ LossGemm P)
 {
+    static_assert(!kParts || MODE == SCORES);
     extern __shared__ uint8_t smem_raw[];
     LossShared &S = *(LossShared *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     constexpr int kCtas = kPair ? 2 : 1;
@@ -255,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_loss_gemm(const __grid_cons
     if (threadIdx.x == 0) {
         S.fail = 0;
         for (int i = 0; i < kMaxStages; ++i) { mbar_init(&S.full_bar[i], 1); mbar_init(&S.empty_bar[i], 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&S.tmem_full[i], 1); mbar_init(&S.tmem_empty[i], kEpiWarps); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&S.tmem_full[i], 1); mbar_init(&S.tmem_empty[i], kPair && kParts ? 2 * kEpiWarps : kEpiWarps); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         prefetch_tensormap(&P.tmA);
         prefetch_tensormap(&P.tmB);
@@ -316,37 +330,43 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_loss_gemm(const __grid_cons
         // ------------------------------------------------------------------ MMA issuer (pair: the leader, for both CTAs)
         if (cta_r == 0 && elect_one()) {
             uint32_t s = 0, ph = 0, n = 0;
-            for (int t = unit; t < total && !*fail; t += P.units, ++n) {
+            for (int t = unit; t < total && !*fail; t += P.units) {
                 const Tile w = tile_at(P, t);
                 const int k0 = (int)((int64_t)P.k_iters * w.share / P.split), k1 = (int)((int64_t)P.k_iters * (w.share + 1) / P.split);
-                const uint32_t buf = n & 1, use = n >> 1, d = tmem_base + buf * kMaxCols;
-                if (!mbar_wait_t<kPair>(&S.tmem_empty[buf], (use & 1) ^ 1, fail)) break;
-                tc_fence_after();
-                for (int k = k0; k < k1; ++k) {
-                    if (!mbar_wait_t<kPair>(&S.full_bar[s], ph, fail)) break;
+                const int part = kParts ? P.part : k1 - k0;
+                for (int p0 = k0; p0 < k1; p0 += part, ++n) {
+                    const int p1 = kParts ? min(p0 + part, k1) : k1;
+                    const uint32_t buf = n & 1, use = n >> 1, d = tmem_base + buf * kMaxCols;
+                    if (!mbar_wait_t<kPair>(&S.tmem_empty[buf], (use & 1) ^ 1, fail)) break;
                     tc_fence_after();
-                    const uint8_t *sa = S.tiles + (size_t)s * stage_bytes, *sb = sa + a_bytes;
-                    const uint64_t da = kMnA ? make_desc_mn(sa) : make_smem_desc(sa), db = kMnB ? make_desc_mn(sb) : make_smem_desc(sb);
+                    for (int k = p0; k < p1; ++k) {
+                        if (!mbar_wait_t<kPair>(&S.full_bar[s], ph, fail)) break;
+                        tc_fence_after();
+                        const uint8_t *sa = S.tiles + (size_t)s * stage_bytes, *sb = sa + a_bytes;
+                        const uint64_t da = kMnA ? make_desc_mn(sa) : make_smem_desc(sa), db = kMnB ? make_desc_mn(sb) : make_smem_desc(sb);
 #pragma unroll
-                    for (int kk = 0; kk < BK / UMMA_K; ++kk) {
-                        const uint64_t a = da + (uint64_t)(kk * (kMnA ? kStepMn : kStepK)), b = db + (uint64_t)(kk * (kMnB ? kStepMn : kStepK));
-                        if (kPair) umma_pair(d, a, b, k != k0 || kk != 0, P.idesc); else umma(d, a, b, k != k0 || kk != 0, P.idesc);
+                        for (int kk = 0; kk < BK / UMMA_K; ++kk) {
+                            const uint64_t a = da + (uint64_t)(kk * (kMnA ? kStepMn : kStepK)), b = db + (uint64_t)(kk * (kMnB ? kStepMn : kStepK));
+                            if (kPair) umma_pair(d, a, b, k != p0 || kk != 0, P.idesc); else umma(d, a, b, k != p0 || kk != 0, P.idesc);
+                        }
+                        if (kPair) umma_commit_pair(&S.empty_bar[s]); else umma_commit(&S.empty_bar[s]);
+                        if (++s == stages) { s = 0; ph ^= 1; }
                     }
-                    if (kPair) umma_commit_pair(&S.empty_bar[s]); else umma_commit(&S.empty_bar[s]);
-                    if (++s == stages) { s = 0; ph ^= 1; }
+                    if (kPair) umma_commit_pair(&S.tmem_full[buf]); else umma_commit(&S.tmem_full[buf]);
+                    if (*fail) break;
                 }
-                if (kPair) umma_commit_pair(&S.tmem_full[buf]); else umma_commit(&S.tmem_full[buf]);
             }
         }
     } else {
         // ------------------------------------------------------------------ epilogue: a warp reaches its TMEM lane quarter.  Single: the two
         // warps of a quarter take half of the columns each.  Pair: they take tiles in turn, one accumulator each, so that one waits for
-        // TMEM while the other stores.
+        // TMEM while the other stores.  In parts: half of the columns each, since a lane has registers for the sums of so many.
+        constexpr bool kTurns = kPair && !kParts;
         const int q4 = warp & 3, group = (warp - 2) >> 2, rl = q4 * 32 + lane;
-        const int mid = (P.cols / 16 + 1) / 2 * 16, half0 = kPair ? 0 : group, halves = kPair ? 2 : 1;
-        const int every = kPair ? 2 : 1;  // tile of this warp
+        const int mid = (P.cols / 16 + 1) / 2 * 16, half0 = kTurns ? 0 : group, halves = kTurns ? 2 : 1;
+        const int every = kTurns ? 2 : 1;  // tile of this warp
         uint8_t *box = S.tiles + kStageSpace - kTurnSpace + (warp - 2) * kTurnWarp;
-        uint32_t n = kPair ? group : 0;
+        uint32_t n = kTurns ? group : 0;
         bool bad = false;
         // This warp has read the accumulator.  Relaxed: the loads are complete, and a release would wait for the results stored so far
         // to reach memory, a microsecond and more on every tile (1531 x 50257 x 1000: scores 153 us, tensor cores busy for 51 %).
@@ -359,36 +379,72 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_loss_gemm(const __grid_cons
         };
         float scale = P.scale;
         if (MODE != SCORES && P.total) scale = *P.total != 0.f ? scale / *P.total : 0.f;
-        for (int t = unit + (int)n * P.units; t < total; t += every * P.units, n += every) {
+        for (int t = unit + (int)n * P.units; t < total; t += every * P.units, n += kParts ? 0 : every) {
             const Tile w = tile_at(P, t);
             const int row = (w.um * kCtas + (int)cta_r) * BM + rl, col0 = w.nt * P.cols;
-            const uint32_t buf = n & 1, use = n >> 1, taddr = tmem_base + buf * kMaxCols + ((uint32_t)(q4 * 32) << 16);
+            const bool rows = row - lane < P.M;  // a warp of rows that do not exist has nothing to do
+            const uint32_t lanes = tmem_base + ((uint32_t)(q4 * 32) << 16);
+            uint32_t buf = n & 1;
             int64_t y = -1;
             if (MODE == SCORES && row < P.M) {
                 const int64_t id = target_of(P.y, P.wide_y, row);
                 if (id != P.ignore) y = id - P.first - col0;  // of this tile's columns; far outside elsewhere
             }
-            bad = bad || !mbar_wait_t<kPair>(&S.tmem_full[buf], use & 1, fail);
-            bad = __any_sync(0xffffffffu, bad);
-            tc_fence_after();
-            if (row - lane >= P.M) {  // a warp of rows that do not exist
-                release(buf);
-                continue;
+            float v[MODE == SCORES && kPair || kParts ? kHalf : 1];
+            if constexpr (kParts) {
+#pragma unroll
+                for (int i = 0; i < kHalf; ++i) v[i] = 0.f;
+                const uint32_t from = lanes + (group ? mid : 0);
+                const int width = group ? P.cols - mid : mid;  // a multiple of 16
+#pragma unroll 1
+                for (int p0 = 0; p0 < P.k_iters; p0 += P.part, ++n) {
+                    buf = n & 1;
+                    bad = bad || !mbar_wait_t<kPair>(&S.tmem_full[buf], (n >> 1) & 1, fail);
+                    bad = __any_sync(0xffffffffu, bad);
+                    tc_fence_after();
+                    const bool end = p0 + P.part >= P.k_iters;
+                    if (rows && !bad) {
+#pragma unroll
+                        for (int c = 0; c < kHalf; c += 16)
+                            if (c < width) {
+                                uint32_t x[16];
+                                tmem_ld16(from + buf * kMaxCols + c, x);
+                                tmem_ld_wait();
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) v[c + i] += __uint_as_float(x[i]);
+                                // single: the code below takes the sums from where the last part was
+                                if (!kPair && end) tmem_st16(from + buf * kMaxCols + c, v + c);
+                            }
+                        if (!kPair && end) asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    }
+                    if (kPair || !end || !rows) release(buf);
+                }
+                if (!rows) continue;
+            } else {
+                bad = bad || !mbar_wait_t<kPair>(&S.tmem_full[buf], (n >> 1) & 1, fail);
+                bad = __any_sync(0xffffffffu, bad);
+                tc_fence_after();
+                if (!rows) {
+                    release(buf);
+                    continue;
+                }
             }
+            const uint32_t taddr = lanes + buf * kMaxCols;
 #pragma unroll 1
             for (int half = half0; half < half0 + halves; ++half) {
                 const int c_lo = half ? mid : 0, c_hi = half ? P.cols : mid;
                 const bool last = half == half0 + halves - 1;  // the accumulator is free when its last half is read
-                if (MODE == SCORES) {
+                if constexpr (MODE == SCORES) {
                     const int exist = min(c_hi, P.N - col0) - c_lo;  // columns of this half that exist, the first of them
                     const int room = (int)min((int64_t)c_hi, P.width - col0) - c_lo;  // the row ends on a multiple of 32, in zeros
                     const int yl = y >= c_lo && y < c_lo + exist ? (int)y - c_lo : -1;
                     __half *e = P.e + (int64_t)row * P.ld + col0 + c_lo;
                     float m = -INFINITY, z = 0.f;
                     if constexpr (kPair) {
-                        float v[kHalf];
-                        if (!bad) tmem_half(taddr + c_lo, v);
-                        if (last) release(buf);
+                        if constexpr (!kParts) {
+                            if (!bad) tmem_half(taddr + c_lo, v);
+                            if (last) release(buf);
+                        }
                         if (exist < kHalf)
 #pragma unroll
                             for (int i = 0; i < kHalf; ++i) v[i] = i < exist ? v[i] : -INFINITY;
@@ -820,11 +876,12 @@ __global__ void __launch_bounds__(32 * kShareSlices) vocab_loss_shares(const __g
 }
 
 // ---------------------------------------------------------------------------------------------------- launches
-const void *gemm_of(int mode, bool pair)
+const void *gemm_of(int mode, bool pair, bool parts)
 {
-    if (mode == SCORES) return pair ? (const void *)vocab_loss_gemm<SCORES, true> : (const void *)vocab_loss_gemm<SCORES, false>;
-    if (mode == DX) return pair ? (const void *)vocab_loss_gemm<DX, true> : (const void *)vocab_loss_gemm<DX, false>;
-    return pair ? (const void *)vocab_loss_gemm<DW, true> : (const void *)vocab_loss_gemm<DW, false>;
+    if (mode == SCORES && parts) return pair ? (const void *)vocab_loss_gemm<SCORES, true, true> : (const void *)vocab_loss_gemm<SCORES, false, true>;
+    if (mode == SCORES) return pair ? (const void *)vocab_loss_gemm<SCORES, true, false> : (const void *)vocab_loss_gemm<SCORES, false, false>;
+    if (mode == DX) return pair ? (const void *)vocab_loss_gemm<DX, true, false> : (const void *)vocab_loss_gemm<DX, false, false>;
+    return pair ? (const void *)vocab_loss_gemm<DW, true, false> : (const void *)vocab_loss_gemm<DW, false, false>;
 }
 
 struct LossDevice { int sms = 0, pairs = 0; };
@@ -842,8 +899,8 @@ HcclResult loss_device(LossDevice *out)
         int sms = 0, pairs = 0;
         cudaError_t e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
         for (int mode = SCORES; mode <= DW && e == cudaSuccess; ++mode)
-            for (int pair = 0; pair < 2 && e == cudaSuccess; ++pair)
-                e = cudaFuncSetAttribute(gemm_of(mode, pair), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes);
+            for (int form = 0; form < 4 && e == cudaSuccess; ++form)
+                e = cudaFuncSetAttribute(gemm_of(mode, form & 1, form >> 1), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes);
         if (e == cudaSuccess) {
             cudaLaunchConfig_t q;
             memset(&q, 0, sizeof(q));
@@ -852,7 +909,7 @@ HcclResult loss_device(LossDevice *out)
             at[0].id = cudaLaunchAttributeClusterDimension;
             at[0].val.clusterDim.x = 2; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
             q.attrs = at; q.numAttrs = 1;
-            e = cudaOccupancyMaxActiveClusters(&pairs, gemm_of(SCORES, true), &q);
+            e = cudaOccupancyMaxActiveClusters(&pairs, gemm_of(SCORES, true, false), &q);
         }
         if (e != cudaSuccess || pairs < 1) { HLOG_ERROR("vocabulary loss set-up failed: %s", cudaGetErrorString(e)); return HCCL_E_RUNTIME; }
         d.pairs = std::min(pairs, sms / 2);
@@ -946,9 +1003,11 @@ HcclResult launch_gemm(int mode, bool pair, LossGemm &P, void *stream)
     P.idesc = instr_desc((uint32_t)(ctas * BM), (uint32_t)P.cols) | (mode == DW ? 1u << 15 : 0u) | (mode != SCORES ? 1u << 16 : 0u);
     // a panel's columns of B stay in L2 (40 MB of it) while the rows stream past
     P.panel = (int)std::min<int64_t>(P.n_tiles, std::max<int64_t>(8, (40ll << 20) / ((int64_t)P.cols * P.k_iters * BK * 2)));
+    const int parts = mode == SCORES ? std::max(1, P.k_iters / (pair ? kPartLeast<true> : kPartLeast<false>)) : 1;
+    P.part = (P.k_iters + parts - 1) / parts;
     const int64_t total = (int64_t)P.um_tiles * P.n_tiles * P.split;
     CHK_RET_LOG(total > INT32_MAX / 2, HCCL_E_PARA, "vocabulary loss: too many tiles");
-    return launch_pdl(gemm_of(mode, pair), dim3((unsigned)(std::min<int64_t>(P.units, total) * ctas)), kThreads, kSmemBytes, &P, stream, "vocabulary loss", ctas);
+    return launch_pdl(gemm_of(mode, pair, parts > 1), dim3((unsigned)(std::min<int64_t>(P.units, total) * ctas)), kThreads, kSmemBytes, &P, stream, "vocabulary loss", ctas);
 }
 
 RowArgs row_args(const VocabLossCall &c)
