@@ -4,7 +4,6 @@
 #pragma once
 #include <cuda_runtime.h>
 #include <cstdint>
-#include <map>
 #include <mutex>
 #include "common/log.h"
 
@@ -12,16 +11,18 @@ namespace hcclb {
 
 inline HcclResult grant_smem(const void *fn, size_t most, const char *what)
 {
+    struct Kernel { const void *fn; uint64_t devices; };  // devices: a bit for each that has the grant
     static std::mutex mu;
-    static std::map<const void *, uint64_t> granted;  // a bit for each device
+    static Kernel known[128];
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return HCCL_E_RUNTIME;
     std::lock_guard<std::mutex> lk(mu);
-    uint64_t &devices = granted[fn];
-    if (devices >> dev & 1) return HCCL_SUCCESS;
+    Kernel *k = known;
+    while (k < known + 128 && k->fn && k->fn != fn) ++k;  // beyond the table a kernel is granted the same anew, which changes nothing
+    if (k < known + 128 && k->fn == fn && (k->devices >> dev & 1)) return HCCL_SUCCESS;
     const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
     CHK_RET_LOG(e != cudaSuccess, HCCL_E_RUNTIME, "%s set-up failed: %s", what, cudaGetErrorString(e));
-    devices |= 1ull << dev;
+    if (k < known + 128) { k->fn = fn; k->devices |= 1ull << dev; }
     return HCCL_SUCCESS;
 }
 

@@ -4,6 +4,7 @@ import ctypes as C
 import pytest
 
 torch = pytest.importorskip("torch")
+import cann_hccl_b200 as H  # noqa: E402
 from cann_hccl_b200 import _lib as L  # noqa: E402
 from cann_hccl_b200.parallel import vocab  # noqa: E402
 from test_gpu_vocab_loss import Exact, problem  # noqa: E402
@@ -79,3 +80,30 @@ def test_two_chunks_as_they_come(monkeypatch):
     assert torch.equal(acc.to(torch.bfloat16), dw) and bool((guard == 3).all())
     # the same fp32 sums of `chunk + rest` losses in another order
     assert abs(float(loss) - sum(losses)) <= 2.0 ** -24 * (2 * (chunk + rest) / 256 + 32) * sum(losses)
+
+
+@pytest.mark.parametrize("p,chunk", [(2, 128), (3, 256)])
+def test_chunks_over_shards(p, chunk, monkeypatch):
+    """Several chunks of tokens, each exchanged between the ranks; the last one short."""
+    cfg = L.CommConfig.default()
+    cfg.hcclBufferSize = 2
+    c = H.Communicator.init_local(p, device=True, device_id=0, config=cfg)
+    T, V, hidden = 2 * chunk + 131, 700 * p, 1096
+    x, w, y = problem(T, V, hidden)
+    weights = torch.rand(T, device="cuda")
+    weights[::7] = 0
+    monkeypatch.setattr(L.lib(), "HcclB200VocabLossChunk", lambda v, g: chunk)
+    e = Exact(x, w, y, weights)
+    shards = [s.contiguous() for s in w.chunk(p)]
+    args = (c, [x] * p, shards, [y] * p, [weights] * p)
+    out = vocab.vocab_parallel_cross_entropy_grad(*args)
+    acc = [torch.zeros(700, hidden, device="cuda") for _ in range(p)]
+    added = vocab.vocab_parallel_cross_entropy_grad(*args, dw=acc)
+    losses = vocab.vocab_parallel_cross_entropy(*args, reduction="none")
+    assert c.sync() == 0, c.describe_status()
+    e.check((out[0][0], out[0][1], torch.cat([o[2] for o in out])), parts=p)
+    e.check((added[0][0], added[0][1], torch.cat(acc)), torch.float32, parts=p)
+    for r in range(p):
+        e.check_losses(losses[r])
+        assert torch.equal(out[r][0], out[0][0]) and torch.equal(out[r][1], out[0][1])
+    c.destroy()
